@@ -170,6 +170,11 @@ extern "C" {
     pub fn ruai_dequant_int4(ctx: *mut ruai_ctx, w: *const ruai_qweight, out_dev: *mut f32) -> c_int;
     pub fn ruai_dequant_int4_ref(ctx: *mut ruai_ctx, q_dev: *const i8, scale_dev: *const f32, k: u32, n: u32, group: u32, out_dev: *mut f32) -> c_int;
 
+    // ---- a cache in pages ----
+    pub fn ruai_page_plan(ctx: *mut ruai_ctx, cached_dev: *const i32, fresh_dev: *const i32, r: u32, tokens: u32, page: u32, table_dev: *mut i32, table_ld: u32, ring_dev: *mut i32, pages: u32, words_in_dev: *const i32, words_out_dev: *mut i32, starts_dev: *mut i32, positions_dev: *mut i32, slots_dev: *mut i32) -> c_int;
+    pub fn ruai_paged_append(ctx: *mut ruai_ctx, x_dtype: c_int, x_dev: *const c_void, ld: u32, k_off: u32, v_off: u32, tokens: u32, h: u32, rot: u32, rope_dev_or_null: *const f32, max_pos: u32, positions_dev: *const i32, slots_dev: *const i32, dtype: c_int, k_pages_dev: *mut c_void, v_pages_dev: *mut c_void, pages: u32, kv: u32, page: u32, hd: u32, q_out_dev_or_null: *mut c_void, q_ld: u32) -> c_int;
+    pub fn ruai_paged_attention(ctx: *mut ruai_ctx, dtype: c_int, q_dev: *const c_void, q_ld: u32, k_pages_dev: *const c_void, v_pages_dev: *const c_void, pages: u32, kv: u32, page: u32, hd: u32, table_dev: *const i32, table_ld: u32, cached_dev: *const i32, starts_dev: *const i32, r: u32, tokens: u32, h: u32, scale: f32, window: u32, most_fresh: u32, most_len: u32, out_dev: *mut c_void, out_ld: u32) -> c_int;
+
     // ---- models ----
     pub fn ruai_llama_create(ctx: *mut ruai_ctx, cfg: *const ruai_llama_config, tp_or_null: *const ruai_tp, out: *mut *mut ruai_model) -> c_int;
     pub fn ruai_gpt2_create(ctx: *mut ruai_ctx, cfg: *const ruai_gpt2_config, out: *mut *mut ruai_model) -> c_int;

@@ -192,6 +192,44 @@ int ruai_dequant_int4(ruai_ctx* ctx, const ruai_qweight* w, float* out_dev);
 int ruai_dequant_int4_ref(ruai_ctx* ctx, const int8_t* q_dev, const float* scale_dev,
                           uint32_t k, uint32_t n, uint32_t group, float* out_dev);
 
+/* ---- a cache in pages --------------------------------------------------------
+ * Requests of different lengths hold pages of one pool: keys and values [pages, KV, page, hd] in f32, f16 or bf16, `page` a
+ * power of two from 16 to 256, hd a multiple of 8 up to 256.  table[r][i] is the page that holds positions i * page .. of
+ * request r.  Free pages wait in a ring of `pages` entries; words[0] is the first one's place, words[1] their number.  A page
+ * belongs to one request.  All of it lives in device memory, and so do the requests' lengths: nothing here waits for the host.
+ * Indices out of range are never followed: what they belong to is left out and the next ruai_ctx_synchronize reports
+ * RUAI_ERR_SHAPE.  The reference keeps one contiguous buffer per batch (KvBuf, transformer.rs:10-53). */
+
+/* Block tables and slots of a step.  Request r < R has cached[r] positions in its pages and brings fresh[r] new tokens
+ * (0: none this time; negative: it has ended and its pages go back, to be given out from the next plan on).  Written: the new
+ * entries of table, ring, starts[R + 1] (the tokens of request r are rows starts[r] .. starts[r + 1] - 1 of the step), and for
+ * each of `tokens` rows its position and slot (page * page size + offset; -1 for rows behind the last token), words_out[3]:
+ * the first two as above, and how many pages were missing.  With pages missing, or lengths that do not fit the table or
+ * `tokens`, nothing is planned: starts are 0, positions and slots -1, table and ring as they were, and the next
+ * ruai_ctx_synchronize fails.  words_out may be words_in; another buffer keeps the old words, with which a step can be planned
+ * again.  R up to 8192, tokens up to 262144. */
+int ruai_page_plan(ruai_ctx* ctx, const int32_t* cached_dev, const int32_t* fresh_dev, uint32_t R, uint32_t tokens, uint32_t page,
+                   int32_t* table_dev, uint32_t table_ld, int32_t* ring_dev, uint32_t pages, const int32_t* words_in_dev,
+                   int32_t* words_out_dev, int32_t* starts_dev, int32_t* positions_dev, int32_t* slots_dev);
+/* KvBuf::append and apply_rope (transformer.rs:27-53, functional.rs:197-204) of a step's rows: row t of x [tokens, ld] holds H
+ * query heads, KV key heads from column k_off and KV value heads from v_off.  Keys and values go to slots[t] (negative: the row
+ * is left out), queries to row t of q_out [tokens, q_ld], all in the pages' type; q_out may be x itself where the types are
+ * equal, or NULL.  With rope [max_pos, rot / 2] (cos, sin), elements i and i + rot / 2 of every query and key head turn by the
+ * angle of positions[t]; rot a multiple of 8 up to hd.  Computed in f32, rounded once. */
+int ruai_paged_append(ruai_ctx* ctx, int x_dtype, const void* x_dev, uint32_t ld, uint32_t k_off, uint32_t v_off, uint32_t tokens,
+                      uint32_t H, uint32_t rot, const float* rope_dev_or_null, uint32_t max_pos, const int32_t* positions_dev,
+                      const int32_t* slots_dev, int dtype, void* k_pages_dev, void* v_pages_dev, uint32_t pages, uint32_t KV,
+                      uint32_t page, uint32_t hd, void* q_out_dev_or_null, uint32_t q_ld);
+/* Scaled dot-product attention (functional.rs:264-296) of a step's new tokens over their requests' pages, which hold their keys
+ * and values already: token i of request r sits at position p = cached[r] + i and sees positions p - window + 1 .. p (window 0:
+ * 0 .. p).  q [tokens, q_ld] and out [tokens, out_ld] are of the pages' type; rows behind the last token stay as they were.
+ * Scores, softmax and sums are f32.  most_fresh and most_len are bounds on a request's new tokens and on its length with them; they
+ * choose the kernels, and a request beyond them is left out (reported as above).  H / KV up to 256, H up to 8191. */
+int ruai_paged_attention(ruai_ctx* ctx, int dtype, const void* q_dev, uint32_t q_ld, const void* k_pages_dev, const void* v_pages_dev,
+                         uint32_t pages, uint32_t KV, uint32_t page, uint32_t hd, const int32_t* table_dev, uint32_t table_ld,
+                         const int32_t* cached_dev, const int32_t* starts_dev, uint32_t R, uint32_t tokens, uint32_t H, float scale,
+                         uint32_t window, uint32_t most_fresh, uint32_t most_len, void* out_dev, uint32_t out_ld);
+
 /* ---- models ---------------------------------------------------------------- */
 
 /* Field names follow `LlamaConfig` (llama.rs:48-75). */

@@ -95,6 +95,9 @@ _PROTOS = {
     "ruai_ctx_force_tile": (C.c_int, [vp, C.c_uint, C.c_uint]),
     "ruai_dequant_int4": (C.c_int, [vp, vp, vp]),
     "ruai_dequant_int4_ref": (C.c_int, [vp, vp, vp, u32, u32, u32, vp]),
+    "ruai_page_plan": (C.c_int, [vp, vp, vp, u32, u32, u32, vp, u32, vp, u32, vp, vp, vp, vp, vp]),
+    "ruai_paged_append": (C.c_int, [vp, C.c_int, vp, u32, u32, u32, u32, u32, u32, vp, u32, vp, vp, C.c_int, vp, vp, u32, u32, u32, u32, vp, u32]),
+    "ruai_paged_attention": (C.c_int, [vp, C.c_int, vp, u32, vp, vp, u32, u32, u32, u32, vp, u32, vp, vp, u32, u32, u32, C.c_float, u32, u32, u32, vp, u32]),
     "ruai_llama_create": (C.c_int, [vp, C.POINTER(LlamaConfig), C.POINTER(TP), C.POINTER(vp)]),
     "ruai_gpt2_create": (C.c_int, [vp, C.POINTER(GPT2Config), C.POINTER(vp)]),
     "ruai_hybrid_create": (C.c_int, [vp, C.POINTER(HybridConfig), C.POINTER(LayerConfig), C.POINTER(vp)]),

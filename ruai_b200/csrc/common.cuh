@@ -37,7 +37,7 @@ struct ruai_ctx {
   unsigned force_cols = 0, force_rows = 0;  // debug: the same for the prefill GEMM's tile
   unsigned long long* trace = nullptr;  // debug: per-launch [first entry, first past the dependency wait, last exit] in ns
   unsigned trace_slots = 0, trace_seq = 0;
-  int* status = nullptr;  // device word: 0 ok, 3 / 4 = a bounded wait inside a kernel ran out (mbarrier / grid barrier), 5 = cache position out of range
+  int* status = nullptr;  // device word: 0 ok, 3 / 4 = a bounded wait inside a kernel ran out (mbarrier / grid barrier), 5 = cache position out of range, 6 / 7 = a page plan refused / a paged cache's index out of range (paged.cuh)
   unsigned long long launches = 0;
   // persistent kernels (pstep.cu)
   unsigned spin_limit = 1u << 20;  // polls of a bounded device-side wait (about a second)

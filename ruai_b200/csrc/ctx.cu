@@ -129,6 +129,8 @@ int ruai_ctx_status_result(ruai_ctx* c, int st) {
     c->ps_bar_base = 0;
   }
   if (st == 5) return ruai_fail(c, RUAI_ERR_SHAPE, "a decode step was launched at a position beyond the cache capacity; nothing was written there");
+  if (st == 6) return ruai_fail(c, RUAI_ERR_SHAPE, "a page plan was refused: too few free pages, or lengths that do not fit the table or the buffers; nothing was planned");
+  if (st == 7) return ruai_fail(c, RUAI_ERR_SHAPE, "a page, slot, position or length of a paged cache was out of range; what it belongs to was left out");
   return ruai_fail(c, RUAI_ERR_TIMEOUT, "a bounded wait inside a kernel ran out (status %d); results of that launch are invalid", st);
 }
 

@@ -10,6 +10,7 @@ nothing here computes on the host.
 """
 import ctypes as C
 import math
+from typing import NamedTuple
 
 import numpy as np
 
@@ -237,6 +238,97 @@ class Sampler:
         logits.dev.check(logits.dev.L.ruai_sample(logits.dev.ctx, logits.ptr, logits.shape[0], self.temperature, self.top_k, self.top_p,
                                                   C.byref(self.state), C.byref(tok)))
         return int(tok.value)
+
+
+class PagePlan(NamedTuple):
+    """What `page_plan` writes: where each request's rows begin, the rows' positions and slots, the pool's words."""
+    starts: Tensor     # int32 [R + 1]
+    positions: Tensor  # int32 [tokens]
+    slots: Tensor      # int32 [tokens]
+    words: Tensor      # int32 [3]: place of the first free page in the ring, free pages, missing pages
+
+
+def _ints(name, t, shape):
+    if t.np_dtype != np.int32 or t.shape != shape:
+        raise ValueError(f"{name} must be int32 {list(shape)}, got {t.np_dtype} {list(t.shape)}")
+
+
+def _same_device(dev, *tensors):
+    if any(t is not None and t.dev.ordinal != dev.ordinal for t in tensors):
+        raise ValueError("tensors of different devices")
+
+
+def _pages(k, v):
+    if len(k.shape) != 4 or k.shape != v.shape or k.rdtype is None or k.rdtype != v.rdtype:
+        raise ValueError(f"pages must be two float tensors [pages, kv_heads, page, dim], got {list(k.shape)} and {list(v.shape)}")
+    return k.shape
+
+
+def page_plan(cached, fresh, table, ring, words, page, tokens=None, out=None):
+    """Block tables and slots of a step over a cache in pages (see `ruai_page_plan`): request r has cached[r] positions and
+    brings fresh[r] new tokens, or has ended (negative).  `tokens` is the number of the step's rows, padding included."""
+    dev = cached.dev
+    R, pages = cached.shape[0], ring.shape[0]
+    if out is None:
+        if tokens is None:
+            raise ValueError("page_plan: the step's number of rows is needed where no buffers are given")
+        out = PagePlan(Tensor(dev, (R + 1,), np.int32), Tensor(dev, (tokens,), np.int32), Tensor(dev, (tokens,), np.int32), Tensor(dev, (3,), np.int32))
+    tokens = out.slots.shape[0] if tokens is None else int(tokens)
+    if len(table.shape) != 2 or len(ring.shape) != 1:
+        raise ValueError("table must be [requests, pages] and ring [pages]")
+    for name, t, shape in (("cached", cached, (R,)), ("fresh", fresh, (R,)), ("table", table, (R, table.shape[1])), ("ring", ring, (pages,)), ("words", words, (3,)),
+                           ("starts", out.starts, (R + 1,)), ("positions", out.positions, (tokens,)), ("slots", out.slots, (tokens,)), ("words", out.words, (3,))):
+        _ints(name, t, shape)
+    _same_device(dev, fresh, table, ring, words, *out)
+    dev.check(dev.L.ruai_page_plan(dev.ctx, cached.ptr, fresh.ptr, R, tokens, page, table.ptr, table.shape[1], ring.ptr, pages, words.ptr, out.words.ptr, out.starts.ptr,
+                                   out.positions.ptr, out.slots.ptr))
+    return out
+
+
+def paged_append(qkv, positions, slots, k_pages, v_pages, rope=None, out=None):
+    """Keys and values of qkv [tokens, (heads + 2 kv_heads) dim] into their slots, queries [tokens, heads, dim] as result, in
+    the pages' type; with rope [positions, rot / 2, 2] (cos, sin) queries and keys are rotated (see `ruai_paged_append`)."""
+    pages, kv, page, dim = _pages(k_pages, v_pages)
+    dev = qkv.dev
+    if qkv.rdtype is None or len(qkv.shape) != 2 or qkv.shape[1] % dim or qkv.shape[1] // dim <= 2 * kv:
+        raise ValueError(f"qkv must be a float tensor [tokens, (heads + {2 * kv}) * {dim}], got {list(qkv.shape)}")
+    tokens, heads = qkv.shape[0], qkv.shape[1] // dim - 2 * kv
+    _ints("positions", positions, (tokens,))
+    _ints("slots", slots, (tokens,))
+    if rope is not None and (rope.rdtype != F32 or len(rope.shape) != 3 or rope.shape[2] != 2):
+        raise ValueError("rope must be f32 [positions, rot / 2, 2]")
+    if out is None:
+        out = Tensor(dev, (tokens, heads, dim), k_pages.np_dtype, k_pages.rdtype)
+    if out.rdtype != k_pages.rdtype or out.shape != (tokens, heads, dim):
+        raise ValueError(f"out must be [{tokens}, {heads}, {dim}] of the pages' type")
+    _same_device(dev, positions, slots, k_pages, v_pages, rope, out)
+    dev.check(dev.L.ruai_paged_append(dev.ctx, qkv.rdtype, qkv.ptr, qkv.shape[1], heads * dim, (heads + kv) * dim, tokens, heads, 2 * rope.shape[1] if rope is not None else 0,
+                                      rope.ptr if rope is not None else None, rope.shape[0] if rope is not None else 0, positions.ptr, slots.ptr, k_pages.rdtype, k_pages.ptr,
+                                      v_pages.ptr, pages, kv, page, dim, out.ptr, heads * dim))
+    return out
+
+
+def paged_attention(q, k_pages, v_pages, table, cached, starts, most_fresh, most_len, scale=None, window=0, out=None):
+    """Causal attention of each request's new tokens, rows starts[r] .. of q [tokens, heads, dim], over its pages (see
+    `ruai_paged_attention`).  No request brings more than most_fresh tokens or is longer than most_len with them."""
+    pages, kv, page, dim = _pages(k_pages, v_pages)
+    dev = q.dev
+    if q.rdtype != k_pages.rdtype or len(q.shape) != 3 or q.shape[2] != dim:
+        raise ValueError(f"q must be [tokens, heads, {dim}] of the pages' type, got {list(q.shape)}")
+    tokens, heads, _ = q.shape
+    R = cached.shape[0]
+    if len(table.shape) != 2:
+        raise ValueError("table must be [requests, pages]")
+    for name, t, shape in (("table", table, (R, table.shape[1])), ("cached", cached, (R,)), ("starts", starts, (R + 1,))):
+        _ints(name, t, shape)
+    if out is None:
+        out = Tensor(dev, q.shape, q.np_dtype, q.rdtype)
+    if out.rdtype != q.rdtype or out.shape != q.shape:
+        raise ValueError(f"out must be {list(q.shape)} of the pages' type")
+    _same_device(dev, k_pages, v_pages, table, cached, starts, out)
+    dev.check(dev.L.ruai_paged_attention(dev.ctx, q.rdtype, q.ptr, heads * dim, k_pages.ptr, v_pages.ptr, pages, kv, page, dim, table.ptr, table.shape[1], cached.ptr, starts.ptr, R,
+                                         tokens, heads, dim ** -0.5 if scale is None else float(scale), int(window), int(most_fresh), int(most_len), out.ptr, heads * dim))
+    return out
 
 
 def matmul_q_stream(x, w, repeat=1):
