@@ -1,52 +1,71 @@
 // Causal attention of every request's new tokens over its pages: softmax(scale q k^T + mask) v, where the token at position p sees
 // keys p - window + 1 .. p (window 0: all of 0 .. p).
 //
-// One warp per (token, query head), a key at a time: the running maximum m, sum l and weighted values o of a softmax in f32,
-// o <- o e^(m - m') + e^(s - m') v.
+// rows_kernel: single tokens, drafts of a few, and whatever the kernels for chunks do not take.  The rows of an item are the (token,
+// query head) pairs of one request and key head, 16 WR of them, so that a cached row is read once for all query heads of its key
+// head.  HBM bounds it; an item's keys pass through once, in tiles of TK, with a running maximum m, sum l and weighted values o per row:
+// o <- o 2^(m - m') + 2^(s - m') v, in f32 registers.
+//   Split: the tiles of all items, in a row, are cut into equal runs, one per CTA, whatever the requests' lengths are (they are known to the
+// device only).  An item cut by a run's end leaves (m, l, o) of its part in scratch, and the CTA that arrives last joins the parts, in
+// their order: the same bits every time.
+//   Tile: four warps; WK = 4 / WR of them share an item's rows and take a part of the tile's keys each.  cp.async copies into padded
+// rows a few tiles ahead (rows behind the request's end arrive as zeros).  Products are mma.sync: the tensor pipe waits for HBM here, and 16 rows
+// by 8 keys fit few query heads where a tcgen05 tile would be a sixteenth full.  f32 operands are split in two tf32 numbers, x = hi + lo
+// (22 bits), three of the four products; the
+// tensor core's sums truncate, so it adds up 32 elements of a score and a tile's keys only, f32 registers the rest.  In 16 bits the weights are rounded once, to the values' type; l sums them unrounded.
+//   A row that is not finite at the end is worked out again key by key (row_again): a key that it does not see, or that weighs
+// nothing, must not reach it through 0 x inf.
+#include <algorithm>
+
 #include "paged.cuh"
+#include "pipeline.cuh"
 
 namespace {
 
-constexpr int kHeadParts = 8;  // elements of a head per lane: heads of up to 256
+using pipe::smem_u32;
 
-template <typename T>
-__global__ void __launch_bounds__(256) one_row_kernel(const PagedAttn a) {
-  grid_dependency_wait();
-  grid_launch_dependents();
-  const uint32_t lane = threadIdx.x & 31u, row = blockIdx.x * 8 + (threadIdx.x >> 5), hd = a.pool.hd;
-  if (row >= a.tokens * a.H) return;
-  const uint32_t t = row / a.H, head = row % a.H, g = head / (a.H / a.pool.KV);
-  uint32_t lo = 0, hi = a.R;  // the last request that starts at or before t
-  while (hi - lo > 1) {
-    const uint32_t mid = (lo + hi) >> 1;
-    if (a.starts[mid] <= (int32_t)t) lo = mid;
-    else hi = mid;
-  }
+constexpr int kHeadParts = 8;  // elements of a head per lane: heads of up to 256
+constexpr float kLog2e = 1.44269504088896341f;
+
+__device__ __forceinline__ float exp2_of(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// What a CTA does with one item: keys of tiles [tile0, tile1) for rows [row0, row0 + rows) of (request r, key head g).
+struct Segment {
   PagedRequest rq;
-  if (!paged_request(a, lo, rq) || t < rq.t0 || t - rq.t0 >= rq.fresh) return;
-  const uint32_t pos = rq.cached + t - rq.t0;
+  uint32_t r, g, row0, rows, tile0, tile1;
+};
+
+// One row over keys [k0, k1) by a warp, a key at a time; m and scores in powers of two, o not divided by l.
+template <typename T>
+__device__ void row_again(const PagedAttn& a, const Segment& s, uint32_t rep, uint32_t row, uint32_t k0, uint32_t k1, float* o_out, float& m_out, float& l_out) {
+  const uint32_t lane = threadIdx.x & 31u, hd = a.pool.hd, i = row / rep, pos = s.rq.cached + i;
+  const T* qs = static_cast<const T*>(a.q) + (size_t)(s.rq.t0 + i) * a.q_ld + (size_t)(s.g * rep + row % rep) * hd;
   float q[kHeadParts], o[kHeadParts], m = -INFINITY, l = 0.0f;
 #pragma unroll
   for (int j = 0; j < kHeadParts; ++j) {
     const uint32_t e = lane + 32u * j;
-    q[j] = e < hd ? to_f32<T>(static_cast<const T*>(a.q)[(size_t)t * a.q_ld + head * hd + e]) : 0.0f;
+    q[j] = e < hd ? to_f32<T>(qs[e]) : 0.0f;
     o[j] = 0.0f;
   }
-  for (uint32_t k = paged_low(pos, a.window); k <= pos; ++k) {
-    const int32_t pg = paged_page(a, lo, k);
+  for (uint32_t k = max(k0, paged_low(pos, a.window)); k < min(k1, pos + 1); ++k) {
+    const int32_t pg = paged_page(a, s.r, k);
     if (pg < 0) continue;
-    const size_t at = ((((size_t)pg * a.pool.KV + g) << a.pool.page_log2) + (k & ((1u << a.pool.page_log2) - 1u))) * hd;
-    float s = 0.0f;
+    const size_t at = ((((size_t)pg * a.pool.KV + s.g) << a.pool.page_log2) + (k & ((1u << a.pool.page_log2) - 1u))) * hd;
+    float d = 0.0f;
 #pragma unroll
     for (int j = 0; j < kHeadParts; ++j) {
       const uint32_t e = lane + 32u * j;
-      if (e < hd) s = fmaf(q[j], to_f32<T>(static_cast<const T*>(a.pool.k)[at + e]), s);
+      if (e < hd) d = fmaf(q[j], to_f32<T>(static_cast<const T*>(a.pool.k)[at + e]), d);
     }
 #pragma unroll
-    for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, off);
-    s *= a.scale;
-    if (s == -INFINITY) continue;
-    const float m_new = fmaxf(m, s), corr = m == -INFINITY ? 0.0f : expf(m - m_new), pr = expf(s - m_new);
+    for (int off = 16; off > 0; off >>= 1) d += __shfl_xor_sync(0xFFFFFFFFu, d, off);
+    d *= a.scale * kLog2e;
+    if (d == -INFINITY) continue;
+    const float m_new = fmaxf(m, d), corr = m == -INFINITY ? 0.0f : exp2_of(m - m_new), pr = exp2_of(d - m_new);
     l = fmaf(l, corr, pr);
     m = m_new;
 #pragma unroll
@@ -58,16 +77,533 @@ __global__ void __launch_bounds__(256) one_row_kernel(const PagedAttn a) {
 #pragma unroll
   for (int j = 0; j < kHeadParts; ++j) {
     const uint32_t e = lane + 32u * j;
-    if (e < hd) static_cast<T*>(a.out)[(size_t)t * a.out_ld + head * hd + e] = from_f32<T>(l == 0.0f ? 0.0f : o[j] / l);
+    if (e < hd) o_out[e] = o[j];
   }
+  m_out = m;
+  l_out = l;
+}
+
+// ---- products ---------------------------------------------------------------------------------------------------------------
+
+template <typename T> __device__ __forceinline__ void mma16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <> __device__ __forceinline__ void mma16<__half>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <> __device__ __forceinline__ void mma16<__nv_bfloat16>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma8(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// x = hi + lo, each of 11 bits (lo's last ones are cut by the tensor core)
+__device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) {
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(x));
+  lo = __float_as_uint(x - __uint_as_float(hi));
+}
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+__device__ __forceinline__ void ldmatrix4t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b);
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// 16 bytes into shared memory; zeros where `take` is false.
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool take) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(take ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// ---- the kernel ---------------------------------------------------------------------------------------------------------------
+
+constexpr int kThreads = 128;
+
+// HP: the head's width, up to 64, 128 or 256.  WR: warps that have rows of their own.
+template <typename T, int HP, int WR>
+struct Shape {
+  static constexpr bool F32 = sizeof(T) == 4;
+  static constexpr int WK = 4 / WR, RB = 16 * WR, TK = F32 ? 32 : 64, KW = TK / WK;
+  static constexpr int PITCH = HP * (int)sizeof(T) + 16;  // bytes of a row in shared memory: eight rows of a column in eight banks of 16 bytes
+  static constexpr int STAGE = 2 * TK * PITCH;
+  static constexpr bool QSMEM = F32 || HP == 256;          // queries in shared memory, not in registers
+  static constexpr int QBYTES = QSMEM ? RB * PITCH : 0;
+  static constexpr int MERGE = 4 * 16 * (HP + 4) * 4;     // the warps' results at the end, in the tiles' place
+  static constexpr int STAGES = 3 * STAGE + QBYTES <= 110 * 1024 ? 3 : 2;
+  static constexpr int SMEM = STAGES * STAGE + QBYTES;
+  static_assert(MERGE <= STAGES * STAGE, "the results fit the tiles");
+  static constexpr size_t PART = (size_t)RB * (HP + 2) * sizeof(float);  // one part of an item in scratch
+};
+
+struct RowsPlan {
+  float* parts;        // [CTAs][2]: the part that ends the item a CTA begins with, the part that begins the one it ends with
+  unsigned* arrived;   // per CTA in which a cut item begins; zero between launches
+  uint32_t rows_most;  // requests with more rows are another kernel's
+  uint32_t tiles_least;
+};
+
+template <typename T, int HP, int WR>
+__global__ void __launch_bounds__(kThreads, 2) rows_kernel(const PagedAttn a, const RowsPlan plan) {
+  using S = Shape<T, HP, WR>;
+  constexpr int WK = S::WK, RB = S::RB, TK = S::TK, KW = S::KW, PITCH = S::PITCH, NS = TK / 16;
+  extern __shared__ __align__(128) unsigned char smem[];
+  __shared__ unsigned long long s_part[4], s_base;
+  __shared__ uint32_t s_r, s_last;
+  __shared__ float s_m[4][16], s_l[4][16];
+  const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g4 = lane >> 2, t4 = lane & 3;
+  const uint32_t hd = a.pool.hd, KV = a.pool.KV, rep = a.H / KV, plog = a.pool.page_log2, pmask = (1u << plog) - 1u;
+  const uint32_t wr = WR == 1 ? 0 : warp % WR, wk = warp / WR;
+  const float c = a.scale * kLog2e;
+  unsigned char* qsm = smem + S::STAGES * S::STAGE;
+  grid_dependency_wait();
+  grid_launch_dependents();
+
+  // ---- which tiles of which items
+  auto tiles_of = [&](const PagedRequest& q) { return (q.len + TK - 1) / TK - paged_low(q.cached, a.window) / TK; };
+  auto units_of = [&](const PagedRequest& q) -> unsigned long long {
+    const uint32_t rows = q.fresh * rep;
+    return rows == 0 || rows > plan.rows_most ? 0ull : (unsigned long long)(KV * ((rows + RB - 1) / RB)) * tiles_of(q);
+  };
+  const uint32_t per_thread = (a.R + kThreads - 1) / kThreads, ra = min(tid * per_thread, a.R), rb = min(ra + per_thread, a.R);
+  unsigned long long mine = 0;
+  for (uint32_t r = ra; r < rb; ++r) {
+    PagedRequest q;
+    paged_request(a, r, q);
+    mine += units_of(q);
+  }
+  unsigned long long inc = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const unsigned long long v = __shfl_up_sync(0xFFFFFFFFu, inc, o);
+    if (lane >= (uint32_t)o) inc += v;
+  }
+  if (lane == 31) s_part[warp] = inc;
+  __syncthreads();
+  unsigned long long before = inc - mine, total = 0;
+  for (uint32_t w = 0; w < 4; ++w) {
+    if (w < warp) before += s_part[w];
+    total += s_part[w];
+  }
+  const unsigned long long per = max((total + gridDim.x - 1) / gridDim.x, (unsigned long long)plan.tiles_least);
+  const unsigned long long u0 = per * blockIdx.x, u1 = min(u0 + per, total);
+  if (u0 >= u1) return;
+  if (before <= u0 && u0 < before + mine) {
+    unsigned long long base = before;
+    for (uint32_t r = ra; r < rb; ++r) {
+      PagedRequest q;
+      paged_request(a, r, q);
+      const unsigned long long n = units_of(q);
+      if (u0 < base + n) { s_r = r; s_base = base; break; }
+      base += n;
+    }
+  }
+  __syncthreads();
+  uint32_t r = s_r;
+  unsigned long long base = s_base, u = u0;
+  const size_t head_rows = (size_t)1 << plog;
+
+  auto clear_edge = [&]() {  // the half step behind the head's end: keys' columns that no copy writes
+    for (uint32_t x = tid; x < S::STAGES * TK; x += kThreads)
+      *reinterpret_cast<uint4*>(smem + (x / TK) * S::STAGE + (x % TK) * PITCH + hd * sizeof(T)) = make_uint4(0, 0, 0, 0);
+  };
+  if (!S::F32 && hd % 16) clear_edge();
+
+  while (u < u1) {
+    Segment s;
+    s.r = r;
+    paged_request(a, r, s.rq);
+    const unsigned long long units = units_of(s.rq);
+    if (u >= base + units) { base += units; ++r; continue; }
+    const uint32_t tiles = tiles_of(s.rq), all_rows = s.rq.fresh * rep, blocks = (all_rows + RB - 1) / RB;
+    const uint32_t item = (uint32_t)((u - base) / tiles);
+    const unsigned long long item_u = base + (unsigned long long)item * tiles;
+    const uint32_t skip = paged_low(s.rq.cached, a.window) / TK;
+    s.g = item / blocks;
+    s.row0 = (item % blocks) * RB;
+    s.rows = min((uint32_t)RB, all_rows - s.row0);
+    s.tile0 = skip + (uint32_t)(u - item_u);
+    s.tile1 = skip + (uint32_t)(min(u1, item_u + tiles) - item_u);
+    // of these, the ones that the rows see
+    const uint32_t pos0 = s.rq.cached + s.row0 / rep, pos1 = s.rq.cached + (s.row0 + s.rows - 1) / rep;  // first and last row's positions
+    const uint32_t low0 = paged_low(pos0, a.window), low1 = paged_low(pos1, a.window);
+    const uint32_t ta = max(s.tile0, low0 / TK), tb = min(s.tile1, pos1 / TK + 1);
+    const int n = tb > ta ? (int)(tb - ta) : 0;
+
+    const T* kp = static_cast<const T*>(a.pool.k) + ((size_t)s.g << plog) * hd;
+    const T* vp = static_cast<const T*>(a.pool.v) + ((size_t)s.g << plog) * hd;
+    const size_t page_elems = (KV * head_rows) * hd;
+    int32_t pg[NS];  // pages of the tile to be requested next, 16 keys each
+    auto look_up = [&](uint32_t tile) {
+#pragma unroll
+      for (int i = 0; i < NS; ++i) {
+        const uint32_t j = tile * TK + 16 * i;
+        pg[i] = j < s.rq.len ? a.table[(size_t)r * a.table_ld + (j >> plog)] : -1;
+      }
+    };
+    auto request = [&](uint32_t tile, uint32_t stage) {
+      const uint32_t chunks = hd * sizeof(T) / 16, kdst = smem_u32(smem) + stage * S::STAGE;
+#pragma unroll
+      for (int i = 0; i < NS; ++i) {
+        if (tile * TK + 16 * i < s.rq.len && (uint32_t)pg[i] >= a.pool.pages) {
+          if (a.status) atomicCAS(a.status, 0, kStatusPaged);
+          pg[i] = -1;
+        }
+        for (uint32_t x = tid; x < 16 * chunks; x += kThreads) {
+          const uint32_t row = x / chunks, col = x % chunks, j = tile * TK + 16 * i + row;
+          const bool take = pg[i] >= 0 && j < s.rq.len;
+          const size_t at = take ? (size_t)pg[i] * page_elems + (size_t)(j & pmask) * hd + col * (16 / sizeof(T)) : 0;
+          const uint32_t d = kdst + (16 * i + row) * PITCH + col * 16;
+          copy16(d, kp + at, take);
+          copy16(d + TK * PITCH, vp + at, take);
+        }
+      }
+    };
+    if (n > 0) look_up(ta);
+#pragma unroll
+    for (int i = 0; i < S::STAGES - 1; ++i) {
+      if (i < n) {
+        request(ta + i, i);
+        if (i + 1 < n) look_up(ta + i + 1);
+      }
+      copy_commit();
+    }
+
+    // ---- queries
+    const uint32_t row_lo = s.row0 + wr * 16 + g4, row_hi = row_lo + 8, row_end = s.row0 + s.rows;
+    auto q_at = [&](uint32_t row) { return static_cast<const T*>(a.q) + (size_t)(s.rq.t0 + row / rep) * a.q_ld + (size_t)(s.g * rep + row % rep) * hd; };
+    uint32_t qf[S::QSMEM ? 1 : HP / 16][4];
+    if constexpr (S::QSMEM) {
+      for (uint32_t x = tid; x < RB * (HP * sizeof(T) / 16); x += kThreads) {
+        const uint32_t row = x / (HP * sizeof(T) / 16), col = x % (HP * sizeof(T) / 16);
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (row < s.rows && col * (16 / sizeof(T)) < hd) v = *reinterpret_cast<const uint4*>(q_at(s.row0 + row) + col * (16 / sizeof(T)));
+        *reinterpret_cast<uint4*>(qsm + row * PITCH + col * 16) = v;
+      }
+    } else {
+      const T* q0 = row_lo < row_end ? q_at(row_lo) : nullptr;
+      const T* q1 = row_hi < row_end ? q_at(row_hi) : nullptr;
+#pragma unroll
+      for (int e = 0; e < HP / 16; ++e)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t col = e * 16 + h * 8 + 2 * t4;
+          qf[e][2 * h] = q0 && col < hd ? *reinterpret_cast<const uint32_t*>(q0 + col) : 0u;
+          qf[e][2 * h + 1] = q1 && col < hd ? *reinterpret_cast<const uint32_t*>(q1 + col) : 0u;
+        }
+    }
+    const uint32_t p_lo = s.rq.cached + min(row_lo, row_end - 1) / rep, p_hi = s.rq.cached + min(row_hi, row_end - 1) / rep;
+    const uint32_t l_lo = paged_low(p_lo, a.window), l_hi = paged_low(p_hi, a.window);
+
+    float o[HP / 8][4], m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
+#pragma unroll
+    for (int i = 0; i < HP / 8; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[i][j] = 0.0f;
+
+    for (int i = 0; i < n; ++i) {
+      copy_wait<S::STAGES - 2>();
+      __syncthreads();
+      if (i + S::STAGES - 1 < n) {
+        request(ta + i + S::STAGES - 1, (i + S::STAGES - 1) % S::STAGES);
+        if (i + S::STAGES < n) look_up(ta + i + S::STAGES);
+      }
+      copy_commit();
+      const unsigned char* ks = smem + (i % S::STAGES) * S::STAGE + wk * KW * PITCH;
+      const unsigned char* vs = ks + TK * PITCH;
+      const uint32_t key0 = (ta + i) * TK + wk * KW;
+      float sc[KW / 8][4];
+#pragma unroll
+      for (int j = 0; j < KW / 8; ++j) sc[j][0] = sc[j][1] = sc[j][2] = sc[j][3] = 0.0f;
+      if constexpr (!S::F32) {
+        const uint32_t kaddr = smem_u32(ks) + ((lane & 7) + ((lane >> 4) << 3)) * PITCH + ((lane >> 3) & 1) * 16;
+        const uint32_t qaddr = smem_u32(qsm) + (wr * 16 + (lane & 15)) * PITCH + (lane >> 4) * 16;
+#pragma unroll
+        for (int e = 0; e < HP / 16; ++e) {
+          if (HP != 64 && e * 16 >= (int)hd) break;
+          uint32_t qa[4];
+          if constexpr (S::QSMEM) ldmatrix4(qa, qaddr + e * 32);
+          else { qa[0] = qf[e][0]; qa[1] = qf[e][1]; qa[2] = qf[e][2]; qa[3] = qf[e][3]; }
+#pragma unroll
+          for (int j = 0; j < KW / 16; ++j) {
+            uint32_t b[4];
+            ldmatrix4(b, kaddr + j * 16 * PITCH + e * 32);
+            mma16<T>(sc[2 * j], qa, b[0], b[1]);
+            mma16<T>(sc[2 * j + 1], qa, b[2], b[3]);
+          }
+        }
+      } else {
+        const float* kf = reinterpret_cast<const float*>(ks) + g4 * (PITCH / 4) + t4;
+        const float* qs = reinterpret_cast<const float*>(qsm) + (wr * 16 + g4) * (PITCH / 4) + t4;
+        for (uint32_t e0 = 0; e0 < hd / 8; e0 += 4) {  // 32 elements of the head at a time
+          float part[KW / 8][4];
+#pragma unroll
+          for (int j = 0; j < KW / 8; ++j) part[j][0] = part[j][1] = part[j][2] = part[j][3] = 0.0f;
+#pragma unroll
+          for (uint32_t f = 0; f < 4; ++f) {
+            const uint32_t e = e0 + f;
+            if (e >= hd / 8) break;
+            uint32_t ah[4], al[4];
+            split_tf32(qs[e * 8], ah[0], al[0]);
+            split_tf32(qs[e * 8 + 8 * (PITCH / 4)], ah[1], al[1]);
+            split_tf32(qs[e * 8 + 4], ah[2], al[2]);
+            split_tf32(qs[e * 8 + 8 * (PITCH / 4) + 4], ah[3], al[3]);
+#pragma unroll
+            for (int j = 0; j < KW / 8; ++j) {
+              uint32_t bh[2], bl[2];
+              split_tf32(kf[j * 8 * (PITCH / 4) + e * 8], bh[0], bl[0]);
+              split_tf32(kf[j * 8 * (PITCH / 4) + e * 8 + 4], bh[1], bl[1]);
+              mma8(part[j], al, bh[0], bh[1]);
+              mma8(part[j], ah, bl[0], bl[1]);
+              mma8(part[j], ah, bh[0], bh[1]);
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < KW / 8; ++j)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) sc[j][x] += part[j][x];
+        }
+      }
+      // ---- softmax; row g4 in elements 0 and 1, row g4 + 8 in 2 and 3
+      const bool whole = (ta + i) * TK >= low1 && (ta + i) * TK + TK <= pos0 + 1;
+#pragma unroll
+      for (int j = 0; j < KW / 8; ++j)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const uint32_t key = key0 + j * 8 + 2 * t4 + (x & 1);
+          const float v = sc[j][x] * c;
+          sc[j][x] = whole || (key <= (x < 2 ? p_lo : p_hi) && key >= (x < 2 ? l_lo : l_hi)) ? v : -INFINITY;
+        }
+      float x0 = -INFINITY, x1 = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < KW / 8; ++j) {
+        x0 = fmaxf(x0, fmaxf(sc[j][0], sc[j][1]));
+        x1 = fmaxf(x1, fmaxf(sc[j][2], sc[j][3]));
+      }
+#pragma unroll
+      for (int off = 1; off < 4; off <<= 1) {
+        x0 = fmaxf(x0, __shfl_xor_sync(0xFFFFFFFFu, x0, off));
+        x1 = fmaxf(x1, __shfl_xor_sync(0xFFFFFFFFu, x1, off));
+      }
+      const float n0 = fmaxf(m0, x0), n1 = fmaxf(m1, x1);
+      if (__any_sync(0xFFFFFFFFu, n0 > m0 || n1 > m1)) {
+        const float c0 = m0 == -INFINITY ? 0.0f : exp2_of(m0 - n0), c1 = m1 == -INFINITY ? 0.0f : exp2_of(m1 - n1);
+        l0 *= c0;
+        l1 *= c1;
+#pragma unroll
+        for (int d = 0; d < HP / 8; ++d) { o[d][0] *= c0; o[d][1] *= c0; o[d][2] *= c1; o[d][3] *= c1; }
+        m0 = n0;
+        m1 = n1;
+      }
+      const float b0 = m0 == -INFINITY ? 0.0f : m0, b1 = m1 == -INFINITY ? 0.0f : m1;
+#pragma unroll
+      for (int j = 0; j < KW / 8; ++j) {
+        sc[j][0] = exp2_of(sc[j][0] - b0); sc[j][1] = exp2_of(sc[j][1] - b0);
+        sc[j][2] = exp2_of(sc[j][2] - b1); sc[j][3] = exp2_of(sc[j][3] - b1);
+        l0 += sc[j][0] + sc[j][1];
+        l1 += sc[j][2] + sc[j][3];
+      }
+      // ---- weighted values
+      if constexpr (!S::F32) {
+        const uint32_t vaddr = smem_u32(vs) + ((lane & 7) + ((lane >> 3) & 1) * 8) * PITCH + (lane >> 4) * 16;
+#pragma unroll
+        for (int j = 0; j < KW / 16; ++j) {
+          const uint32_t pa[4] = {pack2<T>(sc[2 * j][0], sc[2 * j][1]), pack2<T>(sc[2 * j][2], sc[2 * j][3]), pack2<T>(sc[2 * j + 1][0], sc[2 * j + 1][1]),
+                                  pack2<T>(sc[2 * j + 1][2], sc[2 * j + 1][3])};
+#pragma unroll
+          for (int d = 0; d < HP / 16; ++d) {
+            if (HP != 64 && d * 16 >= (int)hd) break;
+            uint32_t b[4];
+            ldmatrix4t(b, vaddr + j * 16 * PITCH + d * 32);
+            mma16<T>(o[2 * d], pa, b[0], b[1]);
+            mma16<T>(o[2 * d + 1], pa, b[2], b[3]);
+          }
+        }
+      } else {
+        const float* vf = reinterpret_cast<const float*>(vs) + 2 * t4 * (PITCH / 4) + g4;
+        uint32_t ph[KW / 8][4], pl[KW / 8][4];  // the product's k is key 2 t4 for t4, 2 t4 + 1 for t4 + 4
+#pragma unroll
+        for (int j = 0; j < KW / 8; ++j) {
+          split_tf32(sc[j][0], ph[j][0], pl[j][0]);
+          split_tf32(sc[j][2], ph[j][1], pl[j][1]);
+          split_tf32(sc[j][1], ph[j][2], pl[j][2]);
+          split_tf32(sc[j][3], ph[j][3], pl[j][3]);
+        }
+#pragma unroll
+        for (int d = 0; d < HP / 8; ++d) {
+          if (d * 8 >= (int)hd) break;
+          float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int j = 0; j < KW / 8; ++j) {
+            uint32_t bh[2], bl[2];
+            split_tf32(vf[j * 8 * (PITCH / 4) + d * 8], bh[0], bl[0]);
+            split_tf32(vf[(j * 8 + 1) * (PITCH / 4) + d * 8], bh[1], bl[1]);
+            mma8(part, pl[j], bh[0], bh[1]);
+            mma8(part, ph[j], bl[0], bl[1]);
+            mma8(part, ph[j], bh[0], bh[1]);
+          }
+#pragma unroll
+          for (int x = 0; x < 4; ++x) o[d][x] += part[x];
+        }
+      }
+    }
+
+    // ---- the warps' results meet in the tiles' place
+    copy_wait<0>();
+    __syncthreads();
+#pragma unroll
+    for (int off = 1; off < 4; off <<= 1) {
+      l0 += __shfl_xor_sync(0xFFFFFFFFu, l0, off);
+      l1 += __shfl_xor_sync(0xFFFFFFFFu, l1, off);
+    }
+    float* res = reinterpret_cast<float*>(smem);  // [warp][16][HP + 4]
+    {
+      float* d0 = res + (warp * 16 + g4) * (HP + 4) + 2 * t4;
+      float* d1 = d0 + 8 * (HP + 4);
+#pragma unroll
+      for (int d = 0; d < HP / 8; ++d) {
+        if (d * 8 >= (int)hd) break;
+        *reinterpret_cast<float2*>(d0 + d * 8) = make_float2(o[d][0], o[d][1]);
+        *reinterpret_cast<float2*>(d1 + d * 8) = make_float2(o[d][2], o[d][3]);
+      }
+      if (t4 == 0) { s_m[warp][g4] = m0; s_l[warp][g4] = l0; s_m[warp][g4 + 8] = m1; s_l[warp][g4 + 8] = l1; }
+    }
+    __syncthreads();
+    const bool cut_begin = u != item_u, cut_end = item_u + tiles > u1;
+    const bool cut = cut_begin || cut_end;
+    float* part = plan.parts + ((size_t)blockIdx.x * 2 + (cut_begin ? 0 : 1)) * (RB * (HP + 2));
+    // a warp per row
+    for (uint32_t row = warp; row < s.rows; row += 4) {
+      const uint32_t w0 = row / 16, rr = row % 16;  // the row's warps are w0, w0 + WR, ...
+      float m = -INFINITY, l = 0.0f, f[WK], v[kHeadParts];
+#pragma unroll
+      for (int w = 0; w < WK; ++w) m = fmaxf(m, s_m[w0 + w * WR][rr]);
+#pragma unroll
+      for (int w = 0; w < WK; ++w) {
+        const float mw = s_m[w0 + w * WR][rr];
+        f[w] = mw == -INFINITY ? 0.0f : exp2_of(mw - m);
+        l = fmaf(s_l[w0 + w * WR][rr], f[w], l);
+      }
+      bool fine = isfinite(l);
+#pragma unroll
+      for (int j = 0; j < HP / 32; ++j) {
+        const uint32_t e = lane + 32 * j;
+        v[j] = 0.0f;
+        if (e < hd) {
+#pragma unroll
+          for (int w = 0; w < WK; ++w) v[j] = fmaf(res[((w0 + w * WR) * 16 + rr) * (HP + 4) + e], f[w], v[j]);
+          fine = fine && isfinite(v[j]);
+        }
+      }
+      if (!__all_sync(0xFFFFFFFFu, fine)) {
+        float* again = res + (w0 * 16 + rr) * (HP + 4);
+        row_again<T>(a, s, rep, s.row0 + row, s.tile0 * TK, s.tile1 * TK, again, m, l);
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < HP / 32; ++j) v[j] = lane + 32 * j < hd ? again[lane + 32 * j] : 0.0f;
+      }
+      if (!cut) {
+        const uint32_t x = s.row0 + row;
+        T* dst = static_cast<T*>(a.out) + (size_t)(s.rq.t0 + x / rep) * a.out_ld + (size_t)(s.g * rep + x % rep) * hd;
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+        for (int j = 0; j < HP / 32; ++j)
+          if (lane + 32 * j < hd) dst[lane + 32 * j] = from_f32<T>(l == 0.0f ? 0.0f : v[j] * inv);
+      } else {
+        float* dst = part + row * (HP + 2);
+#pragma unroll
+        for (int j = 0; j < HP / 32; ++j)
+          if (lane + 32 * j < hd) dst[lane + 32 * j] = v[j];
+        if (lane == 0) { dst[HP] = m; dst[HP + 1] = l; }
+      }
+    }
+    if (cut) {
+      // ---- the item's parts, joined by the CTA that comes last
+      const uint32_t first = (uint32_t)(item_u / per), last = (uint32_t)((item_u + tiles - 1) / per);
+      __threadfence();
+      __syncthreads();
+      if (tid == 0) s_last = atomicAdd(&plan.arrived[first], 1u) == last - first ? 1u : 0u;
+      __syncthreads();
+      if (s_last) {
+        __threadfence();
+        for (uint32_t row = warp; row < s.rows; row += 4) {
+          auto part_of = [&](uint32_t p) { return plan.parts + ((size_t)p * 2 + (p == first ? 1 : 0)) * (RB * (HP + 2)) + row * (HP + 2); };
+          float m = -INFINITY;
+          for (uint32_t p = first + lane; p <= last; p += 32) m = fmaxf(m, __ldcg(part_of(p) + HP));
+#pragma unroll
+          for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, off));
+          float l = 0.0f, v[HP / 32];
+#pragma unroll
+          for (int j = 0; j < HP / 32; ++j) v[j] = 0.0f;
+#pragma unroll 4
+          for (uint32_t p = first; p <= last; ++p) {
+            const float* src = part_of(p);
+            const float mp = __ldcg(src + HP), lp = __ldcg(src + HP + 1), f = mp == -INFINITY ? 0.0f : exp2_of(mp - m);
+            l = fmaf(lp, f, l);
+#pragma unroll
+            for (int j = 0; j < HP / 32; ++j)
+              if (lane + 32 * j < hd) v[j] = fmaf(__ldcg(src + lane + 32 * j), f, v[j]);
+          }
+          const uint32_t x = s.row0 + row;
+          T* dst = static_cast<T*>(a.out) + (size_t)(s.rq.t0 + x / rep) * a.out_ld + (size_t)(s.g * rep + x % rep) * hd;
+#pragma unroll
+          for (int j = 0; j < HP / 32; ++j)
+            if (lane + 32 * j < hd) dst[lane + 32 * j] = from_f32<T>(l == 0.0f ? 0.0f : v[j] / l);
+        }
+        if (tid == 0) plan.arrived[first] = 0;
+      }
+    }
+    __syncthreads();  // the results have been read: tiles may come in their place
+    if (!S::F32 && hd % 16) clear_edge();
+    u = item_u + (s.tile1 - skip);
+  }
+}
+
+template <typename T, int HP, int WR>
+cudaError_t launch_rows(ruai_ctx* c, const PagedAttn& a, uint32_t rows_most) {
+  using S = Shape<T, HP, WR>;
+  static int per_sm[64] = {};
+  int& n = per_sm[c->ordinal & 63];
+  if (!n) {
+    cudaError_t e = cudaFuncSetAttribute(rows_kernel<T, HP, WR>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
+    if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, rows_kernel<T, HP, WR>, kThreads, S::SMEM);
+    if (e != cudaSuccess) return e;
+    n = std::max(n, 1);
+  }
+  RowsPlan p = {c->partial, c->counters, rows_most, 2};
+  // a run per resident CTA, as far as the context's first scratch holds their parts: it never grows for them
+  const uint32_t grid = (uint32_t)std::min<size_t>((size_t)c->sm_count * n, kScratchBytes / (2 * S::PART));
+  return ruai_launch(c, rows_kernel<T, HP, WR>, dim3(grid), dim3(kThreads), S::SMEM, true, a, p);
+}
+
+template <typename T, int HP>
+cudaError_t launch_width(ruai_ctx* c, const PagedAttn& a, uint32_t rows) {
+  if (rows <= 16) return launch_rows<T, HP, 1>(c, a, 0xFFFFFFFFu);
+  if (rows <= 32 || HP == 256) return launch_rows<T, HP, 2>(c, a, 0xFFFFFFFFu);
+  return launch_rows<T, HP == 256 ? 128 : HP, 4>(c, a, 0xFFFFFFFFu);
+}
+
+template <typename T>
+cudaError_t launch_type(ruai_ctx* c, const PagedAttn& a) {
+  const uint32_t rows = (uint32_t)std::min<unsigned long long>((unsigned long long)a.most_fresh * (a.H / a.pool.KV), 0xFFFFFFFFu);
+  return a.pool.hd <= 64 ? launch_width<T, 64>(c, a, rows) : a.pool.hd <= 128 ? launch_width<T, 128>(c, a, rows) : launch_width<T, 256>(c, a, rows);
 }
 
 }  // namespace
 
 int ruai_paged_attention_launch(ruai_ctx* c, const PagedAttn& a) {
-  const dim3 grid((a.tokens * a.H + 7) / 8), block(256);
-  RUAI_CUDA(c, a.pool.dtype == RUAI_F32   ? ruai_launch(c, one_row_kernel<float>, grid, block, 0, true, a)
-               : a.pool.dtype == RUAI_F16 ? ruai_launch(c, one_row_kernel<__half>, grid, block, 0, true, a)
-                                          : ruai_launch(c, one_row_kernel<__nv_bfloat16>, grid, block, 0, true, a));
+  RUAI_CUDA(c, a.pool.dtype == RUAI_F32   ? launch_type<float>(c, a)
+               : a.pool.dtype == RUAI_F16 ? launch_type<__half>(c, a)
+                                          : launch_type<__nv_bfloat16>(c, a));
   return RUAI_OK;
 }

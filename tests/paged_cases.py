@@ -80,7 +80,8 @@ def attention(q, k, v, table, cached, starts, scale, window, dtype):
     T, H, _ = q.shape
     rep = H // KV
     out, tol = np.full((T, H, hd), np.nan), np.zeros((T, H, hd))
-    k, v, q = (np.asarray(x, np.float64) for x in (k, v, q))
+    with np.errstate(invalid="ignore"):  # NaN where nothing is held
+        k, v, q = (np.asarray(x, np.float64) for x in (k, v, q))
     for r in range(len(cached)):
         c, t0, t1 = int(cached[r]), int(starts[r]), int(starts[r + 1])
         if t0 == t1:
