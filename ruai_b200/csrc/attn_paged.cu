@@ -17,71 +17,12 @@
 // nothing, must not reach it through 0 x inf.
 #include <algorithm>
 
-#include "paged.cuh"
+#include "attn_paged.cuh"
 #include "pipeline.cuh"
 
 namespace {
 
 using pipe::smem_u32;
-
-constexpr int kHeadParts = 8;  // elements of a head per lane: heads of up to 256
-constexpr float kLog2e = 1.44269504088896341f;
-
-__device__ __forceinline__ float exp2_of(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-// What a CTA does with one item: keys of tiles [tile0, tile1) for rows [row0, row0 + rows) of (request r, key head g).
-struct Segment {
-  PagedRequest rq;
-  uint32_t r, g, row0, rows, tile0, tile1;
-};
-
-// One row over keys [k0, k1) by a warp, a key at a time; m and scores in powers of two, o not divided by l.
-template <typename T>
-__device__ void row_again(const PagedAttn& a, const Segment& s, uint32_t rep, uint32_t row, uint32_t k0, uint32_t k1, float* o_out, float& m_out, float& l_out) {
-  const uint32_t lane = threadIdx.x & 31u, hd = a.pool.hd, i = row / rep, pos = s.rq.cached + i;
-  const T* qs = static_cast<const T*>(a.q) + (size_t)(s.rq.t0 + i) * a.q_ld + (size_t)(s.g * rep + row % rep) * hd;
-  float q[kHeadParts], o[kHeadParts], m = -INFINITY, l = 0.0f;
-#pragma unroll
-  for (int j = 0; j < kHeadParts; ++j) {
-    const uint32_t e = lane + 32u * j;
-    q[j] = e < hd ? to_f32<T>(qs[e]) : 0.0f;
-    o[j] = 0.0f;
-  }
-  for (uint32_t k = max(k0, paged_low(pos, a.window)); k < min(k1, pos + 1); ++k) {
-    const int32_t pg = paged_page(a, s.r, k);
-    if (pg < 0) continue;
-    const size_t at = ((((size_t)pg * a.pool.KV + s.g) << a.pool.page_log2) + (k & ((1u << a.pool.page_log2) - 1u))) * hd;
-    float d = 0.0f;
-#pragma unroll
-    for (int j = 0; j < kHeadParts; ++j) {
-      const uint32_t e = lane + 32u * j;
-      if (e < hd) d = fmaf(q[j], to_f32<T>(static_cast<const T*>(a.pool.k)[at + e]), d);
-    }
-#pragma unroll
-    for (int off = 16; off > 0; off >>= 1) d += __shfl_xor_sync(0xFFFFFFFFu, d, off);
-    d *= a.scale * kLog2e;
-    if (d == -INFINITY) continue;
-    const float m_new = fmaxf(m, d), corr = m == -INFINITY ? 0.0f : exp2_of(m - m_new), pr = exp2_of(d - m_new);
-    l = fmaf(l, corr, pr);
-    m = m_new;
-#pragma unroll
-    for (int j = 0; j < kHeadParts; ++j) {
-      const uint32_t e = lane + 32u * j;
-      if (e < hd) o[j] = fmaf(pr, to_f32<T>(static_cast<const T*>(a.pool.v)[at + e]), o[j] * corr);
-    }
-  }
-#pragma unroll
-  for (int j = 0; j < kHeadParts; ++j) {
-    const uint32_t e = lane + 32u * j;
-    if (e < hd) o_out[e] = o[j];
-  }
-  m_out = m;
-  l_out = l;
-}
 
 // ---- products ---------------------------------------------------------------------------------------------------------------
 
@@ -587,23 +528,35 @@ cudaError_t launch_rows(ruai_ctx* c, const PagedAttn& a, uint32_t rows_most) {
 }
 
 template <typename T, int HP>
-cudaError_t launch_width(ruai_ctx* c, const PagedAttn& a, uint32_t rows) {
-  if (rows <= 16) return launch_rows<T, HP, 1>(c, a, 0xFFFFFFFFu);
-  if (rows <= 32 || HP == 256) return launch_rows<T, HP, 2>(c, a, 0xFFFFFFFFu);
-  return launch_rows<T, HP == 256 ? 128 : HP, 4>(c, a, 0xFFFFFFFFu);
+cudaError_t launch_width(ruai_ctx* c, const PagedAttn& a, uint32_t rows, uint32_t rows_most) {
+  if (rows <= 16) return launch_rows<T, HP, 1>(c, a, rows_most);
+  if (rows <= 32 || HP == 256) return launch_rows<T, HP, 2>(c, a, rows_most);
+  return launch_rows<T, HP == 256 ? 128 : HP, 4>(c, a, rows_most);
 }
 
 template <typename T>
-cudaError_t launch_type(ruai_ctx* c, const PagedAttn& a) {
-  const uint32_t rows = (uint32_t)std::min<unsigned long long>((unsigned long long)a.most_fresh * (a.H / a.pool.KV), 0xFFFFFFFFu);
-  return a.pool.hd <= 64 ? launch_width<T, 64>(c, a, rows) : a.pool.hd <= 128 ? launch_width<T, 128>(c, a, rows) : launch_width<T, 256>(c, a, rows);
+cudaError_t launch_type(ruai_ctx* c, const PagedAttn& a, uint32_t rows, uint32_t rows_most) {
+  return a.pool.hd <= 64    ? launch_width<T, 64>(c, a, rows, rows_most)
+         : a.pool.hd <= 128 ? launch_width<T, 128>(c, a, rows, rows_most)
+                            : launch_width<T, 256>(c, a, rows, rows_most);
 }
+
+// A step whose requests have no more than this many rows stays on the kernel here; else it keeps those of kRowsBeside at the most.
+constexpr uint32_t kRowsAlone = 64, kRowsBeside = 16;
 
 }  // namespace
 
 int ruai_paged_attention_launch(ruai_ctx* c, const PagedAttn& a) {
-  RUAI_CUDA(c, a.pool.dtype == RUAI_F32   ? launch_type<float>(c, a)
-               : a.pool.dtype == RUAI_F16 ? launch_type<__half>(c, a)
-                                          : launch_type<__nv_bfloat16>(c, a));
+  uint32_t rows = a.most_fresh * (a.H / a.pool.KV), rows_most = 0xFFFFFFFFu;  // below 2^31: most_fresh is checked against the tokens
+  if (rows > kRowsAlone) {
+    const uint32_t rep = a.H / a.pool.KV, over = a.R > 1 && rep <= kRowsBeside ? kRowsBeside : 0u;
+    const int took = ruai_paged_attention_tc(c, a, over);
+    if (took < 0) return RUAI_ERR_CUDA;
+    if (took && !over) return RUAI_OK;
+    if (took) rows = rows_most = over;
+  }
+  RUAI_CUDA(c, a.pool.dtype == RUAI_F32   ? launch_type<float>(c, a, rows, rows_most)
+               : a.pool.dtype == RUAI_F16 ? launch_type<__half>(c, a, rows, rows_most)
+                                          : launch_type<__nv_bfloat16>(c, a, rows, rows_most));
   return RUAI_OK;
 }

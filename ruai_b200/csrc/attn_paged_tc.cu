@@ -1,0 +1,621 @@
+// Attention of chunks over pages on the tensor cores (tcgen05), f16 and bf16: what attn_paged.cu computes, for the requests with many rows.
+//
+// An item is two tiles of up to 128 rows (token, query head; whole tokens) of one request and key head, over the keys that any of them
+// sees, 128 at a time.  One warp copies a tile's keys and values page by page (TMA boxes of a page's rows, so that pages lie in shared
+// memory as one tile, 128-byte swizzle); one issues the MMAs, S_t = Q_t K^T and O_t += P_t V in turn for both row tiles, so that one
+// tile's products run beside the other's softmax; one copies the next item's queries; two warpgroups are the softmax, a thread per row.  Scores,
+// probabilities (written over the scores, rounded once to the values' type) and outputs stay in tensor memory: 2 x (128 + 128)
+// columns.  Outputs are rescaled only where a row's maximum has grown by more than 2^8 since the last time: weights of up to 256 are as exact
+// as those of up to 1, and nearly every tile leaves the outputs where they are.
+//   Split: the key tiles of all items, in a row, in equal runs, one per CTA.  An item cut by a run's end leaves (m, l, o) of its parts in
+// scratch, and join_kernel adds them up, many CTAs to an item (the last CTA to arrive alone took 90 us for 17 parts).
+//   Values of the positions behind a request's end are cleared in shared memory (0 x NaN), and a row that is not finite at the end is worked
+// out again key by key.  Every mbarrier wait is bounded.
+#include <cuda.h>
+
+#include <algorithm>
+#include <type_traits>
+
+#include "attn_paged.cuh"
+#include "pipeline.cuh"
+
+namespace {
+
+using namespace pipe;
+
+constexpr int kKeys = 128, kRows = 128, kItemRows = 2 * kRows;
+constexpr int kPanel = 128 * 128;  // bytes of 128 rows of 64 elements
+constexpr int kThreads = 384;
+constexpr uint32_t kOutCol = 256;  // tensor memory: scores of both tiles, then their outputs
+constexpr float kGrowth = 8.0f;
+constexpr int kTilesLeast = 4;  // of a run: a part costs as much as a few tiles
+
+struct alignas(64) Maps { CUtensorMap q, k, v; };
+
+// A cut item, left by the CTA in which it begins for the CTAs that join it.
+struct Cut { uint32_t last, token, tokens, g; };  // the CTA in which it ends (0: nothing was cut), its tokens' rows of the step, the key head
+struct TcPlan {
+  float* parts;  // [CTAs][2]: the part that ends the item a CTA begins with, the part that begins the one it ends with; [columns / 4][256 rows][4], maxima, sums
+  Cut* cuts;     // [CTAs], or NULL: items stay whole
+  uint32_t rows_over, box_rows, part_floats;
+  uint32_t tile_tokens;  // tokens of a row tile
+};
+
+__device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst), "l"((uint64_t)map), "r"(x), "r"(y),
+               "r"(z), "r"(smem_u32(bar))
+               : "memory");
+}
+__device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
+  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst), "l"((uint64_t)map), "r"(x), "r"(y),
+               "r"(smem_u32(bar))
+               : "memory");
+}
+// 32 columns of this thread's lane, loaded when the call returns.
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float* v) {
+  uint32_t r[32];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, "
+      "%22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n\ttcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+        "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
+        "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const float* v) {
+  uint32_t r[32];
+#pragma unroll
+  for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(v[i]);
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, "
+      "%22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::"r"(r[0]),
+      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]),
+      "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]),
+      "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::"r"(r[0]), "r"(r[1]), "r"(r[2]),
+               "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
+               : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// An operand whose rows are the sum's index (values [key][element]): panels of 64 elements kPanel apart, eight keys 1024 bytes apart.
+__device__ __forceinline__ uint64_t umma_desc_mn128(uint32_t addr) {
+  return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)(kPanel >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b);
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// A part of an item: what every role of the CTA walks through in the same order.
+struct Piece {
+  Segment s;                 // row0: the item's first row; tiles of keys [tile0, tile1)
+  unsigned long long item_u;
+  uint32_t tiles;            // of the whole item
+  uint32_t token, tokens;    // of the request
+  uint32_t n[2], n_all;      // how many tiles from tile0 on each row tile sees
+  bool cut_begin, cut_end;
+};
+struct Walk {
+  unsigned long long u, base;  // the next unit; the first unit of the requests' row block b
+  uint32_t r, b;
+};
+
+struct Runs {
+  unsigned long long u1;
+  uint32_t rep, rows_over, tokens;  // tokens of an item
+  __device__ __forceinline__ uint32_t tiles(const PagedAttn& a, const PagedRequest& q, uint32_t b, uint32_t& skip) const {
+    skip = paged_low(q.cached + b * tokens, a.window) / kKeys;
+    return (q.cached + min((b + 1) * tokens, q.fresh) - 1) / kKeys + 1 - skip;
+  }
+  __device__ unsigned long long units(const PagedAttn& a, const PagedRequest& q) const {
+    if (q.fresh * rep <= rows_over) return 0;
+    unsigned long long n = 0;
+    uint32_t skip;
+    for (uint32_t b = 0; b * tokens < q.fresh; ++b) n += tiles(a, q, b, skip);
+    return n * a.pool.KV;
+  }
+  __device__ bool next(const PagedAttn& a, const TcPlan& plan, Walk& w, Piece& p) const {
+    while (w.u < u1) {
+      PagedRequest q;
+      paged_request(a, w.r, q);
+      if (q.fresh * rep <= rows_over || w.b * tokens >= q.fresh) { ++w.r; w.b = 0; continue; }
+      uint32_t skip;
+      const uint32_t n = tiles(a, q, w.b, skip);
+      const unsigned long long all = (unsigned long long)n * a.pool.KV;
+      if (w.u >= w.base + all) { w.base += all; ++w.b; continue; }
+      const uint32_t g = (uint32_t)(w.u - w.base) / n;  // fewer than 2^32 units in a block of rows: keys / 128 x key heads
+      p.item_u = w.base + (unsigned long long)g * n;
+      if (!plan.cuts && w.u != p.item_u) { w.u = p.item_u + n; continue; }  // the CTA before has the whole item
+      p.tiles = n;
+      p.s.rq = q; p.s.r = w.r; p.s.g = g;
+      p.token = w.b * tokens;
+      p.tokens = min(tokens, q.fresh - p.token);
+      p.s.row0 = p.token * rep;
+      p.s.rows = p.tokens * rep;
+      p.s.tile0 = skip + (uint32_t)(w.u - p.item_u);
+      const unsigned long long end = plan.cuts ? min(u1, p.item_u + n) : p.item_u + n;
+      p.s.tile1 = skip + (uint32_t)(end - p.item_u);
+      p.cut_begin = w.u != p.item_u;
+      p.cut_end = end != p.item_u + n;
+#pragma unroll
+      for (uint32_t t = 0; t < 2; ++t) {
+        p.n[t] = 0;
+        if (p.tokens > t * plan.tile_tokens) {
+          const uint32_t last = (q.cached + p.token + min(p.tokens, (t + 1) * plan.tile_tokens) - 1) / kKeys + 1, stop = min(p.s.tile1, last);
+          p.n[t] = stop > p.s.tile0 ? stop - p.s.tile0 : 0u;
+        }
+      }
+      p.n_all = max(p.n[0], p.n[1]);
+      w.u = end;
+      return true;
+    }
+    return false;
+  }
+};
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const PagedAttn a, const TcPlan plan, const __grid_constant__ Maps maps) {
+  extern __shared__ unsigned char smem_raw[];
+  __shared__ __align__(8) uint64_t q_full, q_empty, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_ready[2], o_full[2], fin;
+  __shared__ uint32_t s_tmem, s_r;
+  __shared__ volatile int s_abort;
+  __shared__ unsigned long long s_part[kThreads / 32], s_base;
+  __shared__ float s_again[8][128];
+  const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, hd = a.pool.hd, panels = (hd + 63) / 64, plog = a.pool.page_log2;
+  unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  const uint32_t q_tile = panels * kPanel, slot_bytes = panels * kPanel;
+  const uint32_t sq = smem_u32(smem), sk = sq + 2 * q_tile, sv = sk + 2 * slot_bytes;
+
+  if (tid == 0) {
+    mbar_init(&q_full, 1); mbar_init(&q_empty, 1); mbar_init(&fin, 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&k_full[i], 1); mbar_init(&k_empty[i], 1); mbar_init(&v_full[i], 1); mbar_init(&v_empty[i], 1);
+      mbar_init(&s_full[i], 1); mbar_init(&p_ready[i], 4); mbar_init(&o_full[i], 1);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    s_abort = 0;
+  }
+  __syncwarp();
+  if (warp == 1) tmem_alloc(&s_tmem, 512);
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem = s_tmem;
+  grid_dependency_wait();
+  grid_launch_dependents();
+
+  // ---- this CTA's run of units (a unit: a tile of keys of an item)
+  Runs runs = {0, a.H / a.pool.KV, plan.rows_over, 2 * plan.tile_tokens};
+  Walk walk0 = {0, 0, 0, 0};
+  unsigned long long per;
+  {
+    const uint32_t each = (a.R + kThreads - 1) / kThreads, ra = min(tid * each, a.R), rb = min(ra + each, a.R);
+    unsigned long long mine = 0;
+    for (uint32_t r = ra; r < rb; ++r) {
+      PagedRequest q;
+      paged_request(a, r, q);
+      mine += runs.units(a, q);
+    }
+    unsigned long long inc = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const unsigned long long v = __shfl_up_sync(0xFFFFFFFFu, inc, o);
+      if (lane >= (uint32_t)o) inc += v;
+    }
+    if (lane == 31) s_part[warp] = inc;
+    __syncthreads();
+    unsigned long long before = inc - mine, total = 0;
+    for (uint32_t w = 0; w < kThreads / 32; ++w) {
+      if (w < warp) before += s_part[w];
+      total += s_part[w];
+    }
+    per = max((total + gridDim.x - 1) / gridDim.x, (unsigned long long)kTilesLeast);
+    walk0.u = per * blockIdx.x;
+    runs.u1 = min(walk0.u + per, total);
+    if (walk0.u < runs.u1 && before <= walk0.u && walk0.u < before + mine) {
+      unsigned long long base = before;
+      for (uint32_t r = ra; r < rb; ++r) {
+        PagedRequest q;
+        paged_request(a, r, q);
+        const unsigned long long n = runs.units(a, q);
+        if (walk0.u < base + n) { s_r = r; s_base = base; break; }
+        base += n;
+      }
+    }
+    __syncthreads();
+    walk0.r = s_r;
+    walk0.base = s_base;
+  }
+
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
+    Walk w = walk0;
+    Piece p;
+    bool ok = true;
+    auto wait = [&](uint64_t* bar, uint32_t parity) {  // the same answer for the whole warp
+      if (ok) ok = __all_sync(0xFFFFFFFFu, !s_abort && mbar_wait(bar, parity));
+      if (!ok) s_abort = 1;
+      return ok;
+    };
+    if (warp == 0) {
+      // ===== keys and values, a lane per box
+      const uint32_t boxes = kKeys / plan.box_rows, box = lane % boxes, panel = lane / boxes;
+      const uint32_t dst = panel * kPanel + box * plan.box_rows * 128;
+      uint32_t kt = 0, vt = 0;  // tiles asked for
+      while (ok && runs.next(a, plan, w, p)) {
+        for (uint32_t j = 0; j < p.n_all; ++j) {
+          const uint32_t key = (p.s.tile0 + j) * kKeys + box * plan.box_rows, slot = kt & 1u;
+          int32_t pg = -1;
+          if (key < p.s.rq.len) pg = paged_page(a, p.s.r, key);
+          const uint32_t bytes = __popc(__ballot_sync(0xFFFFFFFFu, lane < boxes && pg >= 0)) * panels * plan.box_rows * 128;
+          const int y = pg >= 0 ? (int)((((uint32_t)pg * a.pool.KV + p.s.g) << plog) + (key & ((1u << plog) - 1u))) : 0;
+          const bool mine = panel < panels && pg >= 0;
+          if (kt >= 2 && !wait(&k_empty[slot], (kt / 2 - 1) & 1u)) break;
+          if (lane == 0) mbar_expect_tx(&k_full[slot], bytes);
+          __syncwarp();
+          if (mine) tma_2d(sk + slot * slot_bytes + dst, &maps.k, (int)panel * 64, y, &k_full[slot]);
+          ++kt;
+          if (vt >= 2 && !wait(&v_empty[slot], (vt / 2 - 1) & 1u)) break;
+          if (lane == 0) mbar_expect_tx(&v_full[slot], bytes);
+          __syncwarp();
+          if (mine) tma_2d(sv + slot * slot_bytes + dst, &maps.v, (int)panel * 64, y, &v_full[slot]);
+          ++vt;
+        }
+      }
+      // leave no copy in flight into shared memory that another CTA may get, whoever gives up
+      for (uint32_t i = kt > 2 ? kt - 2 : 0; i < kt; ++i) (void)mbar_wait(&k_full[i & 1u], (i / 2) & 1u);
+      for (uint32_t i = vt > 2 ? vt - 2 : 0; i < vt; ++i) (void)mbar_wait(&v_full[i & 1u], (i / 2) & 1u);
+    } else if (warp == 1) {
+      // ===== MMAs
+      constexpr uint32_t kType = sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+      const uint32_t idesc_s = (1u << 4) | (kType << 7) | (kType << 10) | ((kKeys >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
+      const uint32_t vcols = (hd + 15) / 16 * 16;
+      const uint32_t idesc_o = (1u << 4) | (kType << 7) | (kType << 10) | (1u << 16) | ((vcols >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
+      const uint64_t qd = umma_desc_sw128(sq), kd = umma_desc_sw128(sk), vd = umma_desc_mn128(sv);
+      const uint32_t steps = (hd + 15) / 16;
+      uint32_t kt = 0, items = 0, pc[2] = {0, 0};
+      auto scores = [&](uint32_t t, uint32_t slot) {
+        if (elect_one()) {
+          for (uint32_t e = 0; e < steps; ++e)
+            umma_f16_ss(tmem + t * kKeys, umma_desc_advance(qd, t * q_tile + (e >> 2) * kPanel + (e & 3u) * 32u),
+                        umma_desc_advance(kd, slot * slot_bytes + (e >> 2) * kPanel + (e & 3u) * 32u), idesc_s, e != 0 ? 1u : 0u);
+          umma_commit(&s_full[t]);
+        }
+        __syncwarp();
+      };
+      auto commit = [&](uint64_t* bar) {
+        if (elect_one()) umma_commit(bar);
+        __syncwarp();
+      };
+      while (ok && runs.next(a, plan, w, p)) {
+        if (!p.n_all) continue;
+        if (!wait(&q_full, items & 1u) || !wait(&k_full[kt & 1u], (kt / 2) & 1u)) break;
+        tc_fence_after_sync();
+        if (p.n[0]) scores(0, kt & 1u);
+        if (p.n[1]) scores(1, kt & 1u);
+        commit(&k_empty[kt & 1u]);
+        if (p.n_all == 1) commit(&q_empty);
+        for (uint32_t j = 0; j < p.n_all; ++j, ++kt) {
+          const uint32_t slot = kt & 1u, nslot = slot ^ 1u;
+          if (!wait(&v_full[slot], (kt / 2) & 1u)) break;
+          const uint32_t end = (p.s.tile0 + j + 1) * kKeys;
+          if (end > p.s.rq.len) {  // positions behind the request's end: their values weigh nothing, and must be numbers for that
+            const uint32_t from = p.s.rq.len - (end - kKeys);
+            for (uint32_t x = lane; x < (kKeys - from) * 8 * panels; x += 32) {
+              const uint32_t row = from + x / 8 % (kKeys - from), pn = x / 8 / (kKeys - from);
+              asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(sv + slot * slot_bytes + pn * kPanel + row * 128 + (x & 7u) * 16), "r"(0) : "memory");
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+          }
+          bool have_k = false;
+#pragma unroll
+          for (uint32_t t = 0; t < 2; ++t) {
+            if (ok && j < p.n[t]) {
+              if (!wait(&p_ready[t], pc[t] & 1u)) break;
+              ++pc[t];
+              tc_fence_after_sync();
+              if (elect_one()) {
+#pragma unroll
+                for (uint32_t e = 0; e < kKeys / 16; ++e)
+                  umma_f16_ts(tmem + kOutCol + t * 128, tmem + t * kKeys + e * 8, umma_desc_advance(vd, slot * slot_bytes + e * 2048u), idesc_o, (j | e) != 0 ? 1u : 0u);
+                if (j + 1 == p.n[t]) umma_commit(&o_full[t]);
+              }
+              __syncwarp();
+            }
+            if (ok && j + 1 < p.n[t]) {
+              if (!have_k) {
+                if (!wait(&k_full[nslot], ((kt + 1) / 2) & 1u)) break;
+                tc_fence_after_sync();
+                have_k = true;
+              }
+              scores(t, nslot);
+            }
+          }
+          if (!ok) break;
+          if (j + 1 < p.n_all) commit(&k_empty[nslot]);
+          if (j + 2 == p.n_all) commit(&q_empty);
+          commit(&v_empty[slot]);
+        }
+        ++items;
+      }
+      commit(&fin);  // nothing is left running when tensor memory is freed
+      if (!mbar_wait(&fin, 0)) s_abort = 1;
+    } else if (warp == 2) {
+      // ===== queries of the next item; rows behind its tokens hold whatever follows there
+      uint32_t items = 0;
+      while (ok && runs.next(a, plan, w, p)) {
+        if (!p.n_all) continue;
+        if (items && !wait(&q_empty, (items - 1) & 1u)) break;
+        const uint32_t tiles = p.tokens > plan.tile_tokens ? 2u : 1u, t = lane / panels, panel = lane % panels;
+        if (lane == 0) mbar_expect_tx(&q_full, tiles * panels * plan.tile_tokens * runs.rep * 128);
+        __syncwarp();
+        if (t < tiles)
+          tma_3d(sq + t * q_tile + panel * kPanel, &maps.q, (int)panel * 64, (int)(p.s.g * runs.rep), (int)(p.s.rq.t0 + p.token + t * plan.tile_tokens), &q_full);
+        ++items;
+      }
+      if (items) (void)mbar_wait(&q_full, (items - 1) & 1u);  // no copy in flight at the end
+    }
+  } else {
+    // ===== softmax: thread = row
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+    const uint32_t t = (warp - 4) >> 2, quarter = warp & 3u, rep = runs.rep, row = quarter * 32 + lane, mine = row / rep, head = row % rep;
+    const uint32_t lanes = (quarter * 32u) << 16, s_at = tmem + lanes + t * kKeys, o_at = tmem + lanes + kOutCol + t * 128;
+    const float c = a.scale * kLog2e;
+    Walk w = walk0;
+    Piece p;
+    uint32_t sc = 0, oc = 0;
+    bool ok = true;
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+      if (ok) ok = __all_sync(0xFFFFFFFFu, !s_abort && mbar_wait(bar, parity));
+      if (!ok) s_abort = 1;
+      tc_fence_after_sync();
+      return ok;
+    };
+    if (tid == kThreads - 1 && plan.cuts) plan.cuts[blockIdx.x] = {0, 0, 0, 0};
+    while (runs.next(a, plan, w, p)) {
+      const uint32_t n = p.n[t], token = t * plan.tile_tokens + mine;  // of the item
+      const bool live = mine < plan.tile_tokens && token < p.tokens;
+      const uint32_t pos = p.s.rq.cached + p.token + min(token, p.tokens - 1), low = paged_low(pos, a.window);
+      float m = -INFINITY, l = 0.0f;
+      for (uint32_t j = 0; j < n; ++j, ++sc) {
+        if (!wait(&s_full[t], sc & 1u)) break;
+        float s[kKeys];
+#pragma unroll
+        for (int i = 0; i < kKeys; i += 32) tmem_ld32(s_at + i, s + i);
+        const uint32_t key0 = (p.s.tile0 + j) * kKeys;
+        if (!__all_sync(0xFFFFFFFFu, key0 >= low && key0 + kKeys <= pos + 1)) {
+          const int hi = (int)min(pos + 1 > key0 ? pos + 1 - key0 : 0u, (uint32_t)kKeys), lo = low > key0 ? (int)min(low - key0, (uint32_t)kKeys) : 0;
+#pragma unroll
+          for (int i = 0; i < kKeys; ++i) s[i] = i < hi && i >= lo ? s[i] : -INFINITY;
+        }
+        float x[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+        for (int i = 4; i < kKeys; i += 4) {
+          x[0] = fmaxf(x[0], s[i]); x[1] = fmaxf(x[1], s[i + 1]); x[2] = fmaxf(x[2], s[i + 2]); x[3] = fmaxf(x[3], s[i + 3]);
+        }
+        const float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) * c;  // c > 0
+        if (__any_sync(0xFFFFFFFFu, mx > m + kGrowth)) {
+          const float m_new = fmaxf(m, mx), f = m == -INFINITY ? 0.0f : exp2_of(m - m_new);
+          m = m_new;
+          l *= f;
+          if (j > 0) {  // the products before have finished: this tile's scores came after them
+#pragma unroll
+            for (int i = 0; i < 128; i += 32) {
+              if (i >= (int)hd) break;
+              float o[32];
+              tmem_ld32(o_at + i, o);
+#pragma unroll
+              for (int y = 0; y < 32; ++y) o[y] *= f;
+              tmem_st32(o_at + i, o);
+            }
+          }
+        }
+        const float base = m == -INFINITY ? 0.0f : m;
+        float add[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int i = 0; i < kKeys; i += 32) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int y = 0; y < 32; y += 2) {
+            const float e0 = exp2_of(fmaf(s[i + y], c, -base)), e1 = exp2_of(fmaf(s[i + y + 1], c, -base));
+            add[y & 2] += e0;
+            add[(y & 2) + 1] += e1;
+            pk[y / 2] = pack2<T>(e0, e1);
+          }
+          tmem_st16(s_at + i / 2, pk);
+        }
+        l += (add[0] + add[1]) + (add[2] + add[3]);
+        tmem_st_wait();
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_ready[t]);
+      }
+      if (n && ok) { wait(&o_full[t], oc & 1u); ++oc; }
+      // ---- the rows' results: out, or a part of an item
+      const bool cut = p.cut_begin || p.cut_end;
+      float* part = plan.parts + ((size_t)blockIdx.x * 2 + (p.cut_begin ? 0 : 1)) * plan.part_floats;
+      if (tid == kThreads - 1 && p.cut_end && !p.cut_begin)
+        plan.cuts[blockIdx.x] = {(uint32_t)((p.item_u + p.tiles - 1) / per), p.s.rq.t0 + p.token, p.tokens, p.s.g};
+      T* dst = static_cast<T*>(a.out) + (size_t)(p.s.rq.t0 + p.token + (live ? token : 0u)) * a.out_ld + (size_t)(p.s.g * rep + head) * hd;
+      if (ok) {
+        bool fine = isfinite(l);
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        const uint32_t cols = (hd + 31) / 32;
+        for (uint32_t i = 0; i < cols; ++i) {
+          float o[32];
+          if (n) tmem_ld32(o_at + i * 32, o);
+          else {
+#pragma unroll
+            for (int y = 0; y < 32; ++y) o[y] = 0.0f;
+          }
+#pragma unroll
+          for (int y = 0; y < 32; y += 8) {
+            if (i * 32 + y >= hd) break;
+#pragma unroll
+            for (int z = 0; z < 8; ++z) fine = fine && isfinite(o[y + z]);
+            if (live && !cut) {
+              const uint4 v = make_uint4(pack2<T>(o[y] * inv, o[y + 1] * inv), pack2<T>(o[y + 2] * inv, o[y + 3] * inv), pack2<T>(o[y + 4] * inv, o[y + 5] * inv),
+                                         pack2<T>(o[y + 6] * inv, o[y + 7] * inv));
+              *reinterpret_cast<uint4*>(dst + i * 32 + y) = v;
+            }
+            if (live && cut) {
+              float4* q = reinterpret_cast<float4*>(part + ((size_t)(i * 8 + y / 4) * kItemRows + t * kRows + row) * 4);
+              q[0] = make_float4(o[y], o[y + 1], o[y + 2], o[y + 3]);
+              q[kItemRows] = make_float4(o[y + 4], o[y + 5], o[y + 6], o[y + 7]);
+            }
+          }
+        }
+        // rows that are not finite, key by key
+        for (uint32_t bad = __ballot_sync(0xFFFFFFFFu, live && !fine); bad; bad &= bad - 1) {
+          const uint32_t who = (uint32_t)__ffs((int)bad) - 1, which = quarter * 32 + who, x = p.s.row0 + t * plan.tile_tokens * rep + which;
+          float* tmp = s_again[warp - 4];
+          float m2, l2;
+          row_again<T>(a, p.s, rep, x, p.s.tile0 * kKeys, p.s.tile1 * kKeys, tmp, m2, l2);
+          __syncwarp();
+          T* d2 = static_cast<T*>(a.out) + (size_t)(p.s.rq.t0 + x / rep) * a.out_ld + (size_t)(p.s.g * rep + x % rep) * hd;
+          for (uint32_t e = lane; e < hd; e += 32) {
+            if (cut) part[((size_t)(e / 4) * kItemRows + t * kRows + which) * 4 + (e & 3u)] = tmp[e];
+            else d2[e] = from_f32<T>(l2 == 0.0f ? 0.0f : tmp[e] / l2);
+          }
+          __syncwarp();
+          if (lane == who) { m = m2; l = l2; }
+        }
+        if (cut && live) {
+          part[hd * kItemRows + t * kRows + row] = m;
+          part[(hd + 1) * kItemRows + t * kRows + row] = l;
+        }
+      }
+    }
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  if (s_abort && tid == 0 && a.status) atomicCAS(a.status, 0, 3);
+  if (warp == 1) tmem_dealloc(tmem, 512);
+}
+
+// grid (CTAs of chunk_kernel, groups of 32 rows): the parts of an item, in their order.
+constexpr int kJoinThreads = 128;
+template <typename T>
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const PagedAttn a, const TcPlan plan) {
+  grid_dependency_wait();
+  grid_launch_dependents();
+  const Cut cut = plan.cuts[blockIdx.x];
+  if (!cut.last) return;
+  const uint32_t hd = a.pool.hd, rep = a.H / a.pool.KV, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row = blockIdx.y * 32 + lane;
+  const uint32_t tile = row / kRows, mine = row % kRows / rep, token = tile * plan.tile_tokens + mine;
+  if (mine >= plan.tile_tokens || token >= cut.tokens) return;
+  auto part_of = [&](uint32_t i) { return plan.parts + ((size_t)i * 2 + (i == blockIdx.x ? 1 : 0)) * plan.part_floats; };
+  float m = -INFINITY, l = 0.0f;
+#pragma unroll 8
+  for (uint32_t i = blockIdx.x; i <= cut.last; ++i) m = fmaxf(m, part_of(i)[hd * kItemRows + row]);
+#pragma unroll 8
+  for (uint32_t i = blockIdx.x; i <= cut.last; ++i) {
+    const float mp = part_of(i)[hd * kItemRows + row];
+    l = fmaf(part_of(i)[(hd + 1) * kItemRows + row], mp == -INFINITY ? 0.0f : exp2_of(mp - m), l);
+  }
+  T* dst = static_cast<T*>(a.out) + (size_t)(cut.token + token) * a.out_ld + (size_t)(cut.g * rep + row % kRows % rep) * hd;
+  for (uint32_t e = 4 * warp; e < hd; e += 16) {
+    float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 8
+    for (uint32_t i = blockIdx.x; i <= cut.last; ++i) {
+      const float mp = part_of(i)[hd * kItemRows + row], f = mp == -INFINITY ? 0.0f : exp2_of(mp - m);
+      const float4 v = *reinterpret_cast<const float4*>(part_of(i) + ((size_t)(e / 4) * kItemRows + row) * 4);
+      o[0] = fmaf(v.x, f, o[0]); o[1] = fmaf(v.y, f, o[1]); o[2] = fmaf(v.z, f, o[2]); o[3] = fmaf(v.w, f, o[3]);
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    *reinterpret_cast<uint2*>(dst + e) = make_uint2(pack2<T>(o[0] * inv, o[1] * inv), pack2<T>(o[2] * inv, o[3] * inv));
+  }
+}
+
+typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                             const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeFn encode_fn() {
+  static EncodeFn fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult st;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &st) != cudaSuccess || st != cudaDriverEntryPointSuccess) p = nullptr;
+    return (EncodeFn)p;
+  }();
+  return fn;
+}
+// The queries [tokens][heads][hd], in boxes of 64 elements, a key head's query heads and a row tile's tokens; what lies outside reads as zero.
+CUresult encode_q(EncodeFn fn, CUtensorMap* map, const PagedAttn& a, uint32_t rep, uint32_t tile_tokens) {
+  const cuuint64_t dims[3] = {a.pool.hd, a.H, a.tokens}, strides[2] = {(cuuint64_t)a.pool.hd * 2, (cuuint64_t)a.q_ld * 2};
+  const cuuint32_t box[3] = {64, rep, tile_tokens}, one[3] = {1, 1, 1};
+  return fn(map, a.pool.dtype == RUAI_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(a.q), dims, strides, box, one,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+}
+// A pool's rows (page, key head, position in the page) of hd elements, in boxes of box_rows x 64; elements past hd read as zero.
+CUresult encode(EncodeFn fn, CUtensorMap* map, const PagedPool& p, void* base, uint32_t box_rows) {
+  const cuuint64_t dims[2] = {p.hd, ((cuuint64_t)p.pages * p.KV) << p.page_log2}, strides[1] = {(cuuint64_t)p.hd * 2};
+  const cuuint32_t box[2] = {64, box_rows}, one[2] = {1, 1};
+  return fn(map, p.dtype == RUAI_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, base, dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+}
+
+template <typename T>
+cudaError_t launch_chunk(ruai_ctx* c, const PagedAttn& a, const TcPlan& plan, const Maps& maps) {
+  const uint32_t panels = (a.pool.hd + 63) / 64;
+  const int smem = 6 * (int)panels * kPanel + 1024, most = 12 * kPanel + 1024;
+  static bool done[64] = {};
+  if (!done[c->ordinal & 63]) {
+    cudaError_t e = cudaFuncSetAttribute(chunk_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+    if (e != cudaSuccess) return e;
+    done[c->ordinal & 63] = true;
+  }
+  // one CTA per SM: each takes all of tensor memory
+  const cudaError_t e = ruai_launch(c, chunk_kernel<T>, dim3(c->sm_count), dim3(kThreads), (size_t)std::max(smem, 120 * 1024), true, a, plan, maps);
+  if (e != cudaSuccess || !plan.cuts) return e;
+  return ruai_launch(c, join_kernel<T>, dim3(c->sm_count, kItemRows / 32), dim3(kJoinThreads), 0, true, a, plan);
+}
+
+}  // namespace
+
+int ruai_paged_attention_tc(ruai_ctx* c, const PagedAttn& a, uint32_t rows_over) {
+  const PagedPool& p = a.pool;
+  // heads narrower than a copied box, and scores that shrink with their product, stay on attn_paged.cu
+  const uint32_t rep = a.H / p.KV;
+  if (!c->use_tc || p.dtype == RUAI_F32 || p.hd < 64 || p.hd > 128 || rep > (uint32_t)kRows || !(a.scale > 0.0f)) return 0;
+  EncodeFn fn = encode_fn();
+  if (!fn) { ruai_fail(c, RUAI_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver"); return -1; }
+  TcPlan plan = {};
+  plan.rows_over = rows_over;
+  plan.box_rows = std::min(1u << p.page_log2, (uint32_t)kKeys);
+  plan.part_floats = (p.hd + 2) * kItemRows;
+  plan.tile_tokens = kRows / rep;
+  Maps maps;
+  const CUresult rq = encode_q(fn, &maps.q, a, rep, plan.tile_tokens), rk = encode(fn, &maps.k, p, p.k, plan.box_rows), rv = encode(fn, &maps.v, p, p.v, plan.box_rows);
+  if (rq != CUDA_SUCCESS || rk != CUDA_SUCCESS || rv != CUDA_SUCCESS) {
+    ruai_fail(c, RUAI_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d, %d, %d) for %u pages of %u heads of %u", (int)rq, (int)rk, (int)rv, p.pages, p.KV, p.hd);
+    return -1;
+  }
+  // parts of cut items: two per CTA.  Nothing may be allocated while the stream is captured; items then stay whole
+  const size_t parts = 2 * (size_t)c->sm_count * plan.part_floats * sizeof(float), need = parts + c->sm_count * sizeof(Cut), held = c->partial_bytes;
+  bool cuts = true;
+  if (need > held) {
+    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(c->stream, &capture) != cudaSuccess || capture != cudaStreamCaptureStatusNone) cuts = false;
+    else if (ruai_ctx_reserve(c, need, 0) != RUAI_OK) {  // no memory for the parts: the scratch as it was
+      (void)cudaGetLastError();
+      cuts = false;
+      if (ruai_ctx_reserve(c, held, 0) != RUAI_OK) return -1;
+    }
+  }
+  plan.parts = c->partial;
+  plan.cuts = cuts ? reinterpret_cast<Cut*>(reinterpret_cast<unsigned char*>(c->partial) + parts) : nullptr;
+  const cudaError_t e = p.dtype == RUAI_F16 ? launch_chunk<__half>(c, a, plan, maps) : launch_chunk<__nv_bfloat16>(c, a, plan, maps);
+  if (e != cudaSuccess) { ruai_fail(c, RUAI_ERR_CUDA, "attention over pages: %s", cudaGetErrorString(e)); return -1; }
+  return 1;
+}

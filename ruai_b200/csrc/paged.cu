@@ -310,6 +310,7 @@ RUAI_API int ruai_paged_attention(ruai_ctx* c, int dtype, const void* q, uint32_
     return ruai_fail(c, RUAI_ERR_SHAPE, "ruai_paged_attention: %u requests of up to %u pages, %u tokens: up to %u and %u", R, table_ld, tokens, kPlanRowsMax, kPlanTokensMax);
   if (most_len >= (1u << 30) || !(scale == scale)) return ruai_fail(c, RUAI_ERR_ARG, "ruai_paged_attention: lengths of up to %u, scale %f", most_len, (double)scale);
   if (!R || !tokens || !most_fresh) return RUAI_OK;
+  if (a.most_fresh > tokens) a.most_fresh = tokens;  // no request has more
   DeviceGuard g(c->ordinal);
   return ruai_paged_attention_launch(c, a);
 }
