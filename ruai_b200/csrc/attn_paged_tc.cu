@@ -3,7 +3,8 @@
 // An item is two tiles of up to 128 rows (token, query head; whole tokens) of one request and key head, over the keys that any of them
 // sees, 128 at a time.  One warp copies a tile's keys and values page by page (TMA boxes of a page's rows, so that pages lie in shared
 // memory as one tile, 128-byte swizzle); one issues the MMAs, S_t = Q_t K^T and O_t += P_t V in turn for both row tiles, so that one
-// tile's products run beside the other's softmax; one copies the next item's queries; two warpgroups are the softmax, a thread per row.  Scores,
+// tile's products run beside the other's softmax; one finds the items
+// for the others; two warpgroups are the softmax, a thread per row.  Scores,
 // probabilities (written over the scores, rounded once to the values' type) and outputs stay in tensor memory: 2 x (128 + 128)
 // columns.  Outputs are rescaled only where a row's maximum has grown by more than 2^8 since the last time: weights of up to 256 are as exact
 // as those of up to 1, and nearly every tile leaves the outputs where they are.
@@ -28,7 +29,8 @@ constexpr int kPanel = 128 * 128;  // bytes of 128 rows of 64 elements
 constexpr int kThreads = 384;
 constexpr uint32_t kOutCol = 256;  // tensor memory: scores of both tiles, then their outputs
 constexpr float kGrowth = 8.0f;
-constexpr int kTilesLeast = 4;  // of a run: a part costs as much as a few tiles
+constexpr int kItemCost = 2;    // units of a run that an item takes beside its tiles: its queries' and outputs' way, 5500 clocks where a tile takes 3100
+constexpr int kTilesLeast = 6;  // units of a run: a part costs as much as a few tiles
 
 struct alignas(64) Maps { CUtensorMap q, k, v; };
 
@@ -51,21 +53,33 @@ __device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* map, int
                "r"(smem_u32(bar))
                : "memory");
 }
-// 32 columns of this thread's lane, loaded when the call returns.
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float* v) {
-  uint32_t r[32];
+// 32 columns of this thread's lane; the registers may be used once tmem_ld32_end has returned.
+__device__ __forceinline__ void tmem_ld32_start(uint32_t taddr, uint32_t (&r)[32]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, "
-      "%22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n\ttcgen05.wait::ld.sync.aligned;"
+      "%22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
         "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
         "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(taddr)
       : "memory");
+}
+__device__ __forceinline__ void tmem_ld32_end(uint32_t (&r)[32]) {  // nothing that uses them can be placed ahead of it
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]),
+                 "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]),
+                 "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+               :
+               : "memory");
+}
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
+  uint32_t r[32];
+  tmem_ld32_start(taddr, r);
+  tmem_ld32_end(r);
 #pragma unroll
   for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const float* v) {
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const float (&v)[32]) {
   uint32_t r[32];
 #pragma unroll
   for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(v[i]);
@@ -86,6 +100,22 @@ __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.
 // An operand whose rows are the sum's index (values [key][element]): panels of 64 elements kPanel apart, eight keys 1024 bytes apart.
 __device__ __forceinline__ uint64_t umma_desc_mn128(uint32_t addr) {
   return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)(kPanel >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+// Two f32 operations in one instruction.
+__device__ __forceinline__ unsigned long long pair_of(float a, float b) {
+  unsigned long long r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(__float_as_uint(a)), "r"(__float_as_uint(b)));
+  return r;
+}
+__device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigned long long b, unsigned long long c) {
+  unsigned long long r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ unsigned long long add2(unsigned long long a, unsigned long long b) {
+  unsigned long long r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
 }
 template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b);
 template <> __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
@@ -122,7 +152,7 @@ struct Runs {
     if (q.fresh * rep <= rows_over) return 0;
     unsigned long long n = 0;
     uint32_t skip;
-    for (uint32_t b = 0; b * tokens < q.fresh; ++b) n += tiles(a, q, b, skip);
+    for (uint32_t b = 0; b * tokens < q.fresh; ++b) n += tiles(a, q, b, skip) + kItemCost;
     return n * a.pool.KV;
   }
   __device__ bool next(const PagedAttn& a, const TcPlan& plan, Walk& w, Piece& p) const {
@@ -132,10 +162,11 @@ struct Runs {
       if (q.fresh * rep <= rows_over || w.b * tokens >= q.fresh) { ++w.r; w.b = 0; continue; }
       uint32_t skip;
       const uint32_t n = tiles(a, q, w.b, skip);
-      const unsigned long long all = (unsigned long long)n * a.pool.KV;
+      const unsigned long long all = (unsigned long long)(n + kItemCost) * a.pool.KV;
       if (w.u >= w.base + all) { w.base += all; ++w.b; continue; }
-      const uint32_t g = (uint32_t)(w.u - w.base) / n;  // fewer than 2^32 units in a block of rows: keys / 128 x key heads
-      p.item_u = w.base + (unsigned long long)g * n;
+      const uint32_t g = (uint32_t)(w.u - w.base) / (n + kItemCost);  // fewer than 2^32 units in a block of rows: keys / 128 x key heads
+      p.item_u = w.base + (unsigned long long)g * (n + kItemCost) + kItemCost;
+      if (w.u < p.item_u) { w.u = p.item_u; continue; }
       if (!plan.cuts && w.u != p.item_u) { w.u = p.item_u + n; continue; }  // the CTA before has the whole item
       p.tiles = n;
       p.s.rq = q; p.s.r = w.r; p.s.g = g;
@@ -164,25 +195,31 @@ struct Runs {
   }
 };
 
+constexpr int kPieces = 3;  // pieces that the scheduling warp is ahead
+constexpr int kSoftWarps = 8, kControlWarps = 4;
+constexpr int kStage = 32 * 64;  // bytes in which a softmax warp turns 32 rows of 32 columns around for the output
+
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const PagedAttn a, const TcPlan plan, const __grid_constant__ Maps maps) {
   extern __shared__ unsigned char smem_raw[];
-  __shared__ __align__(8) uint64_t q_full, q_empty, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_ready[2], o_full[2], fin;
+  __shared__ __align__(8) uint64_t piece_full[kPieces], piece_empty[kPieces], q_full, q_empty, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_ready[2][2], o_full[2], v_last, v_cleared, fin;
+  __shared__ Piece s_piece[kPieces];
   __shared__ uint32_t s_tmem, s_r;
   __shared__ volatile int s_abort;
   __shared__ unsigned long long s_part[kThreads / 32], s_base;
-  __shared__ float s_again[8][128];
+  __shared__ float s_again[kSoftWarps][128];
   const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, hd = a.pool.hd, panels = (hd + 63) / 64, plog = a.pool.page_log2;
   unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   const uint32_t q_tile = panels * kPanel, slot_bytes = panels * kPanel;
   const uint32_t sq = smem_u32(smem), sk = sq + 2 * q_tile, sv = sk + 2 * slot_bytes;
 
   if (tid == 0) {
-    mbar_init(&q_full, 1); mbar_init(&q_empty, 1); mbar_init(&fin, 1);
+    mbar_init(&q_full, 1); mbar_init(&q_empty, 1); mbar_init(&v_last, 1); mbar_init(&v_cleared, 1); mbar_init(&fin, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&k_full[i], 1); mbar_init(&k_empty[i], 1); mbar_init(&v_full[i], 1); mbar_init(&v_empty[i], 1);
-      mbar_init(&s_full[i], 1); mbar_init(&p_ready[i], 4); mbar_init(&o_full[i], 1);
+      mbar_init(&s_full[i], 1); mbar_init(&p_ready[i][0], 4); mbar_init(&p_ready[i][1], 4); mbar_init(&o_full[i], 1);
     }
+    for (int i = 0; i < kPieces; ++i) { mbar_init(&piece_full[i], 1); mbar_init(&piece_empty[i], kSoftWarps + 2); }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     s_abort = 0;
   }
@@ -197,7 +234,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const PagedAttn a, c
 
   // ---- this CTA's run of units (a unit: a tile of keys of an item)
   Runs runs = {0, a.H / a.pool.KV, plan.rows_over, 2 * plan.tile_tokens};
-  Walk walk0 = {0, 0, 0, 0};
+  Walk walk = {0, 0, 0, 0};
   unsigned long long per;
   {
     const uint32_t each = (a.R + kThreads - 1) / kThreads, ra = min(tid * each, a.R), rb = min(ra + each, a.R);
@@ -221,122 +258,157 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const PagedAttn a, c
       total += s_part[w];
     }
     per = max((total + gridDim.x - 1) / gridDim.x, (unsigned long long)kTilesLeast);
-    walk0.u = per * blockIdx.x;
-    runs.u1 = min(walk0.u + per, total);
-    if (walk0.u < runs.u1 && before <= walk0.u && walk0.u < before + mine) {
+    walk.u = per * blockIdx.x;
+    runs.u1 = min(walk.u + per, total);
+    if (walk.u < runs.u1 && before <= walk.u && walk.u < before + mine) {
       unsigned long long base = before;
       for (uint32_t r = ra; r < rb; ++r) {
         PagedRequest q;
         paged_request(a, r, q);
         const unsigned long long n = runs.units(a, q);
-        if (walk0.u < base + n) { s_r = r; s_base = base; break; }
+        if (walk.u < base + n) { s_r = r; s_base = base; break; }
         base += n;
       }
     }
     __syncthreads();
-    walk0.r = s_r;
-    walk0.base = s_base;
+    walk.r = s_r;
+    walk.base = s_base;
   }
 
-  if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 96;");
-    Walk w = walk0;
+  bool ok = true;
+  auto wait = [&](uint64_t* bar, uint32_t parity) {  // the same answer for the whole warp
+    if (ok) ok = __all_sync(0xFFFFFFFFu, !s_abort && mbar_wait(bar, parity));
+    if (!ok) s_abort = 1;
+    return ok;
+  };
+  uint32_t pieces = 0;
+  auto next = [&](Piece& p) {  // the next piece that the scheduling warp has found; false behind the last one
+    const uint32_t slot = pieces % kPieces;
+    if (!wait(&piece_full[slot], (pieces / kPieces) & 1u)) return false;
+    p = s_piece[slot];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&piece_empty[slot]);
+    ++pieces;
+    return p.tiles != 0;
+  };
+
+  if (warp < (uint32_t)kControlWarps) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
+  if (warp == 0) {
+    // ===== an item's queries, then its keys and values, a lane per box; rows behind the item's tokens hold whatever follows there
+    const uint32_t boxes = kKeys / plan.box_rows, box = lane % boxes, panel = lane / boxes;
+    const uint32_t dst = panel * kPanel + box * plan.box_rows * 128;
+    uint32_t kt = 0, vt = 0, items = 0, lasts = 0;  // asked for
     Piece p;
-    bool ok = true;
-    auto wait = [&](uint64_t* bar, uint32_t parity) {  // the same answer for the whole warp
-      if (ok) ok = __all_sync(0xFFFFFFFFu, !s_abort && mbar_wait(bar, parity));
-      if (!ok) s_abort = 1;
-      return ok;
-    };
-    if (warp == 0) {
-      // ===== keys and values, a lane per box
-      const uint32_t boxes = kKeys / plan.box_rows, box = lane % boxes, panel = lane / boxes;
-      const uint32_t dst = panel * kPanel + box * plan.box_rows * 128;
-      uint32_t kt = 0, vt = 0;  // tiles asked for
-      while (ok && runs.next(a, plan, w, p)) {
-        for (uint32_t j = 0; j < p.n_all; ++j) {
-          const uint32_t key = (p.s.tile0 + j) * kKeys + box * plan.box_rows, slot = kt & 1u;
-          int32_t pg = -1;
-          if (key < p.s.rq.len) pg = paged_page(a, p.s.r, key);
-          const uint32_t bytes = __popc(__ballot_sync(0xFFFFFFFFu, lane < boxes && pg >= 0)) * panels * plan.box_rows * 128;
-          const int y = pg >= 0 ? (int)((((uint32_t)pg * a.pool.KV + p.s.g) << plog) + (key & ((1u << plog) - 1u))) : 0;
-          const bool mine = panel < panels && pg >= 0;
-          if (kt >= 2 && !wait(&k_empty[slot], (kt / 2 - 1) & 1u)) break;
-          if (lane == 0) mbar_expect_tx(&k_full[slot], bytes);
-          __syncwarp();
-          if (mine) tma_2d(sk + slot * slot_bytes + dst, &maps.k, (int)panel * 64, y, &k_full[slot]);
-          ++kt;
-          if (vt >= 2 && !wait(&v_empty[slot], (vt / 2 - 1) & 1u)) break;
-          if (lane == 0) mbar_expect_tx(&v_full[slot], bytes);
-          __syncwarp();
-          if (mine) tma_2d(sv + slot * slot_bytes + dst, &maps.v, (int)panel * 64, y, &v_full[slot]);
-          ++vt;
-        }
+    while (ok && next(p)) {
+      if (!p.n_all) continue;
+      if (items && !wait(&q_empty, (items - 1) & 1u)) break;
+      {
+        const uint32_t tiles = p.tokens > plan.tile_tokens ? 2u : 1u, t = lane / panels, pn = lane % panels;
+        if (lane == 0) mbar_expect_tx(&q_full, tiles * panels * plan.tile_tokens * runs.rep * 128);
+        __syncwarp();
+        if (t < tiles) tma_3d(sq + t * q_tile + pn * kPanel, &maps.q, (int)pn * 64, (int)(p.s.g * runs.rep), (int)(p.s.rq.t0 + p.token + t * plan.tile_tokens), &q_full);
+        ++items;
       }
-      // leave no copy in flight into shared memory that another CTA may get, whoever gives up
-      for (uint32_t i = kt > 2 ? kt - 2 : 0; i < kt; ++i) (void)mbar_wait(&k_full[i & 1u], (i / 2) & 1u);
-      for (uint32_t i = vt > 2 ? vt - 2 : 0; i < vt; ++i) (void)mbar_wait(&v_full[i & 1u], (i / 2) & 1u);
-    } else if (warp == 1) {
-      // ===== MMAs
-      constexpr uint32_t kType = sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
-      const uint32_t idesc_s = (1u << 4) | (kType << 7) | (kType << 10) | ((kKeys >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
-      const uint32_t vcols = (hd + 15) / 16 * 16;
-      const uint32_t idesc_o = (1u << 4) | (kType << 7) | (kType << 10) | (1u << 16) | ((vcols >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
-      const uint64_t qd = umma_desc_sw128(sq), kd = umma_desc_sw128(sk), vd = umma_desc_mn128(sv);
+      for (uint32_t j = 0; j < p.n_all; ++j) {
+        const uint32_t key = (p.s.tile0 + j) * kKeys + box * plan.box_rows, slot = kt & 1u;
+        int32_t pg = -1;
+        if (key < p.s.rq.len) pg = paged_page(a, p.s.r, key);
+        const uint32_t bytes = __popc(__ballot_sync(0xFFFFFFFFu, lane < boxes && pg >= 0)) * panels * plan.box_rows * 128;
+        const int y = pg >= 0 ? (int)((((uint32_t)pg * a.pool.KV + p.s.g) << plog) + (key & ((1u << plog) - 1u))) : 0;
+        const bool mine = panel < panels && pg >= 0;
+        if (kt >= 2 && !wait(&k_empty[slot], (kt / 2 - 1) & 1u)) break;
+        if (lane == 0) mbar_expect_tx(&k_full[slot], bytes);
+        __syncwarp();
+        if (mine) tma_2d(sk + slot * slot_bytes + dst, &maps.k, (int)panel * 64, y, &k_full[slot]);
+        ++kt;
+        if (vt >= 2 && !wait(&v_empty[slot], (vt / 2 - 1) & 1u)) break;
+        if (lane == 0) mbar_expect_tx(&v_full[slot], bytes);
+        __syncwarp();
+        if (mine) tma_2d(sv + slot * slot_bytes + dst, &maps.v, (int)panel * 64, y, &v_full[slot]);
+        ++vt;
+      }
+      const uint32_t end = (p.s.tile0 + p.n_all) * kKeys;
+      if (ok && end > p.s.rq.len) {  // positions behind the request's end: their values weigh nothing, and must be numbers for that
+        if (!wait(&v_last, lasts++ & 1u)) break;  // they have come
+        for (uint32_t r = p.s.rq.len - (end - kKeys) + (lane >> 3); r < (uint32_t)kKeys; r += 4)
+          for (uint32_t pn = 0; pn < panels; ++pn)
+            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(sv + ((vt - 1) & 1u) * slot_bytes + pn * kPanel + r * 128 + (lane & 7u) * 16), "r"(0) : "memory");
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&v_cleared);
+      }
+    }
+    if (items) (void)mbar_wait(&q_full, (items - 1) & 1u);
+    // leave no copy in flight into shared memory that another CTA may get, whoever gives up
+    for (uint32_t i = kt > 2 ? kt - 2 : 0; i < kt; ++i) (void)mbar_wait(&k_full[i & 1u], (i / 2) & 1u);
+    for (uint32_t i = vt > 2 ? vt - 2 : 0; i < vt; ++i) (void)mbar_wait(&v_full[i & 1u], (i / 2) & 1u);
+  } else if (warp == 1) {
+    // ===== MMAs
+    constexpr uint32_t kType = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+    const uint32_t idesc_s = (1u << 4) | (kType << 7) | (kType << 10) | ((kKeys >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
+    const uint32_t vcols = (hd + 15) / 16 * 16;
+    const uint32_t idesc_o = (1u << 4) | (kType << 7) | (kType << 10) | (1u << 16) | ((vcols >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
+    // One thread for all of it: a warp that votes and elects between the products takes 100 clocks an MMA, the tensor core 64.
+    if (elect_one()) {
+      const uint64_t qd[2] = {umma_desc_sw128(sq), umma_desc_sw128(sq + q_tile)}, kd[2] = {umma_desc_sw128(sk), umma_desc_sw128(sk + slot_bytes)},
+                     vd[2] = {umma_desc_mn128(sv), umma_desc_mn128(sv + slot_bytes)};
       const uint32_t steps = (hd + 15) / 16;
-      uint32_t kt = 0, items = 0, pc[2] = {0, 0};
+      uint32_t kt = 0, items = 0, pc[2] = {0, 0}, cleared = 0;
+      auto wait1 = [&](uint64_t* bar, uint32_t parity) {
+        if (ok && !mbar_wait(bar, parity)) { s_abort = 1; ok = false; }
+        return ok;
+      };
       auto scores = [&](uint32_t t, uint32_t slot) {
-        if (elect_one()) {
-          for (uint32_t e = 0; e < steps; ++e)
-            umma_f16_ss(tmem + t * kKeys, umma_desc_advance(qd, t * q_tile + (e >> 2) * kPanel + (e & 3u) * 32u),
-                        umma_desc_advance(kd, slot * slot_bytes + (e >> 2) * kPanel + (e & 3u) * 32u), idesc_s, e != 0 ? 1u : 0u);
-          umma_commit(&s_full[t]);
+        const uint64_t q = qd[t], k = slot ? kd[1] : kd[0];
+#pragma unroll
+        for (uint32_t e = 0; e < 8; ++e) {
+          if (e >= steps) break;
+          umma_f16_ss(tmem + t * kKeys, umma_desc_advance(q, (e >> 2) * kPanel + (e & 3u) * 32u), umma_desc_advance(k, (e >> 2) * kPanel + (e & 3u) * 32u), idesc_s, e != 0 ? 1u : 0u);
         }
-        __syncwarp();
+        umma_commit(&s_full[t]);
       };
-      auto commit = [&](uint64_t* bar) {
-        if (elect_one()) umma_commit(bar);
-        __syncwarp();
-      };
-      while (ok && runs.next(a, plan, w, p)) {
-        if (!p.n_all) continue;
-        if (!wait(&q_full, items & 1u) || !wait(&k_full[kt & 1u], (kt / 2) & 1u)) break;
+      for (; ok; ++pieces) {
+        const uint32_t ps = pieces % kPieces;
+        if (!wait1(&piece_full[ps], (pieces / kPieces) & 1u)) break;
+        const uint32_t n0 = s_piece[ps].n[0], n1 = s_piece[ps].n[1], n = max(n0, n1), stop = s_piece[ps].tiles == 0;
+        const bool tail = (s_piece[ps].s.tile0 + n) * kKeys > s_piece[ps].s.rq.len;
+        mbar_arrive(&piece_empty[ps]);
+        if (stop) break;
+        if (!n) continue;
+        if (!wait1(&q_full, items & 1u) || !wait1(&k_full[kt & 1u], (kt / 2) & 1u)) break;
         tc_fence_after_sync();
-        if (p.n[0]) scores(0, kt & 1u);
-        if (p.n[1]) scores(1, kt & 1u);
-        commit(&k_empty[kt & 1u]);
-        if (p.n_all == 1) commit(&q_empty);
-        for (uint32_t j = 0; j < p.n_all; ++j, ++kt) {
+        if (n0) scores(0, kt & 1u);
+        if (n1) scores(1, kt & 1u);
+        umma_commit(&k_empty[kt & 1u]);
+        if (n == 1) umma_commit(&q_empty);
+        for (uint32_t j = 0; j < n; ++j, ++kt) {
           const uint32_t slot = kt & 1u, nslot = slot ^ 1u;
-          if (!wait(&v_full[slot], (kt / 2) & 1u)) break;
-          const uint32_t end = (p.s.tile0 + j + 1) * kKeys;
-          if (end > p.s.rq.len) {  // positions behind the request's end: their values weigh nothing, and must be numbers for that
-            const uint32_t from = p.s.rq.len - (end - kKeys);
-            for (uint32_t x = lane; x < (kKeys - from) * 8 * panels; x += 32) {
-              const uint32_t row = from + x / 8 % (kKeys - from), pn = x / 8 / (kKeys - from);
-              asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(sv + slot * slot_bytes + pn * kPanel + row * 128 + (x & 7u) * 16), "r"(0) : "memory");
-            }
-            fence_proxy_async_smem();
-            __syncwarp();
+          if (!wait1(&v_full[slot], (kt / 2) & 1u)) break;
+          if (tail && j + 1 == n) {
+            mbar_arrive(&v_last);
+            if (!wait1(&v_cleared, cleared++ & 1u)) break;
           }
           bool have_k = false;
 #pragma unroll
           for (uint32_t t = 0; t < 2; ++t) {
-            if (ok && j < p.n[t]) {
-              if (!wait(&p_ready[t], pc[t] & 1u)) break;
-              ++pc[t];
-              tc_fence_after_sync();
-              if (elect_one()) {
+            const uint32_t nt = t ? n1 : n0;
+            if (ok && j < nt) {
+              const uint64_t v = slot ? vd[1] : vd[0];
 #pragma unroll
-                for (uint32_t e = 0; e < kKeys / 16; ++e)
-                  umma_f16_ts(tmem + kOutCol + t * 128, tmem + t * kKeys + e * 8, umma_desc_advance(vd, slot * slot_bytes + e * 2048u), idesc_o, (j | e) != 0 ? 1u : 0u);
-                if (j + 1 == p.n[t]) umma_commit(&o_full[t]);
+              for (uint32_t h = 0; h < 2; ++h) {  // the first half of the weights is there while the softmax is at the other one
+                if (!wait1(&p_ready[t][h], pc[t] & 1u)) break;
+                tc_fence_after_sync();
+#pragma unroll
+                for (uint32_t e = 4 * h; e < 4 * h + 4; ++e)
+                  umma_f16_ts(tmem + kOutCol + t * 128, tmem + t * kKeys + e * 8, umma_desc_advance(v, e * 2048u), idesc_o, (j | e) != 0 ? 1u : 0u);
+                if (h == 1 && j + 1 == nt) umma_commit(&o_full[t]);
               }
-              __syncwarp();
+              ++pc[t];
             }
-            if (ok && j + 1 < p.n[t]) {
+            if (ok && j + 1 < nt) {
               if (!have_k) {
-                if (!wait(&k_full[nslot], ((kt + 1) / 2) & 1u)) break;
+                if (!wait1(&k_full[nslot], ((kt + 1) / 2) & 1u)) break;
                 tc_fence_after_sync();
                 have_k = true;
               }
@@ -344,76 +416,104 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const PagedAttn a, c
             }
           }
           if (!ok) break;
-          if (j + 1 < p.n_all) commit(&k_empty[nslot]);
-          if (j + 2 == p.n_all) commit(&q_empty);
-          commit(&v_empty[slot]);
+          if (j + 1 < n) umma_commit(&k_empty[nslot]);
+          if (j + 2 == n) umma_commit(&q_empty);
+          umma_commit(&v_empty[slot]);
         }
         ++items;
       }
-      commit(&fin);  // nothing is left running when tensor memory is freed
+      umma_commit(&fin);  // nothing is left running when tensor memory is freed
       if (!mbar_wait(&fin, 0)) s_abort = 1;
-    } else if (warp == 2) {
-      // ===== queries of the next item; rows behind its tokens hold whatever follows there
-      uint32_t items = 0;
-      while (ok && runs.next(a, plan, w, p)) {
-        if (!p.n_all) continue;
-        if (items && !wait(&q_empty, (items - 1) & 1u)) break;
-        const uint32_t tiles = p.tokens > plan.tile_tokens ? 2u : 1u, t = lane / panels, panel = lane % panels;
-        if (lane == 0) mbar_expect_tx(&q_full, tiles * panels * plan.tile_tokens * runs.rep * 128);
-        __syncwarp();
-        if (t < tiles)
-          tma_3d(sq + t * q_tile + panel * kPanel, &maps.q, (int)panel * 64, (int)(p.s.g * runs.rep), (int)(p.s.rq.t0 + p.token + t * plan.tile_tokens), &q_full);
-        ++items;
-      }
-      if (items) (void)mbar_wait(&q_full, (items - 1) & 1u);  // no copy in flight at the end
     }
+    __syncwarp();
+  } else if (warp == 2) {
+    // ===== the run's pieces, and what is cut
+    if (lane == 0) {
+      Cut cut = {0, 0, 0, 0};
+      bool more = true;
+      for (uint32_t i = 0; more; ++i) {
+        Piece p;
+        p.tiles = 0;
+        more = runs.next(a, plan, walk, p);
+        if (more && p.cut_end && !p.cut_begin) cut = {(uint32_t)((p.item_u + p.tiles - 1) / per), p.s.rq.t0 + p.token, p.tokens, p.s.g};
+        if (i >= kPieces && (s_abort || !mbar_wait(&piece_empty[i % kPieces], (i / kPieces - 1) & 1u))) { s_abort = 1; break; }
+        s_piece[i % kPieces] = p;
+        mbar_arrive(&piece_full[i % kPieces]);
+      }
+      if (plan.cuts) plan.cuts[blockIdx.x] = cut;
+    }
+    __syncwarp();
+  }
   } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     // ===== softmax: thread = row
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
-    const uint32_t t = (warp - 4) >> 2, quarter = warp & 3u, rep = runs.rep, row = quarter * 32 + lane, mine = row / rep, head = row % rep;
+    const uint32_t t = (warp - kControlWarps) >> 2, quarter = warp & 3u, rep = runs.rep, row = quarter * 32 + lane, mine = row / rep;
     const uint32_t lanes = (quarter * 32u) << 16, s_at = tmem + lanes + t * kKeys, o_at = tmem + lanes + kOutCol + t * 128;
+    unsigned char* stage = smem + 2 * q_tile + 4 * slot_bytes + (warp - kControlWarps) * kStage;
     const float c = a.scale * kLog2e;
-    Walk w = walk0;
-    Piece p;
+    const unsigned long long c2 = pair_of(c, c);
     uint32_t sc = 0, oc = 0;
-    bool ok = true;
-    auto wait = [&](uint64_t* bar, uint32_t parity) {
-      if (ok) ok = __all_sync(0xFFFFFFFFu, !s_abort && mbar_wait(bar, parity));
-      if (!ok) s_abort = 1;
-      tc_fence_after_sync();
-      return ok;
-    };
-    if (tid == kThreads - 1 && plan.cuts) plan.cuts[blockIdx.x] = {0, 0, 0, 0};
-    while (runs.next(a, plan, w, p)) {
-      const uint32_t n = p.n[t], token = t * plan.tile_tokens + mine;  // of the item
+    size_t row_at[4];  // where the rows that this lane writes out begin, eight rows apart
+#pragma unroll
+    for (uint32_t x = 0; x < 4; ++x) {
+      const uint32_t at = quarter * 32 + 8 * x + (lane >> 2);
+      row_at[x] = (size_t)(at / rep) * a.out_ld + (size_t)(at % rep) * hd;
+    }
+    for (;; ++pieces) {
+      // the piece stays where it is until the rows are done: its numbers are read when they are needed
+      const uint32_t slot = pieces % kPieces;
+      if (!wait(&piece_full[slot], (pieces / kPieces) & 1u)) break;
+      const Piece& p = s_piece[slot];
+      if (p.tiles == 0) break;
+      const uint32_t n = t ? p.n[1] : p.n[0], token = t * plan.tile_tokens + mine;  // of the item
       const bool live = mine < plan.tile_tokens && token < p.tokens;
       const uint32_t pos = p.s.rq.cached + p.token + min(token, p.tokens - 1), low = paged_low(pos, a.window);
       float m = -INFINITY, l = 0.0f;
       for (uint32_t j = 0; j < n; ++j, ++sc) {
         if (!wait(&s_full[t], sc & 1u)) break;
-        float s[kKeys];
-#pragma unroll
-        for (int i = 0; i < kKeys; i += 32) tmem_ld32(s_at + i, s + i);
+        tc_fence_after_sync();
         const uint32_t key0 = (p.s.tile0 + j) * kKeys;
-        if (!__all_sync(0xFFFFFFFFu, key0 >= low && key0 + kKeys <= pos + 1)) {
-          const int hi = (int)min(pos + 1 > key0 ? pos + 1 - key0 : 0u, (uint32_t)kKeys), lo = low > key0 ? (int)min(low - key0, (uint32_t)kKeys) : 0;
+        const uint32_t hi = pos + 1 > key0 ? pos + 1 - key0 : 0u, lo = low > key0 ? low - key0 : 0u;  // keys key0 + lo .. key0 + hi - 1 are seen
+        // which of the 32 keys from i on: all of them for nearly every tile
+        auto seen = [&](uint32_t i) {
+          const uint32_t up = hi <= i ? 0u : hi - i >= 32 ? 0xFFFFFFFFu : (1u << (hi - i)) - 1u;
+          return lo <= i ? up : lo - i >= 32 ? 0u : up & ~((1u << (lo - i)) - 1u);
+        };
+        float s[kKeys];
+        {
+          uint32_t r[4][32];
 #pragma unroll
-          for (int i = 0; i < kKeys; ++i) s[i] = i < hi && i >= lo ? s[i] : -INFINITY;
-        }
-        float x[4] = {s[0], s[1], s[2], s[3]};
+          for (int x = 0; x < 4; ++x) tmem_ld32_start(s_at + 32 * x, r[x]);
 #pragma unroll
-        for (int i = 4; i < kKeys; i += 4) {
-          x[0] = fmaxf(x[0], s[i]); x[1] = fmaxf(x[1], s[i + 1]); x[2] = fmaxf(x[2], s[i + 2]); x[3] = fmaxf(x[3], s[i + 3]);
+          for (int x = 0; x < 4; ++x) tmem_ld32_end(r[x]);
+#pragma unroll
+          for (int y = 0; y < kKeys; ++y) s[y] = __uint_as_float(r[y / 32][y % 32]);
         }
-        const float mx = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) * c;  // c > 0
+        if (!__all_sync(0xFFFFFFFFu, lo == 0 && hi >= (uint32_t)kKeys)) {
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const uint32_t bits = seen(32 * x);
+#pragma unroll
+            for (int y = 0; y < 32; ++y) s[32 * x + y] = (bits >> y) & 1u ? s[32 * x + y] : -INFINITY;
+          }
+        }
+        float top[4];
+#pragma unroll
+        for (int y = 0; y < 4; ++y) top[y] = fmaxf(s[y], s[y + 4]);
+#pragma unroll
+        for (int y = 8; y < kKeys; y += 8) {
+#pragma unroll
+          for (int z = 0; z < 4; ++z) top[z] = fmaxf(fmaxf(top[z], s[y + z]), s[y + z + 4]);
+        }
+        float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+        mx *= c;  // c > 0
         if (__any_sync(0xFFFFFFFFu, mx > m + kGrowth)) {
           const float m_new = fmaxf(m, mx), f = m == -INFINITY ? 0.0f : exp2_of(m - m_new);
           m = m_new;
           l *= f;
           if (j > 0) {  // the products before have finished: this tile's scores came after them
-#pragma unroll
-            for (int i = 0; i < 128; i += 32) {
-              if (i >= (int)hd) break;
+#pragma unroll 1
+            for (uint32_t i = 0; i < hd; i += 32) {
               float o[32];
               tmem_ld32(o_at + i, o);
 #pragma unroll
@@ -422,81 +522,99 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const PagedAttn a, c
             }
           }
         }
-        const float base = m == -INFINITY ? 0.0f : m;
-        float add[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        const float base = m == -INFINITY ? 0.0f : -m;
+        const unsigned long long base2 = pair_of(base, base);
+        unsigned long long add0 = 0, add1 = 0;
 #pragma unroll
         for (int i = 0; i < kKeys; i += 32) {
           uint32_t pk[16];
 #pragma unroll
           for (int y = 0; y < 32; y += 2) {
-            const float e0 = exp2_of(fmaf(s[i + y], c, -base)), e1 = exp2_of(fmaf(s[i + y + 1], c, -base));
-            add[y & 2] += e0;
-            add[(y & 2) + 1] += e1;
+            const unsigned long long v = fma2(pair_of(s[i + y], s[i + y + 1]), c2, base2);
+            const float e0 = exp2_of(__uint_as_float((uint32_t)v)), e1 = exp2_of(__uint_as_float((uint32_t)(v >> 32)));
+            if (y & 2) add1 = add2(add1, pair_of(e0, e1));
+            else add0 = add2(add0, pair_of(e0, e1));
             pk[y / 2] = pack2<T>(e0, e1);
           }
           tmem_st16(s_at + i / 2, pk);
+          if (i & 32) {  // half of the weights
+            tmem_st_wait();
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_ready[t][i >> 6]);
+          }
         }
-        l += (add[0] + add[1]) + (add[2] + add[3]);
-        tmem_st_wait();
-        tc_fence_before_sync();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&p_ready[t]);
+        add0 = add2(add0, add1);
+        l += __uint_as_float((uint32_t)add0) + __uint_as_float((uint32_t)(add0 >> 32));
       }
-      if (n && ok) { wait(&o_full[t], oc & 1u); ++oc; }
+      if (n) { wait(&o_full[t], oc & 1u); ++oc; tc_fence_after_sync(); }
+      if (!ok) break;
       // ---- the rows' results: out, or a part of an item
       const bool cut = p.cut_begin || p.cut_end;
       float* part = plan.parts + ((size_t)blockIdx.x * 2 + (p.cut_begin ? 0 : 1)) * plan.part_floats;
-      if (tid == kThreads - 1 && p.cut_end && !p.cut_begin)
-        plan.cuts[blockIdx.x] = {(uint32_t)((p.item_u + p.tiles - 1) / per), p.s.rq.t0 + p.token, p.tokens, p.s.g};
-      T* dst = static_cast<T*>(a.out) + (size_t)(p.s.rq.t0 + p.token + (live ? token : 0u)) * a.out_ld + (size_t)(p.s.g * rep + head) * hd;
-      if (ok) {
-        bool fine = isfinite(l);
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        const uint32_t cols = (hd + 31) / 32;
-        for (uint32_t i = 0; i < cols; ++i) {
-          float o[32];
-          if (n) tmem_ld32(o_at + i * 32, o);
-          else {
+      T* out = static_cast<T*>(a.out) + (size_t)(p.s.rq.t0 + p.token + t * plan.tile_tokens) * a.out_ld + (size_t)(p.s.g * rep) * hd;
+      const uint32_t row_end = (p.tokens > t * plan.tile_tokens ? min(p.tokens - t * plan.tile_tokens, plan.tile_tokens) : 0u) * rep;  // of the tile
+      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+      unsigned long long odd[2] = {pair_of(l * 0.0f, 0.0f), 0};  // NaN where anything is not finite
+#pragma unroll 1
+      for (uint32_t i = 0; i < hd; i += 32) {
+        float o[32];
+        if (n) tmem_ld32(o_at + i, o);
+        else {
 #pragma unroll
-            for (int y = 0; y < 32; ++y) o[y] = 0.0f;
-          }
-#pragma unroll
-          for (int y = 0; y < 32; y += 8) {
-            if (i * 32 + y >= hd) break;
-#pragma unroll
-            for (int z = 0; z < 8; ++z) fine = fine && isfinite(o[y + z]);
-            if (live && !cut) {
-              const uint4 v = make_uint4(pack2<T>(o[y] * inv, o[y + 1] * inv), pack2<T>(o[y + 2] * inv, o[y + 3] * inv), pack2<T>(o[y + 4] * inv, o[y + 5] * inv),
-                                         pack2<T>(o[y + 6] * inv, o[y + 7] * inv));
-              *reinterpret_cast<uint4*>(dst + i * 32 + y) = v;
-            }
-            if (live && cut) {
-              float4* q = reinterpret_cast<float4*>(part + ((size_t)(i * 8 + y / 4) * kItemRows + t * kRows + row) * 4);
-              q[0] = make_float4(o[y], o[y + 1], o[y + 2], o[y + 3]);
-              q[kItemRows] = make_float4(o[y + 4], o[y + 5], o[y + 6], o[y + 7]);
-            }
-          }
+          for (int y = 0; y < 32; ++y) o[y] = 0.0f;
         }
-        // rows that are not finite, key by key
-        for (uint32_t bad = __ballot_sync(0xFFFFFFFFu, live && !fine); bad; bad &= bad - 1) {
-          const uint32_t who = (uint32_t)__ffs((int)bad) - 1, which = quarter * 32 + who, x = p.s.row0 + t * plan.tile_tokens * rep + which;
-          float* tmp = s_again[warp - 4];
-          float m2, l2;
-          row_again<T>(a, p.s, rep, x, p.s.tile0 * kKeys, p.s.tile1 * kKeys, tmp, m2, l2);
+        if (i + 32 > hd) {  // columns that no product wrote
+#pragma unroll
+          for (int y = 0; y < 32; y += 8)
+            if (i + y >= hd) {
+#pragma unroll
+              for (int z = 0; z < 8; ++z) o[y + z] = 0.0f;
+            }
+        }
+#pragma unroll
+        for (int y = 0; y < 32; y += 2) odd[(y / 2) & 1] = fma2(pair_of(o[y], o[y + 1]), 0ull, odd[(y / 2) & 1]);
+        if (cut) {
+#pragma unroll
+          for (int y = 0; y < 32; y += 4)
+            if (live && i + y < hd) *reinterpret_cast<float4*>(part + ((size_t)((i + y) / 4) * kItemRows + t * kRows + row) * 4) = make_float4(o[y], o[y + 1], o[y + 2], o[y + 3]);
+        } else {
+#pragma unroll
+          for (int y = 0; y < 32; y += 8)
+            *reinterpret_cast<uint4*>(stage + lane * 64 + (((y / 8) ^ (lane >> 1)) & 3) * 16) =
+                make_uint4(pack2<T>(o[y] * inv, o[y + 1] * inv), pack2<T>(o[y + 2] * inv, o[y + 3] * inv), pack2<T>(o[y + 4] * inv, o[y + 5] * inv), pack2<T>(o[y + 6] * inv, o[y + 7] * inv));
           __syncwarp();
-          T* d2 = static_cast<T*>(a.out) + (size_t)(p.s.rq.t0 + x / rep) * a.out_ld + (size_t)(p.s.g * rep + x % rep) * hd;
-          for (uint32_t e = lane; e < hd; e += 32) {
-            if (cut) part[((size_t)(e / 4) * kItemRows + t * kRows + which) * 4 + (e & 3u)] = tmp[e];
-            else d2[e] = from_f32<T>(l2 == 0.0f ? 0.0f : tmp[e] / l2);
+#pragma unroll
+          for (uint32_t x = 0; x < 4; ++x) {  // eight rows of 64 bytes at a time
+            const uint32_t rr = 8 * x + (lane >> 2), at = quarter * 32 + rr, col = i + (lane & 3u) * 8;
+            const uint4 v = *reinterpret_cast<const uint4*>(stage + rr * 64 + (((lane & 3u) ^ (rr >> 1)) & 3u) * 16);
+            if (at < row_end && col < hd) *reinterpret_cast<uint4*>(out + row_at[x] + col) = v;
           }
           __syncwarp();
-          if (lane == who) { m = m2; l = l2; }
-        }
-        if (cut && live) {
-          part[hd * kItemRows + t * kRows + row] = m;
-          part[(hd + 1) * kItemRows + t * kRows + row] = l;
         }
       }
+      // rows that are not finite, key by key
+      odd[0] = add2(odd[0], odd[1]);
+      const bool fine = __uint_as_float((uint32_t)odd[0]) + __uint_as_float((uint32_t)(odd[0] >> 32)) == 0.0f;
+      for (uint32_t bad = __ballot_sync(0xFFFFFFFFu, live && !fine); bad; bad &= bad - 1) {
+        const uint32_t who = (uint32_t)__ffs((int)bad) - 1, which = quarter * 32 + who;
+        float* tmp = s_again[warp - kControlWarps];
+        float m2, l2;
+        row_again<T>(a, p.s, rep, p.s.row0 + t * plan.tile_tokens * rep + which, p.s.tile0 * kKeys, p.s.tile1 * kKeys, tmp, m2, l2);
+        __syncwarp();
+        for (uint32_t e = lane; e < hd; e += 32) {
+          if (cut) part[((size_t)(e / 4) * kItemRows + t * kRows + which) * 4 + (e & 3u)] = tmp[e];
+          else out[(size_t)(which / rep) * a.out_ld + (size_t)(which % rep) * hd + e] = from_f32<T>(l2 == 0.0f ? 0.0f : tmp[e] / l2);
+        }
+        __syncwarp();
+        if (lane == who) { m = m2; l = l2; }
+      }
+      if (cut && live) {
+        part[hd * kItemRows + t * kRows + row] = m;
+        part[(hd + 1) * kItemRows + t * kRows + row] = l;
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&piece_empty[slot]);
     }
   }
   tc_fence_before_sync();
@@ -568,7 +686,7 @@ CUresult encode(EncodeFn fn, CUtensorMap* map, const PagedPool& p, void* base, u
 template <typename T>
 cudaError_t launch_chunk(ruai_ctx* c, const PagedAttn& a, const TcPlan& plan, const Maps& maps) {
   const uint32_t panels = (a.pool.hd + 63) / 64;
-  const int smem = 6 * (int)panels * kPanel + 1024, most = 12 * kPanel + 1024;
+  const int extra = kSoftWarps * kStage + 1024, smem = 6 * (int)panels * kPanel + extra, most = 12 * kPanel + extra;
   static bool done[64] = {};
   if (!done[c->ordinal & 63]) {
     cudaError_t e = cudaFuncSetAttribute(chunk_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
