@@ -32,7 +32,7 @@ constexpr float kGrowth = 8.0f;
 constexpr int kItemCost = 2;    // units of a run that an item takes beside its tiles: its queries' and outputs' way, 5500 clocks where a tile takes 3100
 constexpr int kTilesLeast = 6;  // units of a run: a part costs as much as a few tiles
 
-struct alignas(64) Maps { CUtensorMap q, k, v; };
+struct alignas(64) Maps { CUtensorMap q, k, v, o; };
 
 // A cut item, left by the CTA in which it begins for the CTAs that join it.
 struct Cut { uint32_t last, token, tokens, g; };  // the CTA in which it ends (0: nothing was cut), its tokens' rows of the step, the key head
@@ -41,12 +41,16 @@ struct TcPlan {
   Cut* cuts;     // [CTAs], or NULL: items stay whole
   uint32_t rows_over, box_rows, part_floats;
   uint32_t tile_tokens;  // tokens of a row tile
+  uint32_t boxed;        // 32 rows of a tile are a box of the output's map
 };
 
 __device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
   asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst), "l"((uint64_t)map), "r"(x), "r"(y),
                "r"(z), "r"(smem_u32(bar))
                : "memory");
+}
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, uint32_t src, int x, int y, int z) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"((uint64_t)map), "r"(x), "r"(y), "r"(z), "r"(src) : "memory");
 }
 __device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
   asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst), "l"((uint64_t)map), "r"(x), "r"(y),
@@ -115,6 +119,11 @@ __device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigne
 __device__ __forceinline__ unsigned long long add2(unsigned long long a, unsigned long long b) {
   unsigned long long r;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
 template <typename T> __device__ __forceinline__ uint32_t pack2(float a, float b);
@@ -197,7 +206,7 @@ struct Runs {
 
 constexpr int kPieces = 3;  // pieces that the scheduling warp is ahead
 constexpr int kSoftWarps = 8, kControlWarps = 4;
-constexpr int kStage = 32 * 64;  // bytes in which a softmax warp turns 32 rows of 32 columns around for the output
+constexpr int kStage = 32 * 128;  // bytes in which a softmax warp leaves 32 rows of 64 columns for their copy to the output
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const PagedAttn a, const TcPlan plan, const __grid_constant__ Maps maps) {
@@ -207,7 +216,6 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const PagedAttn a, c
   __shared__ uint32_t s_tmem, s_r;
   __shared__ volatile int s_abort;
   __shared__ unsigned long long s_part[kThreads / 32], s_base;
-  __shared__ float s_again[kSoftWarps][128];
   const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, hd = a.pool.hd, panels = (hd + 63) / 64, plog = a.pool.page_log2;
   unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   const uint32_t q_tile = panels * kPanel, slot_bytes = panels * kPanel;
@@ -225,6 +233,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const PagedAttn a, c
   }
   __syncwarp();
   if (warp == 1) tmem_alloc(&s_tmem, 512);
+  if (warp == 0 && lane < 4) asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)(&maps.q + lane)) : "memory");
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
@@ -292,173 +301,169 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const PagedAttn a, c
     return p.tiles != 0;
   };
 
+  // registers: the launch's 384 x 168 hold 128 x 72 and 256 x 216
   if (warp < (uint32_t)kControlWarps) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 80;");
-  if (warp == 0) {
-    // ===== an item's queries, then its keys and values, a lane per box; rows behind the item's tokens hold whatever follows there
-    const uint32_t boxes = kKeys / plan.box_rows, box = lane % boxes, panel = lane / boxes;
-    const uint32_t dst = panel * kPanel + box * plan.box_rows * 128;
-    uint32_t kt = 0, vt = 0, items = 0, lasts = 0;  // asked for
-    Piece p;
-    while (ok && next(p)) {
-      if (!p.n_all) continue;
-      if (items && !wait(&q_empty, (items - 1) & 1u)) break;
-      {
-        const uint32_t tiles = p.tokens > plan.tile_tokens ? 2u : 1u, t = lane / panels, pn = lane % panels;
-        if (lane == 0) mbar_expect_tx(&q_full, tiles * panels * plan.tile_tokens * runs.rep * 128);
-        __syncwarp();
-        if (t < tiles) tma_3d(sq + t * q_tile + pn * kPanel, &maps.q, (int)pn * 64, (int)(p.s.g * runs.rep), (int)(p.s.rq.t0 + p.token + t * plan.tile_tokens), &q_full);
-        ++items;
-      }
-      for (uint32_t j = 0; j < p.n_all; ++j) {
-        const uint32_t key = (p.s.tile0 + j) * kKeys + box * plan.box_rows, slot = kt & 1u;
-        int32_t pg = -1;
-        if (key < p.s.rq.len) pg = paged_page(a, p.s.r, key);
-        const uint32_t bytes = __popc(__ballot_sync(0xFFFFFFFFu, lane < boxes && pg >= 0)) * panels * plan.box_rows * 128;
-        const int y = pg >= 0 ? (int)((((uint32_t)pg * a.pool.KV + p.s.g) << plog) + (key & ((1u << plog) - 1u))) : 0;
-        const bool mine = panel < panels && pg >= 0;
-        if (kt >= 2 && !wait(&k_empty[slot], (kt / 2 - 1) & 1u)) break;
-        if (lane == 0) mbar_expect_tx(&k_full[slot], bytes);
-        __syncwarp();
-        if (mine) tma_2d(sk + slot * slot_bytes + dst, &maps.k, (int)panel * 64, y, &k_full[slot]);
-        ++kt;
-        if (vt >= 2 && !wait(&v_empty[slot], (vt / 2 - 1) & 1u)) break;
-        if (lane == 0) mbar_expect_tx(&v_full[slot], bytes);
-        __syncwarp();
-        if (mine) tma_2d(sv + slot * slot_bytes + dst, &maps.v, (int)panel * 64, y, &v_full[slot]);
-        ++vt;
-      }
-      const uint32_t end = (p.s.tile0 + p.n_all) * kKeys;
-      if (ok && end > p.s.rq.len) {  // positions behind the request's end: their values weigh nothing, and must be numbers for that
-        if (!wait(&v_last, lasts++ & 1u)) break;  // they have come
-        for (uint32_t r = p.s.rq.len - (end - kKeys) + (lane >> 3); r < (uint32_t)kKeys; r += 4)
-          for (uint32_t pn = 0; pn < panels; ++pn)
-            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(sv + ((vt - 1) & 1u) * slot_bytes + pn * kPanel + r * 128 + (lane & 7u) * 16), "r"(0) : "memory");
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&v_cleared);
-      }
-    }
-    if (items) (void)mbar_wait(&q_full, (items - 1) & 1u);
-    // leave no copy in flight into shared memory that another CTA may get, whoever gives up
-    for (uint32_t i = kt > 2 ? kt - 2 : 0; i < kt; ++i) (void)mbar_wait(&k_full[i & 1u], (i / 2) & 1u);
-    for (uint32_t i = vt > 2 ? vt - 2 : 0; i < vt; ++i) (void)mbar_wait(&v_full[i & 1u], (i / 2) & 1u);
-  } else if (warp == 1) {
-    // ===== MMAs
-    constexpr uint32_t kType = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
-    const uint32_t idesc_s = (1u << 4) | (kType << 7) | (kType << 10) | ((kKeys >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
-    const uint32_t vcols = (hd + 15) / 16 * 16;
-    const uint32_t idesc_o = (1u << 4) | (kType << 7) | (kType << 10) | (1u << 16) | ((vcols >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
-    // One thread for all of it: a warp that votes and elects between the products takes 100 clocks an MMA, the tensor core 64.
-    if (elect_one()) {
-      const uint64_t qd[2] = {umma_desc_sw128(sq), umma_desc_sw128(sq + q_tile)}, kd[2] = {umma_desc_sw128(sk), umma_desc_sw128(sk + slot_bytes)},
-                     vd[2] = {umma_desc_mn128(sv), umma_desc_mn128(sv + slot_bytes)};
-      const uint32_t steps = (hd + 15) / 16;
-      uint32_t kt = 0, items = 0, pc[2] = {0, 0}, cleared = 0;
-      auto wait1 = [&](uint64_t* bar, uint32_t parity) {
-        if (ok && !mbar_wait(bar, parity)) { s_abort = 1; ok = false; }
-        return ok;
-      };
-      auto scores = [&](uint32_t t, uint32_t slot) {
-        const uint64_t q = qd[t], k = slot ? kd[1] : kd[0];
-#pragma unroll
-        for (uint32_t e = 0; e < 8; ++e) {
-          if (e >= steps) break;
-          umma_f16_ss(tmem + t * kKeys, umma_desc_advance(q, (e >> 2) * kPanel + (e & 3u) * 32u), umma_desc_advance(k, (e >> 2) * kPanel + (e & 3u) * 32u), idesc_s, e != 0 ? 1u : 0u);
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    if (warp == 0) {
+      // ===== an item's queries, then its keys and values, a lane per box; rows behind the item's tokens hold whatever follows there
+      const uint32_t boxes = kKeys / plan.box_rows, box = lane % boxes, panel = lane / boxes;
+      const uint32_t dst = panel * kPanel + box * plan.box_rows * 128;
+      uint32_t kt = 0, vt = 0, items = 0, lasts = 0;  // asked for
+      Piece p;
+      while (ok && next(p)) {
+        if (!p.n_all) continue;
+        if (items && !wait(&q_empty, (items - 1) & 1u)) break;
+        {
+          const uint32_t tiles = p.tokens > plan.tile_tokens ? 2u : 1u, t = lane / panels, pn = lane % panels;
+          if (lane == 0) mbar_expect_tx(&q_full, tiles * panels * plan.tile_tokens * runs.rep * 128);
+          __syncwarp();
+          if (t < tiles) tma_3d(sq + t * q_tile + pn * kPanel, &maps.q, (int)pn * 64, (int)(p.s.g * runs.rep), (int)(p.s.rq.t0 + p.token + t * plan.tile_tokens), &q_full);
+          ++items;
         }
-        umma_commit(&s_full[t]);
-      };
-      for (; ok; ++pieces) {
-        const uint32_t ps = pieces % kPieces;
-        if (!wait1(&piece_full[ps], (pieces / kPieces) & 1u)) break;
-        const uint32_t n0 = s_piece[ps].n[0], n1 = s_piece[ps].n[1], n = max(n0, n1), stop = s_piece[ps].tiles == 0;
-        const bool tail = (s_piece[ps].s.tile0 + n) * kKeys > s_piece[ps].s.rq.len;
-        mbar_arrive(&piece_empty[ps]);
-        if (stop) break;
-        if (!n) continue;
-        if (!wait1(&q_full, items & 1u) || !wait1(&k_full[kt & 1u], (kt / 2) & 1u)) break;
-        tc_fence_after_sync();
-        if (n0) scores(0, kt & 1u);
-        if (n1) scores(1, kt & 1u);
-        umma_commit(&k_empty[kt & 1u]);
-        if (n == 1) umma_commit(&q_empty);
-        for (uint32_t j = 0; j < n; ++j, ++kt) {
-          const uint32_t slot = kt & 1u, nslot = slot ^ 1u;
-          if (!wait1(&v_full[slot], (kt / 2) & 1u)) break;
-          if (tail && j + 1 == n) {
-            mbar_arrive(&v_last);
-            if (!wait1(&v_cleared, cleared++ & 1u)) break;
-          }
-          bool have_k = false;
-#pragma unroll
-          for (uint32_t t = 0; t < 2; ++t) {
-            const uint32_t nt = t ? n1 : n0;
-            if (ok && j < nt) {
-              const uint64_t v = slot ? vd[1] : vd[0];
-#pragma unroll
-              for (uint32_t h = 0; h < 2; ++h) {  // the first half of the weights is there while the softmax is at the other one
-                if (!wait1(&p_ready[t][h], pc[t] & 1u)) break;
-                tc_fence_after_sync();
-#pragma unroll
-                for (uint32_t e = 4 * h; e < 4 * h + 4; ++e)
-                  umma_f16_ts(tmem + kOutCol + t * 128, tmem + t * kKeys + e * 8, umma_desc_advance(v, e * 2048u), idesc_o, (j | e) != 0 ? 1u : 0u);
-                if (h == 1 && j + 1 == nt) umma_commit(&o_full[t]);
-              }
-              ++pc[t];
-            }
-            if (ok && j + 1 < nt) {
-              if (!have_k) {
-                if (!wait1(&k_full[nslot], ((kt + 1) / 2) & 1u)) break;
-                tc_fence_after_sync();
-                have_k = true;
-              }
-              scores(t, nslot);
-            }
-          }
-          if (!ok) break;
-          if (j + 1 < n) umma_commit(&k_empty[nslot]);
-          if (j + 2 == n) umma_commit(&q_empty);
-          umma_commit(&v_empty[slot]);
+        for (uint32_t j = 0; j < p.n_all; ++j) {
+          const uint32_t key = (p.s.tile0 + j) * kKeys + box * plan.box_rows, slot = kt & 1u;
+          int32_t pg = -1;
+          if (key < p.s.rq.len) pg = paged_page(a, p.s.r, key);
+          const uint32_t bytes = __popc(__ballot_sync(0xFFFFFFFFu, lane < boxes && pg >= 0)) * panels * plan.box_rows * 128;
+          const int y = pg >= 0 ? (int)((((uint32_t)pg * a.pool.KV + p.s.g) << plog) + (key & ((1u << plog) - 1u))) : 0;
+          const bool mine = panel < panels && pg >= 0;
+          if (kt >= 2 && !wait(&k_empty[slot], (kt / 2 - 1) & 1u)) break;
+          if (lane == 0) mbar_expect_tx(&k_full[slot], bytes);
+          __syncwarp();
+          if (mine) tma_2d(sk + slot * slot_bytes + dst, &maps.k, (int)panel * 64, y, &k_full[slot]);
+          ++kt;
+          if (vt >= 2 && !wait(&v_empty[slot], (vt / 2 - 1) & 1u)) break;
+          if (lane == 0) mbar_expect_tx(&v_full[slot], bytes);
+          __syncwarp();
+          if (mine) tma_2d(sv + slot * slot_bytes + dst, &maps.v, (int)panel * 64, y, &v_full[slot]);
+          ++vt;
         }
-        ++items;
+        const uint32_t end = (p.s.tile0 + p.n_all) * kKeys;
+        if (ok && end > p.s.rq.len) {  // positions behind the request's end: their values weigh nothing, and must be numbers for that
+          if (!wait(&v_last, lasts++ & 1u)) break;  // they have come
+          for (uint32_t r = p.s.rq.len - (end - kKeys) + (lane >> 3); r < (uint32_t)kKeys; r += 4)
+            for (uint32_t pn = 0; pn < panels; ++pn)
+              asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(sv + ((vt - 1) & 1u) * slot_bytes + pn * kPanel + r * 128 + (lane & 7u) * 16), "r"(0) : "memory");
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&v_cleared);
+        }
       }
-      umma_commit(&fin);  // nothing is left running when tensor memory is freed
-      if (!mbar_wait(&fin, 0)) s_abort = 1;
-    }
-    __syncwarp();
-  } else if (warp == 2) {
-    // ===== the run's pieces, and what is cut
-    if (lane == 0) {
-      Cut cut = {0, 0, 0, 0};
-      bool more = true;
-      for (uint32_t i = 0; more; ++i) {
-        Piece p;
-        p.tiles = 0;
-        more = runs.next(a, plan, walk, p);
-        if (more && p.cut_end && !p.cut_begin) cut = {(uint32_t)((p.item_u + p.tiles - 1) / per), p.s.rq.t0 + p.token, p.tokens, p.s.g};
-        if (i >= kPieces && (s_abort || !mbar_wait(&piece_empty[i % kPieces], (i / kPieces - 1) & 1u))) { s_abort = 1; break; }
-        s_piece[i % kPieces] = p;
-        mbar_arrive(&piece_full[i % kPieces]);
+      if (items) (void)mbar_wait(&q_full, (items - 1) & 1u);
+      // leave no copy in flight into shared memory that another CTA may get, whoever gives up
+      for (uint32_t i = kt > 2 ? kt - 2 : 0; i < kt; ++i) (void)mbar_wait(&k_full[i & 1u], (i / 2) & 1u);
+      for (uint32_t i = vt > 2 ? vt - 2 : 0; i < vt; ++i) (void)mbar_wait(&v_full[i & 1u], (i / 2) & 1u);
+    } else if (warp == 1) {
+      // ===== MMAs
+      constexpr uint32_t kType = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+      const uint32_t idesc_s = (1u << 4) | (kType << 7) | (kType << 10) | ((kKeys >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
+      const uint32_t vcols = (hd + 15) / 16 * 16;
+      const uint32_t idesc_o = (1u << 4) | (kType << 7) | (kType << 10) | (1u << 16) | ((vcols >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
+      // One thread for all of it: a warp that votes and elects between the products takes 100 clocks an MMA, the tensor core 64.
+      if (elect_one()) {
+        const uint64_t qd[2] = {umma_desc_sw128(sq), umma_desc_sw128(sq + q_tile)}, kd[2] = {umma_desc_sw128(sk), umma_desc_sw128(sk + slot_bytes)},
+                       vd[2] = {umma_desc_mn128(sv), umma_desc_mn128(sv + slot_bytes)};
+        const uint32_t steps = (hd + 15) / 16;
+        uint32_t kt = 0, items = 0, pc[2] = {0, 0}, cleared = 0;
+        auto wait1 = [&](uint64_t* bar, uint32_t parity) {
+          if (ok && !mbar_wait(bar, parity)) { s_abort = 1; ok = false; }
+          return ok;
+        };
+        auto scores = [&](uint32_t t, uint32_t slot) {
+          const uint64_t q = qd[t], k = slot ? kd[1] : kd[0];
+#pragma unroll
+          for (uint32_t e = 0; e < 8; ++e) {
+            if (e >= steps) break;
+            umma_f16_ss(tmem + t * kKeys, umma_desc_advance(q, (e >> 2) * kPanel + (e & 3u) * 32u), umma_desc_advance(k, (e >> 2) * kPanel + (e & 3u) * 32u), idesc_s, e != 0 ? 1u : 0u);
+          }
+          umma_commit(&s_full[t]);
+        };
+        for (; ok; ++pieces) {
+          const uint32_t ps = pieces % kPieces;
+          if (!wait1(&piece_full[ps], (pieces / kPieces) & 1u)) break;
+          const uint32_t n0 = s_piece[ps].n[0], n1 = s_piece[ps].n[1], n = max(n0, n1), stop = s_piece[ps].tiles == 0;
+          const bool tail = (s_piece[ps].s.tile0 + n) * kKeys > s_piece[ps].s.rq.len;
+          mbar_arrive(&piece_empty[ps]);
+          if (stop) break;
+          if (!n) continue;
+          if (!wait1(&q_full, items & 1u) || !wait1(&k_full[kt & 1u], (kt / 2) & 1u)) break;
+          tc_fence_after_sync();
+          if (n0) scores(0, kt & 1u);
+          if (n1) scores(1, kt & 1u);
+          umma_commit(&k_empty[kt & 1u]);
+          if (n == 1) umma_commit(&q_empty);
+          for (uint32_t j = 0; j < n; ++j, ++kt) {
+            const uint32_t slot = kt & 1u, nslot = slot ^ 1u;
+            if (!wait1(&v_full[slot], (kt / 2) & 1u)) break;
+            if (tail && j + 1 == n) {
+              mbar_arrive(&v_last);
+              if (!wait1(&v_cleared, cleared++ & 1u)) break;
+            }
+            bool have_k = false;
+#pragma unroll
+            for (uint32_t t = 0; t < 2; ++t) {
+              const uint32_t nt = t ? n1 : n0;
+              if (ok && j < nt) {
+                const uint64_t v = slot ? vd[1] : vd[0];
+#pragma unroll
+                for (uint32_t h = 0; h < 2; ++h) {  // the first half of the weights is there while the softmax is at the other one
+                  if (!wait1(&p_ready[t][h], pc[t] & 1u)) break;
+                  tc_fence_after_sync();
+#pragma unroll
+                  for (uint32_t e = 4 * h; e < 4 * h + 4; ++e)
+                    umma_f16_ts(tmem + kOutCol + t * 128, tmem + t * kKeys + e * 8, umma_desc_advance(v, e * 2048u), idesc_o, (j | e) != 0 ? 1u : 0u);
+                  if (h == 1 && j + 1 == nt) umma_commit(&o_full[t]);
+                }
+                ++pc[t];
+              }
+              if (ok && j + 1 < nt) {
+                if (!have_k) {
+                  if (!wait1(&k_full[nslot], ((kt + 1) / 2) & 1u)) break;
+                  tc_fence_after_sync();
+                  have_k = true;
+                }
+                scores(t, nslot);
+              }
+            }
+            if (!ok) break;
+            if (j + 1 < n) umma_commit(&k_empty[nslot]);
+            if (j + 2 == n) umma_commit(&q_empty);
+            umma_commit(&v_empty[slot]);
+          }
+          ++items;
+        }
+        umma_commit(&fin);  // nothing is left running when tensor memory is freed
+        if (!mbar_wait(&fin, 0)) s_abort = 1;
       }
-      if (plan.cuts) plan.cuts[blockIdx.x] = cut;
+      __syncwarp();
+    } else if (warp == 2) {
+      // ===== the run's pieces, and what is cut
+      if (lane == 0) {
+        Cut cut = {0, 0, 0, 0};
+        bool more = true;
+        for (uint32_t i = 0; more; ++i) {
+          Piece p;
+          p.tiles = 0;
+          more = runs.next(a, plan, walk, p);
+          if (more && p.cut_end && !p.cut_begin) cut = {(uint32_t)((p.item_u + p.tiles - 1) / per), p.s.rq.t0 + p.token, p.tokens, p.s.g};
+          if (i >= kPieces && (s_abort || !mbar_wait(&piece_empty[i % kPieces], (i / kPieces - 1) & 1u))) { s_abort = 1; break; }
+          s_piece[i % kPieces] = p;
+          mbar_arrive(&piece_full[i % kPieces]);
+        }
+        if (plan.cuts) plan.cuts[blockIdx.x] = cut;
+      }
+      __syncwarp();
     }
-    __syncwarp();
-  }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
     // ===== softmax: thread = row
     const uint32_t t = (warp - kControlWarps) >> 2, quarter = warp & 3u, rep = runs.rep, row = quarter * 32 + lane, mine = row / rep;
     const uint32_t lanes = (quarter * 32u) << 16, s_at = tmem + lanes + t * kKeys, o_at = tmem + lanes + kOutCol + t * 128;
     unsigned char* stage = smem + 2 * q_tile + 4 * slot_bytes + (warp - kControlWarps) * kStage;
+    const uint32_t box_head = quarter * 32 % rep, box_token = t * plan.tile_tokens + quarter * 32 / rep;
     const float c = a.scale * kLog2e;
     const unsigned long long c2 = pair_of(c, c);
     uint32_t sc = 0, oc = 0;
-    size_t row_at[4];  // where the rows that this lane writes out begin, eight rows apart
-#pragma unroll
-    for (uint32_t x = 0; x < 4; ++x) {
-      const uint32_t at = quarter * 32 + 8 * x + (lane >> 2);
-      row_at[x] = (size_t)(at / rep) * a.out_ld + (size_t)(at % rep) * hd;
-    }
     for (;; ++pieces) {
       // the piece stays where it is until the rows are done: its numbers are read when they are needed
       const uint32_t slot = pieces % kPieces;
@@ -493,8 +498,10 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const PagedAttn a, c
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
             const uint32_t bits = seen(32 * x);
+            if (!__all_sync(0xFFFFFFFFu, bits == 0xFFFFFFFFu)) {
 #pragma unroll
-            for (int y = 0; y < 32; ++y) s[32 * x + y] = (bits >> y) & 1u ? s[32 * x + y] : -INFINITY;
+              for (int y = 0; y < 32; ++y) s[32 * x + y] = (bits >> y) & 1u ? s[32 * x + y] : -INFINITY;
+            }
           }
         }
         float top[4];
@@ -503,7 +510,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const PagedAttn a, c
 #pragma unroll
         for (int y = 8; y < kKeys; y += 8) {
 #pragma unroll
-          for (int z = 0; z < 4; ++z) top[z] = fmaxf(fmaxf(top[z], s[y + z]), s[y + z + 4]);
+          for (int z = 0; z < 4; ++z) top[z] = max3(top[z], s[y + z], s[y + z + 4]);
         }
         float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
         mx *= c;  // c > 0
@@ -554,51 +561,74 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const PagedAttn a, c
       float* part = plan.parts + ((size_t)blockIdx.x * 2 + (p.cut_begin ? 0 : 1)) * plan.part_floats;
       T* out = static_cast<T*>(a.out) + (size_t)(p.s.rq.t0 + p.token + t * plan.tile_tokens) * a.out_ld + (size_t)(p.s.g * rep) * hd;
       const uint32_t row_end = (p.tokens > t * plan.tile_tokens ? min(p.tokens - t * plan.tile_tokens, plan.tile_tokens) : 0u) * rep;  // of the tile
+      const bool boxed = plan.boxed && quarter * 32 + 32 <= row_end;  // a box of the output's map: all of the warp's rows
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;
       unsigned long long odd[2] = {pair_of(l * 0.0f, 0.0f), 0};  // NaN where anything is not finite
 #pragma unroll 1
-      for (uint32_t i = 0; i < hd; i += 32) {
-        float o[32];
-        if (n) tmem_ld32(o_at + i, o);
-        else {
-#pragma unroll
-          for (int y = 0; y < 32; ++y) o[y] = 0.0f;
-        }
-        if (i + 32 > hd) {  // columns that no product wrote
-#pragma unroll
-          for (int y = 0; y < 32; y += 8)
-            if (i + y >= hd) {
-#pragma unroll
-              for (int z = 0; z < 8; ++z) o[y + z] = 0.0f;
-            }
-        }
-#pragma unroll
-        for (int y = 0; y < 32; y += 2) odd[(y / 2) & 1] = fma2(pair_of(o[y], o[y + 1]), 0ull, odd[(y / 2) & 1]);
-        if (cut) {
-#pragma unroll
-          for (int y = 0; y < 32; y += 4)
-            if (live && i + y < hd) *reinterpret_cast<float4*>(part + ((size_t)((i + y) / 4) * kItemRows + t * kRows + row) * 4) = make_float4(o[y], o[y + 1], o[y + 2], o[y + 3]);
-        } else {
-#pragma unroll
-          for (int y = 0; y < 32; y += 8)
-            *reinterpret_cast<uint4*>(stage + lane * 64 + (((y / 8) ^ (lane >> 1)) & 3) * 16) =
-                make_uint4(pack2<T>(o[y] * inv, o[y + 1] * inv), pack2<T>(o[y + 2] * inv, o[y + 3] * inv), pack2<T>(o[y + 4] * inv, o[y + 5] * inv), pack2<T>(o[y + 6] * inv, o[y + 7] * inv));
+      for (uint32_t i = 0; i < hd; i += 64) {
+        if (!cut) {
+          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");  // the staged rows before have been read
           __syncwarp();
+        }
+#pragma unroll 1
+        for (uint32_t x = i; x < i + 64 && x < hd; x += 32) {
+          float o[32];
+          if (n) tmem_ld32(o_at + x, o);
+          else {
 #pragma unroll
-          for (uint32_t x = 0; x < 4; ++x) {  // eight rows of 64 bytes at a time
-            const uint32_t rr = 8 * x + (lane >> 2), at = quarter * 32 + rr, col = i + (lane & 3u) * 8;
-            const uint4 v = *reinterpret_cast<const uint4*>(stage + rr * 64 + (((lane & 3u) ^ (rr >> 1)) & 3u) * 16);
-            if (at < row_end && col < hd) *reinterpret_cast<uint4*>(out + row_at[x] + col) = v;
+            for (int y = 0; y < 32; ++y) o[y] = 0.0f;
           }
+          if (x + 32 > hd) {  // columns that no product wrote
+#pragma unroll
+            for (int y = 0; y < 32; y += 8)
+              if (x + y >= hd) {
+#pragma unroll
+                for (int z = 0; z < 8; ++z) o[y + z] = 0.0f;
+              }
+          }
+#pragma unroll
+          for (int y = 0; y < 32; y += 2) odd[(y / 2) & 1] = fma2(pair_of(o[y], o[y + 1]), 0ull, odd[(y / 2) & 1]);
+          if (cut) {
+#pragma unroll
+            for (int y = 0; y < 32; y += 4)
+              if (live && x + y < hd) *reinterpret_cast<float4*>(part + ((size_t)((x + y) / 4) * kItemRows + t * kRows + row) * 4) = make_float4(o[y], o[y + 1], o[y + 2], o[y + 3]);
+          } else {
+#pragma unroll
+            for (int y = 0; y < 32; y += 8)
+              *reinterpret_cast<uint4*>(stage + lane * 128 + ((((x & 32u) / 8 + y / 8) ^ lane) & 7u) * 16) =
+                  make_uint4(pack2<T>(o[y] * inv, o[y + 1] * inv), pack2<T>(o[y + 2] * inv, o[y + 3] * inv), pack2<T>(o[y + 4] * inv, o[y + 5] * inv), pack2<T>(o[y + 6] * inv, o[y + 7] * inv));
+          }
+        }
+        if (!cut) {
+          if (boxed) fence_proxy_async_smem();
           __syncwarp();
+          if (boxed) {
+            if (lane == 0) {
+              tma_store_3d(&maps.o, smem_u32(stage), (int)i, (int)(p.s.g * rep + box_head), (int)(p.s.rq.t0 + p.token + box_token));
+              asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+            }
+          } else {
+#pragma unroll 1
+            for (uint32_t x = 0; x < 32; x += 4) {  // four rows of 128 bytes at a time
+              const uint32_t rr = x + (lane >> 3), at = quarter * 32 + rr, col = i + (lane & 7u) * 8;
+              const uint4 v = *reinterpret_cast<const uint4*>(stage + rr * 128 + ((lane ^ rr) & 7u) * 16);
+              if (at < row_end && col < hd) *reinterpret_cast<uint4*>(out + (size_t)(at / rep) * a.out_ld + (size_t)(at % rep) * hd + col) = v;
+            }
+            __syncwarp();
+          }
         }
       }
       // rows that are not finite, key by key
       odd[0] = add2(odd[0], odd[1]);
       const bool fine = __uint_as_float((uint32_t)odd[0]) + __uint_as_float((uint32_t)(odd[0] >> 32)) == 0.0f;
-      for (uint32_t bad = __ballot_sync(0xFFFFFFFFu, live && !fine); bad; bad &= bad - 1) {
+      uint32_t bad = __ballot_sync(0xFFFFFFFFu, live && !fine);
+      if (bad) {
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");  // what they replace has been written
+        __syncwarp();
+      }
+      for (; bad; bad &= bad - 1) {
         const uint32_t who = (uint32_t)__ffs((int)bad) - 1, which = quarter * 32 + who;
-        float* tmp = s_again[warp - kControlWarps];
+        float* tmp = reinterpret_cast<float*>(stage);
         float m2, l2;
         row_again<T>(a, p.s, rep, p.s.row0 + t * plan.tile_tokens * rep + which, p.s.tile0 * kKeys, p.s.tile1 * kKeys, tmp, m2, l2);
         __syncwarp();
@@ -616,6 +646,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const PagedAttn a, c
       __syncwarp();
       if (lane == 0) mbar_arrive(&piece_empty[slot]);
     }
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
   }
   tc_fence_before_sync();
   __syncthreads();
@@ -668,12 +699,12 @@ EncodeFn encode_fn() {
   }();
   return fn;
 }
-// The queries [tokens][heads][hd], in boxes of 64 elements, a key head's query heads and a row tile's tokens; what lies outside reads as zero.
-CUresult encode_q(EncodeFn fn, CUtensorMap* map, const PagedAttn& a, uint32_t rep, uint32_t tile_tokens) {
-  const cuuint64_t dims[3] = {a.pool.hd, a.H, a.tokens}, strides[2] = {(cuuint64_t)a.pool.hd * 2, (cuuint64_t)a.q_ld * 2};
-  const cuuint32_t box[3] = {64, rep, tile_tokens}, one[3] = {1, 1, 1};
-  return fn(map, a.pool.dtype == RUAI_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(a.q), dims, strides, box, one,
-            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+// Queries or outputs [tokens][heads][hd], in boxes of 64 elements, some heads and some tokens; what lies outside reads as zero and is not written.
+CUresult encode_rows(EncodeFn fn, CUtensorMap* map, const PagedAttn& a, void* base, uint32_t ld, uint32_t heads, uint32_t tokens) {
+  const cuuint64_t dims[3] = {a.pool.hd, a.H, a.tokens}, strides[2] = {(cuuint64_t)a.pool.hd * 2, (cuuint64_t)ld * 2};
+  const cuuint32_t box[3] = {64, heads, tokens}, one[3] = {1, 1, 1};
+  return fn(map, a.pool.dtype == RUAI_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, base, dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
 }
 // A pool's rows (page, key head, position in the page) of hd elements, in boxes of box_rows x 64; elements past hd read as zero.
 CUresult encode(EncodeFn fn, CUtensorMap* map, const PagedPool& p, void* base, uint32_t box_rows) {
@@ -714,9 +745,11 @@ int ruai_paged_attention_tc(ruai_ctx* c, const PagedAttn& a, uint32_t rows_over)
   plan.part_floats = (p.hd + 2) * kItemRows;
   plan.tile_tokens = kRows / rep;
   Maps maps;
-  const CUresult rq = encode_q(fn, &maps.q, a, rep, plan.tile_tokens), rk = encode(fn, &maps.k, p, p.k, plan.box_rows), rv = encode(fn, &maps.v, p, p.v, plan.box_rows);
-  if (rq != CUDA_SUCCESS || rk != CUDA_SUCCESS || rv != CUDA_SUCCESS) {
-    ruai_fail(c, RUAI_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d, %d, %d) for %u pages of %u heads of %u", (int)rq, (int)rk, (int)rv, p.pages, p.KV, p.hd);
+  plan.boxed = 32 % rep == 0 || rep % 32 == 0;
+  const uint32_t heads = std::min(rep, 32u);
+  const CUresult rq = encode_rows(fn, &maps.q, a, const_cast<void*>(a.q), a.q_ld, rep, plan.tile_tokens), ro = encode_rows(fn, &maps.o, a, a.out, a.out_ld, heads, 32 / heads), rk = encode(fn, &maps.k, p, p.k, plan.box_rows), rv = encode(fn, &maps.v, p, p.v, plan.box_rows);
+  if (rq != CUDA_SUCCESS || ro != CUDA_SUCCESS || rk != CUDA_SUCCESS || rv != CUDA_SUCCESS) {
+    ruai_fail(c, RUAI_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d, %d, %d, %d) for %u pages of %u heads of %u", (int)rq, (int)ro, (int)rk, (int)rv, p.pages, p.KV, p.hd);
     return -1;
   }
   // parts of cut items: two per CTA.  Nothing may be allocated while the stream is captured; items then stay whole
