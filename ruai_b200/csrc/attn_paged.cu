@@ -8,13 +8,15 @@
 //   Split: the tiles of all items, in a row, are cut into equal runs, one per CTA, whatever the requests' lengths are (they are known to the
 // device only).  An item cut by a run's end leaves (m, l, o) of its part in scratch, and the CTA that arrives last joins the parts, in
 // their order: the same bits every time.
-//   Tile: four warps; WK = 4 / WR of them share an item's rows and take a part of the tile's keys each.  cp.async copies into padded
-// rows a few tiles ahead (rows behind the request's end arrive as zeros).  Products are mma.sync: the tensor pipe waits for HBM here, and 16 rows
+//   Tile: four warps; WK = 4 / WR of them share an item's rows and take a part of the tile's keys each.  A fifth walks the run and copies
+// tiles ahead, across items, page by page (TMA boxes with the 128-byte swizzle, so that eight rows of a column lie in eight banks of 16 bytes).  Products are mma.sync: the tensor pipe waits for HBM here, and 16 rows
 // by 8 keys fit few query heads where a tcgen05 tile would be a sixteenth full.  f32 operands are split in two tf32 numbers, x = hi + lo
 // (22 bits), three of the four products; the
 // tensor core's sums truncate, so it adds up 32 elements of a score and a tile's keys only, f32 registers the rest.  In 16 bits the weights are rounded once, to the values' type; l sums them unrounded.
 //   A row that is not finite at the end is worked out again key by key (row_again): a key that it does not see, or that weighs
 // nothing, must not reach it through 0 x inf.
+#include <cuda.h>
+
 #include <algorithm>
 
 #include "attn_paged.cuh"
@@ -60,53 +62,79 @@ template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, fl
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// 16 bytes into shared memory; zeros where `take` is false.
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool take) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(take ? 16 : 0) : "memory");
+__device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint64_t* bar) {
+  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst), "l"((uint64_t)map), "r"(x), "r"(y),
+               "r"(smem_u32(bar))
+               : "memory");
 }
-__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 // ---- the kernel ---------------------------------------------------------------------------------------------------------------
 
-constexpr int kThreads = 128;
+constexpr int kSoftWarps = 4, kThreads = 32 * (kSoftWarps + 1);
+constexpr int kSegments = 3;   // segments that the copying warp is ahead
+constexpr int kItemCost = 1;   // tiles that an item's queries and results take as long as
+constexpr int kTilesLeast = 3; // of a run, that cost included
 
 // HP: the head's width, up to 64, 128 or 256.  WR: warps that have rows of their own.
 template <typename T, int HP, int WR>
 struct Shape {
   static constexpr bool F32 = sizeof(T) == 4;
-  static constexpr int WK = 4 / WR, RB = 16 * WR, TK = F32 ? 32 : 64, KW = TK / WK;
-  static constexpr int PITCH = HP * (int)sizeof(T) + 16;  // bytes of a row in shared memory: eight rows of a column in eight banks of 16 bytes
-  static constexpr int STAGE = 2 * TK * PITCH;
-  static constexpr bool QSMEM = F32 || HP == 256;          // queries in shared memory, not in registers
-  static constexpr int QBYTES = QSMEM ? RB * PITCH : 0;
-  static constexpr int MERGE = 4 * 16 * (HP + 4) * 4;     // the warps' results at the end, in the tiles' place
-  static constexpr int STAGES = 3 * STAGE + QBYTES <= 110 * 1024 ? 3 : 2;
-  static constexpr int SMEM = STAGES * STAGE + QBYTES;
-  static_assert(MERGE <= STAGES * STAGE, "the results fit the tiles");
+  static constexpr int WK = 4 / WR, RB = 16 * WR, TK = !F32 ? 64 : HP == 256 && WR == 2 ? 16 : 32, KW = TK / WK;
+  static constexpr int PANEL_ELEMS = 128 / (int)sizeof(T), PANELS = HP / PANEL_ELEMS, PANEL = TK * 128;  // 128 bytes of every key of a tile
+  static constexpr int HALF = PANELS * PANEL, STAGE = 2 * HALF;                                          // keys, values
+  static constexpr bool QSMEM = F32 || HP == 256;  // queries in shared memory, not in registers
+  static constexpr int QPITCH = HP * (int)sizeof(T) + 16, QBYTES = QSMEM ? RB * QPITCH : 0;
+  static constexpr int MERGE = kSoftWarps * 16 * (HP + 4) * 4;  // the warps' results at the end, in the queries' place
+  static constexpr int KEPT = MERGE > QBYTES ? MERGE : QBYTES;
+  static constexpr bool ONE = HP == 256 || (HP == 128 && WR == 4);  // one CTA per SM: two have too few registers
+  static constexpr int ROOM = (ONE ? 216 : 108) * 1024 - KEPT, STAGES = ROOM / STAGE < 6 ? ROOM / STAGE : 6;
+  static constexpr int SMEM = STAGES * STAGE + KEPT + 1024;
+  static_assert(STAGES >= 2 && PANELS >= 1, "two stages at least");
   static constexpr size_t PART = (size_t)RB * (HP + 2) * sizeof(float);  // one part of an item in scratch
 };
+
+struct alignas(64) Maps { CUtensorMap k, v; };
 
 struct RowsPlan {
   float* parts;        // [CTAs][2]: the part that ends the item a CTA begins with, the part that begins the one it ends with
   unsigned* arrived;   // per CTA in which a cut item begins; zero between launches
   uint32_t rows_most;  // requests with more rows are another kernel's
-  uint32_t tiles_least;
+  uint32_t box_rows;
+};
+
+// What the copying warp tells the others of a segment.
+struct Work {
+  Segment s;
+  uint32_t ta, n;         // its tiles that a row sees
+  uint32_t whole0, whole1;  // keys that all rows see: [whole0, whole1)
+  uint32_t cut, first, last;  // 0: the whole item, 1: a part of it, 2: the part that begins it; the CTAs in which it begins and ends
+  uint32_t more;
 };
 
 template <typename T, int HP, int WR>
-__global__ void __launch_bounds__(kThreads, 2) rows_kernel(const PagedAttn a, const RowsPlan plan) {
+__global__ void __launch_bounds__(kThreads, Shape<T, HP, WR>::ONE ? 1 : 2) rows_kernel(const PagedAttn a, const RowsPlan plan, const __grid_constant__ Maps maps) {
   using S = Shape<T, HP, WR>;
-  constexpr int WK = S::WK, RB = S::RB, TK = S::TK, KW = S::KW, PITCH = S::PITCH, NS = TK / 16;
-  extern __shared__ __align__(128) unsigned char smem[];
-  __shared__ unsigned long long s_part[4], s_base;
+  constexpr int WK = S::WK, RB = S::RB, TK = S::TK, KW = S::KW, ST = S::STAGES;
+  extern __shared__ unsigned char smem_raw[];
+  __shared__ __align__(8) uint64_t full[ST], empty[ST], work_full[kSegments], work_empty[kSegments], meet;
+  __shared__ Work s_work[kSegments];
+  __shared__ unsigned long long s_part[kSoftWarps + 1], s_base;
   __shared__ uint32_t s_r, s_last;
-  __shared__ float s_m[4][16], s_l[4][16];
-  const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g4 = lane >> 2, t4 = lane & 3;
-  const uint32_t hd = a.pool.hd, KV = a.pool.KV, rep = a.H / KV, plog = a.pool.page_log2, pmask = (1u << plog) - 1u;
-  const uint32_t wr = WR == 1 ? 0 : warp % WR, wk = warp / WR;
-  const float c = a.scale * kLog2e;
-  unsigned char* qsm = smem + S::STAGES * S::STAGE;
+  __shared__ volatile int s_abort;
+  __shared__ float s_m[kSoftWarps][16], s_l[kSoftWarps][16];
+  const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const uint32_t hd = a.pool.hd, KV = a.pool.KV, rep = a.H / KV, plog = a.pool.page_log2;
+  unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  float* res = reinterpret_cast<float*>(smem + ST * S::STAGE);  // [warp][16][HP + 4]
+  unsigned char* qsm = smem + ST * S::STAGE;
+  if (tid == 0) {
+    for (int i = 0; i < ST; ++i) { pipe::mbar_init(&full[i], 1); pipe::mbar_init(&empty[i], kSoftWarps); }
+    for (int i = 0; i < kSegments; ++i) { pipe::mbar_init(&work_full[i], 1); pipe::mbar_init(&work_empty[i], kSoftWarps); }
+    pipe::mbar_init(&meet, kSoftWarps);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    s_abort = 0;
+  }
+  if (warp == 0 && lane < 2) asm volatile("prefetch.tensormap [%0];" ::"l"((uint64_t)(&maps.k + lane)) : "memory");
   grid_dependency_wait();
   grid_launch_dependents();
 
@@ -114,7 +142,7 @@ __global__ void __launch_bounds__(kThreads, 2) rows_kernel(const PagedAttn a, co
   auto tiles_of = [&](const PagedRequest& q) { return (q.len + TK - 1) / TK - paged_low(q.cached, a.window) / TK; };
   auto units_of = [&](const PagedRequest& q) -> unsigned long long {
     const uint32_t rows = q.fresh * rep;
-    return rows == 0 || rows > plan.rows_most ? 0ull : (unsigned long long)(KV * ((rows + RB - 1) / RB)) * tiles_of(q);
+    return rows == 0 || rows > plan.rows_most ? 0ull : (unsigned long long)(KV * ((rows + RB - 1) / RB)) * (tiles_of(q) + kItemCost);
   };
   const uint32_t per_thread = (a.R + kThreads - 1) / kThreads, ra = min(tid * per_thread, a.R), rb = min(ra + per_thread, a.R);
   unsigned long long mine = 0;
@@ -132,11 +160,11 @@ __global__ void __launch_bounds__(kThreads, 2) rows_kernel(const PagedAttn a, co
   if (lane == 31) s_part[warp] = inc;
   __syncthreads();
   unsigned long long before = inc - mine, total = 0;
-  for (uint32_t w = 0; w < 4; ++w) {
+  for (uint32_t w = 0; w <= (uint32_t)kSoftWarps; ++w) {
     if (w < warp) before += s_part[w];
     total += s_part[w];
   }
-  const unsigned long long per = max((total + gridDim.x - 1) / gridDim.x, (unsigned long long)plan.tiles_least);
+  const unsigned long long per = max((total + gridDim.x - 1) / gridDim.x, (unsigned long long)kTilesLeast);
   const unsigned long long u0 = per * blockIdx.x, u1 = min(u0 + per, total);
   if (u0 >= u1) return;
   if (before <= u0 && u0 < before + mine) {
@@ -150,87 +178,119 @@ __global__ void __launch_bounds__(kThreads, 2) rows_kernel(const PagedAttn a, co
     }
   }
   __syncthreads();
-  uint32_t r = s_r;
-  unsigned long long base = s_base, u = u0;
-  const size_t head_rows = (size_t)1 << plog;
 
-  auto clear_edge = [&]() {  // the half step behind the head's end: keys' columns that no copy writes
-    for (uint32_t x = tid; x < S::STAGES * TK; x += kThreads)
-      *reinterpret_cast<uint4*>(smem + (x / TK) * S::STAGE + (x % TK) * PITCH + hd * sizeof(T)) = make_uint4(0, 0, 0, 0);
+  bool ok = true;
+  // A warp whose wait ran out walks on without waiting, so that the others meet it; the results are void, and the host is told.
+  auto wait = [&](uint64_t* bar, uint32_t parity) {
+    if (ok) ok = __all_sync(0xFFFFFFFFu, !s_abort && pipe::mbar_wait(bar, parity));
+    if (!ok) s_abort = 1;
+    return ok;
   };
-  if (!S::F32 && hd % 16) clear_edge();
 
-  while (u < u1) {
-    Segment s;
-    s.r = r;
-    paged_request(a, r, s.rq);
-    const unsigned long long units = units_of(s.rq);
-    if (u >= base + units) { base += units; ++r; continue; }
-    const uint32_t tiles = tiles_of(s.rq), all_rows = s.rq.fresh * rep, blocks = (all_rows + RB - 1) / RB;
-    const uint32_t item = (uint32_t)((u - base) / tiles);
-    const unsigned long long item_u = base + (unsigned long long)item * tiles;
-    const uint32_t skip = paged_low(s.rq.cached, a.window) / TK;
-    s.g = item / blocks;
-    s.row0 = (item % blocks) * RB;
-    s.rows = min((uint32_t)RB, all_rows - s.row0);
-    s.tile0 = skip + (uint32_t)(u - item_u);
-    s.tile1 = skip + (uint32_t)(min(u1, item_u + tiles) - item_u);
-    // of these, the ones that the rows see
-    const uint32_t pos0 = s.rq.cached + s.row0 / rep, pos1 = s.rq.cached + (s.row0 + s.rows - 1) / rep;  // first and last row's positions
-    const uint32_t low0 = paged_low(pos0, a.window), low1 = paged_low(pos1, a.window);
-    const uint32_t ta = max(s.tile0, low0 / TK), tb = min(s.tile1, pos1 / TK + 1);
-    const int n = tb > ta ? (int)(tb - ta) : 0;
-
-    const T* kp = static_cast<const T*>(a.pool.k) + ((size_t)s.g << plog) * hd;
-    const T* vp = static_cast<const T*>(a.pool.v) + ((size_t)s.g << plog) * hd;
-    const size_t page_elems = (KV * head_rows) * hd;
-    int32_t pg[NS];  // pages of the tile to be requested next, 16 keys each
-    auto look_up = [&](uint32_t tile) {
-#pragma unroll
-      for (int i = 0; i < NS; ++i) {
-        const uint32_t j = tile * TK + 16 * i;
-        pg[i] = j < s.rq.len ? a.table[(size_t)r * a.table_ld + (j >> plog)] : -1;
-      }
+  if (warp == kSoftWarps) {
+    // ===== segments, their keys and values: a lane per box
+    uint32_t r = s_r, segs = 0, st = 0;  // stages asked for
+    unsigned long long base = s_base, u = u0;
+    const uint32_t boxes = TK / plan.box_rows, box = lane % boxes, panel = lane / boxes;
+    const uint32_t dst = smem_u32(smem) + panel * S::PANEL + box * plan.box_rows * 128;
+    auto page_at = [&](uint32_t tile, uint32_t len) {
+      const uint32_t key = tile * TK + box * plan.box_rows;
+      return key < len ? a.table[(size_t)r * a.table_ld + (key >> plog)] : -1;
     };
-    auto request = [&](uint32_t tile, uint32_t stage) {
-      const uint32_t chunks = hd * sizeof(T) / 16, kdst = smem_u32(smem) + stage * S::STAGE;
-#pragma unroll
-      for (int i = 0; i < NS; ++i) {
-        if (tile * TK + 16 * i < s.rq.len && (uint32_t)pg[i] >= a.pool.pages) {
+    while (u < u1 && ok) {
+      Work w;
+      w.s.r = r;
+      paged_request(a, r, w.s.rq);
+      const unsigned long long units = units_of(w.s.rq);
+      if (u >= base + units) { base += units; ++r; continue; }
+      const uint32_t tiles = tiles_of(w.s.rq), all_rows = w.s.rq.fresh * rep, blocks = (all_rows + RB - 1) / RB;
+      const uint32_t item = (uint32_t)((u - base) / (tiles + kItemCost));
+      const unsigned long long item_u = base + (unsigned long long)item * (tiles + kItemCost) + kItemCost;
+      if (u < item_u) { u = item_u; continue; }
+      const unsigned long long end = min(u1, item_u + tiles);
+      const uint32_t skip = paged_low(w.s.rq.cached, a.window) / TK;
+      w.s.g = item / blocks;
+      w.s.row0 = (item % blocks) * RB;
+      w.s.rows = min((uint32_t)RB, all_rows - w.s.row0);
+      w.s.tile0 = skip + (uint32_t)(u - item_u);
+      w.s.tile1 = skip + (uint32_t)(end - item_u);
+      w.first = (uint32_t)(item_u / per);
+      w.last = (uint32_t)((item_u + tiles - 1) / per);
+      w.cut = w.first == w.last ? 0u : u == item_u ? 2u : 1u;
+      // of these tiles, the ones that the rows see
+      const uint32_t pos0 = w.s.rq.cached + w.s.row0 / rep, pos1 = w.s.rq.cached + (w.s.row0 + w.s.rows - 1) / rep;  // first and last row's positions
+      w.whole0 = paged_low(pos1, a.window);
+      w.whole1 = pos0 + 1;
+      w.ta = max(w.s.tile0, paged_low(pos0, a.window) / TK);
+      const uint32_t tb = min(w.s.tile1, pos1 / TK + 1);
+      w.n = tb > w.ta ? tb - w.ta : 0;
+      w.more = 1;
+      int32_t pg = w.n ? page_at(w.ta, w.s.rq.len) : -1;
+      if (segs >= kSegments && !wait(&work_empty[segs % kSegments], (segs / kSegments - 1) & 1u)) break;
+      if (lane == 0) {
+        s_work[segs % kSegments] = w;
+        pipe::mbar_arrive(&work_full[segs % kSegments]);
+      }
+      ++segs;
+      for (uint32_t i = 0; i < w.n; ++i, ++st) {
+        const uint32_t key = (w.ta + i) * TK + box * plan.box_rows, slot = st % ST;
+        if (pg < -1 || pg >= (int32_t)a.pool.pages || (pg < 0 && key < w.s.rq.len)) {
           if (a.status) atomicCAS(a.status, 0, kStatusPaged);
-          pg[i] = -1;
+          pg = -1;
         }
-        for (uint32_t x = tid; x < 16 * chunks; x += kThreads) {
-          const uint32_t row = x / chunks, col = x % chunks, j = tile * TK + 16 * i + row;
-          const bool take = pg[i] >= 0 && j < s.rq.len;
-          const size_t at = take ? (size_t)pg[i] * page_elems + (size_t)(j & pmask) * hd + col * (16 / sizeof(T)) : 0;
-          const uint32_t d = kdst + (16 * i + row) * PITCH + col * 16;
-          copy16(d, kp + at, take);
-          copy16(d + TK * PITCH, vp + at, take);
+        const int y = pg >= 0 ? (int)((((uint32_t)pg * KV + w.s.g) << plog) + (key & ((1u << plog) - 1u))) : 0;
+        const bool take = pg >= 0 && panel * S::PANEL_ELEMS < hd;
+        const uint32_t bytes = 2 * __popc(__ballot_sync(0xFFFFFFFFu, take && panel < (uint32_t)S::PANELS)) * plan.box_rows * 128;
+        pg = i + 1 < w.n ? page_at(w.ta + i + 1, w.s.rq.len) : -1;
+        if (st >= ST && !wait(&empty[slot], (st / ST - 1) & 1u)) break;
+        if (lane == 0) pipe::mbar_expect_tx(&full[slot], bytes);
+        __syncwarp();
+        if (take && panel < (uint32_t)S::PANELS) {
+          tma_2d(dst + slot * S::STAGE, &maps.k, (int)panel * S::PANEL_ELEMS, y, &full[slot]);
+          tma_2d(dst + slot * S::STAGE + S::HALF, &maps.v, (int)panel * S::PANEL_ELEMS, y, &full[slot]);
         }
       }
-    };
-    if (n > 0) look_up(ta);
-#pragma unroll
-    for (int i = 0; i < S::STAGES - 1; ++i) {
-      if (i < n) {
-        request(ta + i, i);
-        if (i + 1 < n) look_up(ta + i + 1);
-      }
-      copy_commit();
+      u = end;
     }
+    if (ok && (segs < kSegments || wait(&work_empty[segs % kSegments], (segs / kSegments - 1) & 1u)) && lane == 0) {
+      s_work[segs % kSegments].more = 0;
+      pipe::mbar_arrive(&work_full[segs % kSegments]);
+    }
+    // leave no copy in flight into shared memory that another CTA may get
+    for (uint32_t i = st > ST ? st - ST : 0; i < st; ++i) (void)pipe::mbar_wait(&full[i % ST], (i / ST) & 1u);
+    if (s_abort && lane == 0 && a.status) atomicCAS(a.status, 0, 3);
+    return;
+  }
+
+  // ===== products and softmax
+  const uint32_t g4 = lane >> 2, t4 = lane & 3, wr = WR == 1 ? 0 : warp % WR, wk = warp / WR;
+  const float c = a.scale * kLog2e;
+  uint32_t st = 0, meets = 0;
+  auto gather = [&]() {  // the four warps meet
+    __syncwarp();
+    if (lane == 0) pipe::mbar_arrive(&meet);
+    wait(&meet, meets++ & 1u);
+  };
+  for (uint32_t segs = 0;; ++segs) {
+    if (!wait(&work_full[segs % kSegments], (segs / kSegments) & 1u)) return;  // the copying warp has given up: nobody meets again
+    const Work& w = s_work[segs % kSegments];
+    if (!w.more) return;
+    const Segment& s = w.s;
+    const uint32_t t0 = s.rq.t0, cached = s.rq.cached, len = s.rq.len, row_end = s.row0 + s.rows, n = w.n, ta = w.ta;
 
     // ---- queries
-    const uint32_t row_lo = s.row0 + wr * 16 + g4, row_hi = row_lo + 8, row_end = s.row0 + s.rows;
-    auto q_at = [&](uint32_t row) { return static_cast<const T*>(a.q) + (size_t)(s.rq.t0 + row / rep) * a.q_ld + (size_t)(s.g * rep + row % rep) * hd; };
+    const uint32_t row_lo = s.row0 + wr * 16 + g4, row_hi = row_lo + 8;
+    auto q_at = [&](uint32_t row) { return static_cast<const T*>(a.q) + (size_t)(t0 + row / rep) * a.q_ld + (size_t)(s.g * rep + row % rep) * hd; };
     uint32_t qf[S::QSMEM ? 1 : HP / 16][4];
     if constexpr (S::QSMEM) {
-      for (uint32_t x = tid; x < RB * (HP * sizeof(T) / 16); x += kThreads) {
-        const uint32_t row = x / (HP * sizeof(T) / 16), col = x % (HP * sizeof(T) / 16);
+      constexpr uint32_t kChunks = HP * sizeof(T) / 16;
+      for (uint32_t x = tid; x < RB * kChunks; x += 32 * kSoftWarps) {
+        const uint32_t row = x / kChunks, col = x % kChunks;
         uint4 v = make_uint4(0, 0, 0, 0);
         if (row < s.rows && col * (16 / sizeof(T)) < hd) v = *reinterpret_cast<const uint4*>(q_at(s.row0 + row) + col * (16 / sizeof(T)));
-        *reinterpret_cast<uint4*>(qsm + row * PITCH + col * 16) = v;
+        *reinterpret_cast<uint4*>(qsm + row * S::QPITCH + col * 16) = v;
       }
+      gather();
     } else {
       const T* q0 = row_lo < row_end ? q_at(row_lo) : nullptr;
       const T* q1 = row_hi < row_end ? q_at(row_hi) : nullptr;
@@ -243,8 +303,8 @@ __global__ void __launch_bounds__(kThreads, 2) rows_kernel(const PagedAttn a, co
           qf[e][2 * h + 1] = q1 && col < hd ? *reinterpret_cast<const uint32_t*>(q1 + col) : 0u;
         }
     }
-    const uint32_t p_lo = s.rq.cached + min(row_lo, row_end - 1) / rep, p_hi = s.rq.cached + min(row_hi, row_end - 1) / rep;
-    const uint32_t l_lo = paged_low(p_lo, a.window), l_hi = paged_low(p_hi, a.window);
+    const uint32_t p_lo = cached + min(row_lo, row_end - 1) / rep, p_hi = cached + min(row_hi, row_end - 1) / rep;
+    const uint32_t l_lo = paged_low(p_lo, a.window), l_hi = paged_low(p_hi, a.window), whole0 = w.whole0, whole1 = w.whole1;
 
     float o[HP / 8][4], m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
 #pragma unroll
@@ -252,23 +312,26 @@ __global__ void __launch_bounds__(kThreads, 2) rows_kernel(const PagedAttn a, co
 #pragma unroll
       for (int j = 0; j < 4; ++j) o[i][j] = 0.0f;
 
-    for (int i = 0; i < n; ++i) {
-      copy_wait<S::STAGES - 2>();
-      __syncthreads();
-      if (i + S::STAGES - 1 < n) {
-        request(ta + i + S::STAGES - 1, (i + S::STAGES - 1) % S::STAGES);
-        if (i + S::STAGES < n) look_up(ta + i + S::STAGES);
-      }
-      copy_commit();
-      const unsigned char* ks = smem + (i % S::STAGES) * S::STAGE + wk * KW * PITCH;
-      const unsigned char* vs = ks + TK * PITCH;
+    for (uint32_t i = 0; i < n; ++i, ++st) {
+      const uint32_t slot = st % ST;
+      wait(&full[slot], (st / ST) & 1u);
+      unsigned char* ks = smem + slot * S::STAGE + wk * KW * 128;
+      unsigned char* vs = ks + S::HALF;
       const uint32_t key0 = (ta + i) * TK + wk * KW;
+      if (key0 + KW > len) {  // positions behind the request's end: their values weigh nothing, and must be numbers for that
+        for (uint32_t x = lane; x < KW * 8 * S::PANELS; x += 32) {
+          const uint32_t row = x / 8 % KW;
+          if (key0 + row >= len) *reinterpret_cast<uint4*>(vs + x / (8 * KW) * S::PANEL + row * 128 + (x & 7u) * 16) = make_uint4(0, 0, 0, 0);
+        }
+        pipe::fence_proxy_async_smem();
+        __syncwarp();
+      }
       float sc[KW / 8][4];
 #pragma unroll
       for (int j = 0; j < KW / 8; ++j) sc[j][0] = sc[j][1] = sc[j][2] = sc[j][3] = 0.0f;
       if constexpr (!S::F32) {
-        const uint32_t kaddr = smem_u32(ks) + ((lane & 7) + ((lane >> 4) << 3)) * PITCH + ((lane >> 3) & 1) * 16;
-        const uint32_t qaddr = smem_u32(qsm) + (wr * 16 + (lane & 15)) * PITCH + (lane >> 4) * 16;
+        const uint32_t kaddr = smem_u32(ks) + ((lane & 7) + ((lane >> 4) << 3)) * 128, hi = (lane >> 3) & 1, sw = lane & 7;
+        const uint32_t qaddr = smem_u32(qsm) + (wr * 16 + (lane & 15)) * S::QPITCH + (lane >> 4) * 16;
 #pragma unroll
         for (int e = 0; e < HP / 16; ++e) {
           if (HP != 64 && e * 16 >= (int)hd) break;
@@ -278,14 +341,15 @@ __global__ void __launch_bounds__(kThreads, 2) rows_kernel(const PagedAttn a, co
 #pragma unroll
           for (int j = 0; j < KW / 16; ++j) {
             uint32_t b[4];
-            ldmatrix4(b, kaddr + j * 16 * PITCH + e * 32);
+            ldmatrix4(b, kaddr + (e / 4) * S::PANEL + j * 16 * 128 + ((((e & 3) * 2 + hi) ^ sw) << 4));
             mma16<T>(sc[2 * j], qa, b[0], b[1]);
             mma16<T>(sc[2 * j + 1], qa, b[2], b[3]);
           }
         }
       } else {
-        const float* kf = reinterpret_cast<const float*>(ks) + g4 * (PITCH / 4) + t4;
-        const float* qs = reinterpret_cast<const float*>(qsm) + (wr * 16 + g4) * (PITCH / 4) + t4;
+        const unsigned char* kf = ks + g4 * 128 + t4 * 4;
+        const float* qs = reinterpret_cast<const float*>(qsm) + (wr * 16 + g4) * (S::QPITCH / 4) + t4;
+#pragma unroll 1
         for (uint32_t e0 = 0; e0 < hd / 8; e0 += 4) {  // 32 elements of the head at a time
           float part[KW / 8][4];
 #pragma unroll
@@ -296,14 +360,15 @@ __global__ void __launch_bounds__(kThreads, 2) rows_kernel(const PagedAttn a, co
             if (e >= hd / 8) break;
             uint32_t ah[4], al[4];
             split_tf32(qs[e * 8], ah[0], al[0]);
-            split_tf32(qs[e * 8 + 8 * (PITCH / 4)], ah[1], al[1]);
+            split_tf32(qs[e * 8 + 8 * (S::QPITCH / 4)], ah[1], al[1]);
             split_tf32(qs[e * 8 + 4], ah[2], al[2]);
-            split_tf32(qs[e * 8 + 8 * (PITCH / 4) + 4], ah[3], al[3]);
+            split_tf32(qs[e * 8 + 8 * (S::QPITCH / 4) + 4], ah[3], al[3]);
 #pragma unroll
             for (int j = 0; j < KW / 8; ++j) {
+              const unsigned char* kj = kf + (e0 / 4) * S::PANEL + j * 8 * 128;
               uint32_t bh[2], bl[2];
-              split_tf32(kf[j * 8 * (PITCH / 4) + e * 8], bh[0], bl[0]);
-              split_tf32(kf[j * 8 * (PITCH / 4) + e * 8 + 4], bh[1], bl[1]);
+              split_tf32(*reinterpret_cast<const float*>(kj + (((2 * f) ^ g4) << 4)), bh[0], bl[0]);
+              split_tf32(*reinterpret_cast<const float*>(kj + (((2 * f + 1) ^ g4) << 4)), bh[1], bl[1]);
               mma8(part[j], al, bh[0], bh[1]);
               mma8(part[j], ah, bl[0], bl[1]);
               mma8(part[j], ah, bh[0], bh[1]);
@@ -316,7 +381,7 @@ __global__ void __launch_bounds__(kThreads, 2) rows_kernel(const PagedAttn a, co
         }
       }
       // ---- softmax; row g4 in elements 0 and 1, row g4 + 8 in 2 and 3
-      const bool whole = (ta + i) * TK >= low1 && (ta + i) * TK + TK <= pos0 + 1;
+      const bool whole = key0 >= whole0 && key0 + KW <= whole1;
 #pragma unroll
       for (int j = 0; j < KW / 8; ++j)
 #pragma unroll
@@ -356,7 +421,7 @@ __global__ void __launch_bounds__(kThreads, 2) rows_kernel(const PagedAttn a, co
       }
       // ---- weighted values
       if constexpr (!S::F32) {
-        const uint32_t vaddr = smem_u32(vs) + ((lane & 7) + ((lane >> 3) & 1) * 8) * PITCH + (lane >> 4) * 16;
+        const uint32_t vaddr = smem_u32(vs) + ((lane & 7) + ((lane >> 3) & 1) * 8) * 128, hi = lane >> 4, sw = lane & 7;
 #pragma unroll
         for (int j = 0; j < KW / 16; ++j) {
           const uint32_t pa[4] = {pack2<T>(sc[2 * j][0], sc[2 * j][1]), pack2<T>(sc[2 * j][2], sc[2 * j][3]), pack2<T>(sc[2 * j + 1][0], sc[2 * j + 1][1]),
@@ -365,13 +430,13 @@ __global__ void __launch_bounds__(kThreads, 2) rows_kernel(const PagedAttn a, co
           for (int d = 0; d < HP / 16; ++d) {
             if (HP != 64 && d * 16 >= (int)hd) break;
             uint32_t b[4];
-            ldmatrix4t(b, vaddr + j * 16 * PITCH + d * 32);
+            ldmatrix4t(b, vaddr + (d / 4) * S::PANEL + j * 16 * 128 + ((((d & 3) * 2 + hi) ^ sw) << 4));
             mma16<T>(o[2 * d], pa, b[0], b[1]);
             mma16<T>(o[2 * d + 1], pa, b[2], b[3]);
           }
         }
       } else {
-        const float* vf = reinterpret_cast<const float*>(vs) + 2 * t4 * (PITCH / 4) + g4;
+        const unsigned char* v0 = vs + 2 * t4 * 128 + (g4 & 3) * 4;
         uint32_t ph[KW / 8][4], pl[KW / 8][4];  // the product's k is key 2 t4 for t4, 2 t4 + 1 for t4 + 4
 #pragma unroll
         for (int j = 0; j < KW / 8; ++j) {
@@ -383,12 +448,14 @@ __global__ void __launch_bounds__(kThreads, 2) rows_kernel(const PagedAttn a, co
 #pragma unroll
         for (int d = 0; d < HP / 8; ++d) {
           if (d * 8 >= (int)hd) break;
+          const uint32_t ch = (d & 3) * 2 + (g4 >> 2);
           float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
           for (int j = 0; j < KW / 8; ++j) {
+            const unsigned char* vj = v0 + (d / 4) * S::PANEL + j * 8 * 128;
             uint32_t bh[2], bl[2];
-            split_tf32(vf[j * 8 * (PITCH / 4) + d * 8], bh[0], bl[0]);
-            split_tf32(vf[(j * 8 + 1) * (PITCH / 4) + d * 8], bh[1], bl[1]);
+            split_tf32(*reinterpret_cast<const float*>(vj + ((ch ^ (2 * t4)) << 4)), bh[0], bl[0]);
+            split_tf32(*reinterpret_cast<const float*>(vj + 128 + ((ch ^ (2 * t4 + 1)) << 4)), bh[1], bl[1]);
             mma8(part, pl[j], bh[0], bh[1]);
             mma8(part, ph[j], bl[0], bl[1]);
             mma8(part, ph[j], bh[0], bh[1]);
@@ -397,17 +464,17 @@ __global__ void __launch_bounds__(kThreads, 2) rows_kernel(const PagedAttn a, co
           for (int x = 0; x < 4; ++x) o[d][x] += part[x];
         }
       }
+      __syncwarp();
+      if (lane == 0) pipe::mbar_arrive(&empty[slot]);
     }
 
-    // ---- the warps' results meet in the tiles' place
-    copy_wait<0>();
-    __syncthreads();
+    // ---- the warps' results meet
 #pragma unroll
     for (int off = 1; off < 4; off <<= 1) {
       l0 += __shfl_xor_sync(0xFFFFFFFFu, l0, off);
       l1 += __shfl_xor_sync(0xFFFFFFFFu, l1, off);
     }
-    float* res = reinterpret_cast<float*>(smem);  // [warp][16][HP + 4]
+    if constexpr (S::QSMEM) gather();  // the queries have been read
     {
       float* d0 = res + (warp * 16 + g4) * (HP + 4) + 2 * t4;
       float* d1 = d0 + 8 * (HP + 4);
@@ -419,21 +486,21 @@ __global__ void __launch_bounds__(kThreads, 2) rows_kernel(const PagedAttn a, co
       }
       if (t4 == 0) { s_m[warp][g4] = m0; s_l[warp][g4] = l0; s_m[warp][g4 + 8] = m1; s_l[warp][g4 + 8] = l1; }
     }
-    __syncthreads();
-    const bool cut_begin = u != item_u, cut_end = item_u + tiles > u1;
-    const bool cut = cut_begin || cut_end;
-    float* part = plan.parts + ((size_t)blockIdx.x * 2 + (cut_begin ? 0 : 1)) * (RB * (HP + 2));
+    gather();
+    const uint32_t cut = w.cut, first = w.first, last = w.last;
+    float* part = plan.parts + ((size_t)blockIdx.x * 2 + (cut == 2 ? 1 : 0)) * (RB * (HP + 2));
+    auto out_at = [&](uint32_t row) { return static_cast<T*>(a.out) + (size_t)(t0 + row / rep) * a.out_ld + (size_t)(s.g * rep + row % rep) * hd; };
     // a warp per row
-    for (uint32_t row = warp; row < s.rows; row += 4) {
+    for (uint32_t row = warp; row < s.rows; row += kSoftWarps) {
       const uint32_t w0 = row / 16, rr = row % 16;  // the row's warps are w0, w0 + WR, ...
-      float m = -INFINITY, l = 0.0f, f[WK], v[kHeadParts];
+      float m = -INFINITY, l = 0.0f, f[WK], v[HP / 32];
 #pragma unroll
-      for (int w = 0; w < WK; ++w) m = fmaxf(m, s_m[w0 + w * WR][rr]);
+      for (int x = 0; x < WK; ++x) m = fmaxf(m, s_m[w0 + x * WR][rr]);
 #pragma unroll
-      for (int w = 0; w < WK; ++w) {
-        const float mw = s_m[w0 + w * WR][rr];
-        f[w] = mw == -INFINITY ? 0.0f : exp2_of(mw - m);
-        l = fmaf(s_l[w0 + w * WR][rr], f[w], l);
+      for (int x = 0; x < WK; ++x) {
+        const float mw = s_m[w0 + x * WR][rr];
+        f[x] = mw == -INFINITY ? 0.0f : exp2_of(mw - m);
+        l = fmaf(s_l[w0 + x * WR][rr], f[x], l);
       }
       bool fine = isfinite(l);
 #pragma unroll
@@ -442,7 +509,7 @@ __global__ void __launch_bounds__(kThreads, 2) rows_kernel(const PagedAttn a, co
         v[j] = 0.0f;
         if (e < hd) {
 #pragma unroll
-          for (int w = 0; w < WK; ++w) v[j] = fmaf(res[((w0 + w * WR) * 16 + rr) * (HP + 4) + e], f[w], v[j]);
+          for (int x = 0; x < WK; ++x) v[j] = fmaf(res[((w0 + x * WR) * 16 + rr) * (HP + 4) + e], f[x], v[j]);
           fine = fine && isfinite(v[j]);
         }
       }
@@ -454,8 +521,7 @@ __global__ void __launch_bounds__(kThreads, 2) rows_kernel(const PagedAttn a, co
         for (int j = 0; j < HP / 32; ++j) v[j] = lane + 32 * j < hd ? again[lane + 32 * j] : 0.0f;
       }
       if (!cut) {
-        const uint32_t x = s.row0 + row;
-        T* dst = static_cast<T*>(a.out) + (size_t)(s.rq.t0 + x / rep) * a.out_ld + (size_t)(s.g * rep + x % rep) * hd;
+        T* dst = out_at(s.row0 + row);
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
         for (int j = 0; j < HP / 32; ++j)
@@ -470,14 +536,13 @@ __global__ void __launch_bounds__(kThreads, 2) rows_kernel(const PagedAttn a, co
     }
     if (cut) {
       // ---- the item's parts, joined by the CTA that comes last
-      const uint32_t first = (uint32_t)(item_u / per), last = (uint32_t)((item_u + tiles - 1) / per);
       __threadfence();
-      __syncthreads();
+      gather();
       if (tid == 0) s_last = atomicAdd(&plan.arrived[first], 1u) == last - first ? 1u : 0u;
-      __syncthreads();
+      gather();
       if (s_last) {
         __threadfence();
-        for (uint32_t row = warp; row < s.rows; row += 4) {
+        for (uint32_t row = warp; row < s.rows; row += kSoftWarps) {
           auto part_of = [&](uint32_t p) { return plan.parts + ((size_t)p * 2 + (p == first ? 1 : 0)) * (RB * (HP + 2)) + row * (HP + 2); };
           float m = -INFINITY;
           for (uint32_t p = first + lane; p <= last; p += 32) m = fmaxf(m, __ldcg(part_of(p) + HP));
@@ -495,8 +560,7 @@ __global__ void __launch_bounds__(kThreads, 2) rows_kernel(const PagedAttn a, co
             for (int j = 0; j < HP / 32; ++j)
               if (lane + 32 * j < hd) v[j] = fmaf(__ldcg(src + lane + 32 * j), f, v[j]);
           }
-          const uint32_t x = s.row0 + row;
-          T* dst = static_cast<T*>(a.out) + (size_t)(s.rq.t0 + x / rep) * a.out_ld + (size_t)(s.g * rep + x % rep) * hd;
+          T* dst = out_at(s.row0 + row);
 #pragma unroll
           for (int j = 0; j < HP / 32; ++j)
             if (lane + 32 * j < hd) dst[lane + 32 * j] = from_f32<T>(l == 0.0f ? 0.0f : v[j] / l);
@@ -504,38 +568,51 @@ __global__ void __launch_bounds__(kThreads, 2) rows_kernel(const PagedAttn a, co
         if (tid == 0) plan.arrived[first] = 0;
       }
     }
-    __syncthreads();  // the results have been read: tiles may come in their place
-    if (!S::F32 && hd % 16) clear_edge();
-    u = item_u + (s.tile1 - skip);
+    gather();  // the results have been read
+    if (lane == 0) pipe::mbar_arrive(&work_empty[segs % kSegments]);
   }
 }
 
+// A pool's rows (page, key head, position in the page) of hd elements, in boxes of box_rows x 128 bytes; elements past hd read as zero.
+CUresult encode(CUtensorMap* map, const PagedPool& p, void* base, uint32_t box_rows) {
+  const bool f32 = p.dtype == RUAI_F32;
+  const cuuint64_t dims[2] = {p.hd, ((cuuint64_t)p.pages * p.KV) << p.page_log2}, strides[1] = {(cuuint64_t)p.hd * (f32 ? 4 : 2)};
+  const cuuint32_t box[2] = {f32 ? 32u : 64u, box_rows}, one[2] = {1, 1};
+  return ruai_tensor_map_fn()(map, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : p.dtype == RUAI_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, base, dims,
+                              strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+}
+
 template <typename T, int HP, int WR>
-cudaError_t launch_rows(ruai_ctx* c, const PagedAttn& a, uint32_t rows_most) {
+int launch_rows(ruai_ctx* c, const PagedAttn& a, uint32_t rows_most) {
   using S = Shape<T, HP, WR>;
   static int per_sm[64] = {};
   int& n = per_sm[c->ordinal & 63];
   if (!n) {
-    cudaError_t e = cudaFuncSetAttribute(rows_kernel<T, HP, WR>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
-    if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, rows_kernel<T, HP, WR>, kThreads, S::SMEM);
-    if (e != cudaSuccess) return e;
+    RUAI_CUDA(c, cudaFuncSetAttribute(rows_kernel<T, HP, WR>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM));
+    RUAI_CUDA(c, cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, rows_kernel<T, HP, WR>, kThreads, S::SMEM));
     n = std::max(n, 1);
   }
-  RowsPlan p = {c->partial, c->counters, rows_most, 2};
+  RowsPlan p = {c->partial, c->counters, rows_most, std::min(1u << a.pool.page_log2, (uint32_t)S::TK)};
+  Maps maps;
+  if (!ruai_tensor_map_fn()) return ruai_fail(c, RUAI_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
+  const CUresult rk = encode(&maps.k, a.pool, a.pool.k, p.box_rows), rv = encode(&maps.v, a.pool, a.pool.v, p.box_rows);
+  if (rk != CUDA_SUCCESS || rv != CUDA_SUCCESS)
+    return ruai_fail(c, RUAI_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d, %d) for %u pages of %u heads of %u", (int)rk, (int)rv, a.pool.pages, a.pool.KV, a.pool.hd);
   // a run per resident CTA, as far as the context's first scratch holds their parts: it never grows for them
   const uint32_t grid = (uint32_t)std::min<size_t>((size_t)c->sm_count * n, kScratchBytes / (2 * S::PART));
-  return ruai_launch(c, rows_kernel<T, HP, WR>, dim3(grid), dim3(kThreads), S::SMEM, true, a, p);
+  RUAI_CUDA(c, ruai_launch(c, rows_kernel<T, HP, WR>, dim3(grid), dim3(kThreads), S::SMEM, true, a, p, maps));
+  return RUAI_OK;
 }
 
 template <typename T, int HP>
-cudaError_t launch_width(ruai_ctx* c, const PagedAttn& a, uint32_t rows, uint32_t rows_most) {
+int launch_width(ruai_ctx* c, const PagedAttn& a, uint32_t rows, uint32_t rows_most) {
   if (rows <= 16) return launch_rows<T, HP, 1>(c, a, rows_most);
   if (rows <= 32 || HP == 256) return launch_rows<T, HP, 2>(c, a, rows_most);
   return launch_rows<T, HP == 256 ? 128 : HP, 4>(c, a, rows_most);
 }
 
 template <typename T>
-cudaError_t launch_type(ruai_ctx* c, const PagedAttn& a, uint32_t rows, uint32_t rows_most) {
+int launch_type(ruai_ctx* c, const PagedAttn& a, uint32_t rows, uint32_t rows_most) {
   return a.pool.hd <= 64    ? launch_width<T, 64>(c, a, rows, rows_most)
          : a.pool.hd <= 128 ? launch_width<T, 128>(c, a, rows, rows_most)
                             : launch_width<T, 256>(c, a, rows, rows_most);
@@ -555,8 +632,7 @@ int ruai_paged_attention_launch(ruai_ctx* c, const PagedAttn& a) {
     if (took && !over) return RUAI_OK;
     if (took) rows = rows_most = over;
   }
-  RUAI_CUDA(c, a.pool.dtype == RUAI_F32   ? launch_type<float>(c, a, rows, rows_most)
-               : a.pool.dtype == RUAI_F16 ? launch_type<__half>(c, a, rows, rows_most)
-                                          : launch_type<__nv_bfloat16>(c, a, rows, rows_most));
-  return RUAI_OK;
+  return a.pool.dtype == RUAI_F32   ? launch_type<float>(c, a, rows, rows_most)
+         : a.pool.dtype == RUAI_F16 ? launch_type<__half>(c, a, rows, rows_most)
+                                    : launch_type<__nv_bfloat16>(c, a, rows, rows_most);
 }

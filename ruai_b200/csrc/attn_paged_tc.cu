@@ -12,8 +12,6 @@
 // scratch, and join_kernel adds them up, many CTAs to an item (the last CTA to arrive alone took 90 us for 17 parts).
 //   Values of the positions behind a request's end are cleared in shared memory (0 x NaN), and a row that is not finite at the end is worked
 // out again key by key.  Every mbarrier wait is bounded.
-#include <cuda.h>
-
 #include <algorithm>
 #include <type_traits>
 
@@ -688,26 +686,15 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const PagedAttn a, c
   }
 }
 
-typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
-                             const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-EncodeFn encode_fn() {
-  static EncodeFn fn = [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult st;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &st) != cudaSuccess || st != cudaDriverEntryPointSuccess) p = nullptr;
-    return (EncodeFn)p;
-  }();
-  return fn;
-}
 // Queries or outputs [tokens][heads][hd], in boxes of 64 elements, some heads and some tokens; what lies outside reads as zero and is not written.
-CUresult encode_rows(EncodeFn fn, CUtensorMap* map, const PagedAttn& a, void* base, uint32_t ld, uint32_t heads, uint32_t tokens) {
+CUresult encode_rows(ruai_tensor_map_encode fn, CUtensorMap* map, const PagedAttn& a, void* base, uint32_t ld, uint32_t heads, uint32_t tokens) {
   const cuuint64_t dims[3] = {a.pool.hd, a.H, a.tokens}, strides[2] = {(cuuint64_t)a.pool.hd * 2, (cuuint64_t)ld * 2};
   const cuuint32_t box[3] = {64, heads, tokens}, one[3] = {1, 1, 1};
   return fn(map, a.pool.dtype == RUAI_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, base, dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
 }
 // A pool's rows (page, key head, position in the page) of hd elements, in boxes of box_rows x 64; elements past hd read as zero.
-CUresult encode(EncodeFn fn, CUtensorMap* map, const PagedPool& p, void* base, uint32_t box_rows) {
+CUresult encode(ruai_tensor_map_encode fn, CUtensorMap* map, const PagedPool& p, void* base, uint32_t box_rows) {
   const cuuint64_t dims[2] = {p.hd, ((cuuint64_t)p.pages * p.KV) << p.page_log2}, strides[1] = {(cuuint64_t)p.hd * 2};
   const cuuint32_t box[2] = {64, box_rows}, one[2] = {1, 1};
   return fn(map, p.dtype == RUAI_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, base, dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
@@ -737,7 +724,7 @@ int ruai_paged_attention_tc(ruai_ctx* c, const PagedAttn& a, uint32_t rows_over)
   // heads narrower than a copied box, and scores that shrink with their product, stay on attn_paged.cu
   const uint32_t rep = a.H / p.KV;
   if (!c->use_tc || p.dtype == RUAI_F32 || p.hd < 64 || p.hd > 128 || rep > (uint32_t)kRows || !(a.scale > 0.0f)) return 0;
-  EncodeFn fn = encode_fn();
+  const ruai_tensor_map_encode fn = ruai_tensor_map_fn();
   if (!fn) { ruai_fail(c, RUAI_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver"); return -1; }
   TcPlan plan = {};
   plan.rows_over = rows_over;

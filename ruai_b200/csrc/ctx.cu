@@ -124,6 +124,7 @@ int ruai_ctx_check_status(ruai_ctx* c) {
 int ruai_ctx_status_result(ruai_ctx* c, int st) {
   if (st == 0) return RUAI_OK;
   cudaMemsetAsync(c->status, 0, sizeof(int), c->stream);
+  if (st == 3) cudaMemsetAsync(c->counters, 0, c->counters_n * sizeof(unsigned), c->stream);  // a launch that gave up may have left some counted
   if (c->ps_sync) {  // a persistent launch that gave up leaves its barrier count undefined: start over
     cudaMemsetAsync(c->ps_sync, 0, 64, c->stream);
     c->ps_bar_base = 0;

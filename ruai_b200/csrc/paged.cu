@@ -10,7 +10,7 @@
 // append_kernel.  A CTA per token; a thread takes eight elements of a head, the two fours that rotate into each other where there is a
 // rotation: y_i = x_i cos - x_(i+h) sin, y_(i+h) = x_(i+h) cos + x_i sin, in f32, rounded once to the cache's type.  Bound by HBM: every
 // element is read and written once.
-#include "paged.cuh"
+#include "attn_paged.cuh"
 #include "pipeline.cuh"
 
 namespace {
@@ -222,6 +222,16 @@ int ruai_paged_check_pool(ruai_ctx* c, const PagedPool& p, const char* who) {
     return ruai_fail(c, RUAI_ERR_SHAPE, "%s: %u pages of %u x %u rows are 2^31 rows or more", who, p.pages, p.KV, 1u << p.page_log2);
   if (!aligned(p.k, 16) || !aligned(p.v, 16)) return ruai_fail(c, RUAI_ERR_ARG, "%s: pages must start on 16-byte boundaries", who);
   return RUAI_OK;
+}
+
+ruai_tensor_map_encode ruai_tensor_map_fn() {
+  static const ruai_tensor_map_encode fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult st;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &st) != cudaSuccess || st != cudaDriverEntryPointSuccess) p = nullptr;
+    return (ruai_tensor_map_encode)p;
+  }();
+  return fn;
 }
 
 int ruai_paged_append_launch(ruai_ctx* c, const PagedAppend& a) {
