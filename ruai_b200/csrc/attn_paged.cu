@@ -349,35 +349,47 @@ __global__ void __launch_bounds__(kThreads, Shape<T, HP, WR>::ONE ? 1 : 2) rows_
       } else {
         const unsigned char* kf = ks + g4 * 128 + t4 * 4;
         const float* qs = reinterpret_cast<const float*>(qsm) + (wr * 16 + g4) * (S::QPITCH / 4) + t4;
+        constexpr int G = KW >= 32 ? 1 : HP == 64 ? 2 : 32 / KW;  // panels at a time: four sums that do not wait for one another, where there are
 #pragma unroll 1
-        for (uint32_t e0 = 0; e0 < hd / 8; e0 += 4) {  // 32 elements of the head at a time
-          float part[KW / 8][4];
+        for (uint32_t p0 = 0; 32 * p0 < hd; p0 += G) {
+          float part[G][KW / 8][4];
 #pragma unroll
-          for (int j = 0; j < KW / 8; ++j) part[j][0] = part[j][1] = part[j][2] = part[j][3] = 0.0f;
+          for (int y = 0; y < G; ++y)
 #pragma unroll
-          for (uint32_t f = 0; f < 4; ++f) {
-            const uint32_t e = e0 + f;
-            if (e >= hd / 8) break;
-            uint32_t ah[4], al[4];
-            split_tf32(qs[e * 8], ah[0], al[0]);
-            split_tf32(qs[e * 8 + 8 * (S::QPITCH / 4)], ah[1], al[1]);
-            split_tf32(qs[e * 8 + 4], ah[2], al[2]);
-            split_tf32(qs[e * 8 + 8 * (S::QPITCH / 4) + 4], ah[3], al[3]);
+            for (int j = 0; j < KW / 8; ++j) part[y][j][0] = part[y][j][1] = part[y][j][2] = part[y][j][3] = 0.0f;
 #pragma unroll
-            for (int j = 0; j < KW / 8; ++j) {
-              const unsigned char* kj = kf + (e0 / 4) * S::PANEL + j * 8 * 128;
-              uint32_t bh[2], bl[2];
-              split_tf32(*reinterpret_cast<const float*>(kj + (((2 * f) ^ g4) << 4)), bh[0], bl[0]);
-              split_tf32(*reinterpret_cast<const float*>(kj + (((2 * f + 1) ^ g4) << 4)), bh[1], bl[1]);
-              mma8(part[j], al, bh[0], bh[1]);
-              mma8(part[j], ah, bl[0], bl[1]);
-              mma8(part[j], ah, bh[0], bh[1]);
+          for (uint32_t f = 0; f < 4; ++f) {  // eight elements of each of the panels; zeros behind the head's end
+            uint32_t ah[G][4], al[G][4], bh[G][KW / 8][2], bl[G][KW / 8][2];
+#pragma unroll
+            for (int y = 0; y < G; ++y) {
+              const float* q = qs + (p0 + y) * 32 + f * 8;
+              split_tf32(q[0], ah[y][0], al[y][0]);
+              split_tf32(q[8 * (S::QPITCH / 4)], ah[y][1], al[y][1]);
+              split_tf32(q[4], ah[y][2], al[y][2]);
+              split_tf32(q[8 * (S::QPITCH / 4) + 4], ah[y][3], al[y][3]);
+#pragma unroll
+              for (int j = 0; j < KW / 8; ++j) {
+                const unsigned char* kj = kf + (p0 + y) * S::PANEL + j * 8 * 128;
+                split_tf32(*reinterpret_cast<const float*>(kj + (((2 * f) ^ g4) << 4)), bh[y][j][0], bl[y][j][0]);
+                split_tf32(*reinterpret_cast<const float*>(kj + (((2 * f + 1) ^ g4) << 4)), bh[y][j][1], bl[y][j][1]);
+              }
             }
+#pragma unroll
+            for (int z = 0; z < 3; ++z)  // the small products first
+#pragma unroll
+              for (int y = 0; y < G; ++y)
+#pragma unroll
+                for (int j = 0; j < KW / 8; ++j)
+                  mma8(part[y][j], z == 0 ? al[y] : ah[y], z == 1 ? bl[y][j][0] : bh[y][j][0], z == 1 ? bl[y][j][1] : bh[y][j][1]);
           }
 #pragma unroll
-          for (int j = 0; j < KW / 8; ++j)
+          for (int y = 0; y < G; ++y)
+            if (32 * (p0 + y) < hd) {
 #pragma unroll
-            for (int x = 0; x < 4; ++x) sc[j][x] += part[j][x];
+              for (int j = 0; j < KW / 8; ++j)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) sc[j][x] += part[y][j][x];
+            }
         }
       }
       // ---- softmax; row g4 in elements 0 and 1, row g4 + 8 in 2 and 3
@@ -446,22 +458,30 @@ __global__ void __launch_bounds__(kThreads, Shape<T, HP, WR>::ONE ? 1 : 2) rows_
           split_tf32(sc[j][3], ph[j][3], pl[j][3]);
         }
 #pragma unroll
-        for (int d = 0; d < HP / 8; ++d) {
-          if (d * 8 >= (int)hd) break;
-          const uint32_t ch = (d & 3) * 2 + (g4 >> 2);
-          float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int d0 = 0; d0 < HP / 8; d0 += 4) {  // a panel of 32 columns: four sums that do not wait for one another
+          if (d0 * 8 >= (int)hd) break;
+          float part[4][4];
+#pragma unroll
+          for (int y = 0; y < 4; ++y) part[y][0] = part[y][1] = part[y][2] = part[y][3] = 0.0f;
 #pragma unroll
           for (int j = 0; j < KW / 8; ++j) {
-            const unsigned char* vj = v0 + (d / 4) * S::PANEL + j * 8 * 128;
-            uint32_t bh[2], bl[2];
-            split_tf32(*reinterpret_cast<const float*>(vj + ((ch ^ (2 * t4)) << 4)), bh[0], bl[0]);
-            split_tf32(*reinterpret_cast<const float*>(vj + 128 + ((ch ^ (2 * t4 + 1)) << 4)), bh[1], bl[1]);
-            mma8(part, pl[j], bh[0], bh[1]);
-            mma8(part, ph[j], bl[0], bl[1]);
-            mma8(part, ph[j], bh[0], bh[1]);
+            const unsigned char* vj = v0 + (d0 / 4) * S::PANEL + j * 8 * 128;
+            uint32_t bh[4][2], bl[4][2];
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+              const uint32_t ch = 2 * y + (g4 >> 2);
+              split_tf32(*reinterpret_cast<const float*>(vj + ((ch ^ (2 * t4)) << 4)), bh[y][0], bl[y][0]);
+              split_tf32(*reinterpret_cast<const float*>(vj + 128 + ((ch ^ (2 * t4 + 1)) << 4)), bh[y][1], bl[y][1]);
+            }
+#pragma unroll
+            for (int z = 0; z < 3; ++z)
+#pragma unroll
+              for (int y = 0; y < 4; ++y) mma8(part[y], z == 0 ? pl[j] : ph[j], z == 1 ? bl[y][0] : bh[y][0], z == 1 ? bl[y][1] : bh[y][1]);
           }
 #pragma unroll
-          for (int x = 0; x < 4; ++x) o[d][x] += part[x];
+          for (int y = 0; y < 4; ++y)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) o[d0 + y][x] += part[y][x];
         }
       }
       __syncwarp();
