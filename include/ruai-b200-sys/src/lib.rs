@@ -194,6 +194,10 @@ extern "C" {
     pub fn ruai_model_cache_clear(m: *mut ruai_model) -> c_int;
     pub fn ruai_model_cache_len(m: *const ruai_model, len: *mut u32, capacity: *mut u32) -> c_int;
     pub fn ruai_model_generate(m: *mut ruai_model, prompt_host: *const i32, t: u32, n_new: u32, out_ids_host: *mut i32) -> c_int;
+    pub fn ruai_model_serve_start(m: *mut ruai_model, pages: u32, page: u32, requests: u32, request_pages: u32, dtype: c_int) -> c_int;
+    pub fn ruai_model_serve_stop(m: *mut ruai_model) -> c_int;
+    pub fn ruai_model_serve_free(m: *const ruai_model, free_pages: *mut u32) -> c_int;
+    pub fn ruai_model_serve_step(m: *mut ruai_model, fresh_host: *const i32, ids_host: *const i32, logits_host_or_null: *mut f32, next_ids_host_or_null: *mut i32) -> c_int;
     pub fn ruai_model_decode_step(m: *mut ruai_model, ids_dev_or_null: *const i32, b: u32, next_ids_host_or_null: *mut i32) -> c_int;
     pub fn ruai_model_cache_reserve(m: *mut ruai_model, b: u32, positions: u32) -> c_int;
     pub fn ruai_model_cache_assume(m: *mut ruai_model, b: u32, len: u32) -> c_int;

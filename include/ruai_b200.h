@@ -373,6 +373,21 @@ int ruai_model_generate_sampled(ruai_model* m, const int32_t* prompt_host, uint3
 int ruai_sample(ruai_ctx* ctx, const float* logits_dev, uint32_t vocab, float temperature, uint32_t top_k, float top_p,
                 uint64_t* rng_state, int32_t* token_host);
 
+/* Serving: up to `requests` requests of a Llama or GPT-2, of different lengths, that come and go, over a pool of `pages` pages of
+ * `page` positions per layer in f32, f16 or bf16 (see "a cache in pages"); a request holds up to request_pages of them.  Beside
+ * the model's own cache, which stays as it is.  A second start begins anew.  One GPU. */
+int ruai_model_serve_start(ruai_model* m, uint32_t pages, uint32_t page, uint32_t requests, uint32_t request_pages, int dtype);
+int ruai_model_serve_stop(ruai_model* m);
+int ruai_model_serve_free(const ruai_model* m, uint32_t* free_pages);
+/* One step: request r < requests goes on by fresh_host[r] tokens (0: it waits; negative: it has ended, and its pages are free
+ * from the next step on), whose ids lie side by side in ids_host in the order of the requests: whole prompts, parts of
+ * prompts and single tokens in one step.  logits_host_or_null receives [n, V] and next_ids_host_or_null [n] (greedy, the
+ * last maximum), for the n requests with new tokens, in their order, after the last of them.  What does not fit (pages, a
+ * request's pages, the model's positions) is refused before anything runs, and a step that fails leaves the requests as they
+ * were before it. */
+int ruai_model_serve_step(ruai_model* m, const int32_t* fresh_host, const int32_t* ids_host, float* logits_host_or_null,
+                          int32_t* next_ids_host_or_null);
+
 /* One decode step that never leaves the device: the ids are read from
  * ids_dev_or_null [B] (NULL: the argmax of the previous step), the argmax of
  * the new logits is left on the device and, if next_ids_host_or_null is given,

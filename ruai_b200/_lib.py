@@ -116,6 +116,10 @@ _PROTOS = {
     "ruai_model_cache_clear": (C.c_int, [vp]),
     "ruai_model_cache_len": (C.c_int, [vp, C.POINTER(u32), C.POINTER(u32)]),
     "ruai_model_generate": (C.c_int, [vp, vp, u32, u32, vp]),
+    "ruai_model_serve_start": (C.c_int, [vp, u32, u32, u32, u32, C.c_int]),
+    "ruai_model_serve_stop": (C.c_int, [vp]),
+    "ruai_model_serve_free": (C.c_int, [vp, C.POINTER(u32)]),
+    "ruai_model_serve_step": (C.c_int, [vp, vp, vp, vp, vp]),
     "ruai_model_decode_step": (C.c_int, [vp, vp, u32, vp]),
     "ruai_model_cache_assume": (C.c_int, [vp, u32, u32]),
     "ruai_model_cache_reserve": (C.c_int, [vp, u32, u32]),

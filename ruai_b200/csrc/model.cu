@@ -413,7 +413,9 @@ int ensure_cache(ruai_model* m, uint32_t B, uint32_t need) {
   return RUAI_OK;
 }
 
-int ensure_activations(ruai_model* m, uint32_t rows, uint32_t out_rows, uint32_t B, uint32_t T) {
+}  // namespace
+
+int model_activations(ruai_model* m, uint32_t rows, uint32_t out_rows, uint32_t B, uint32_t T) {
   ruai_ctx* c = m->ctx;
   if (m->hy) return hybrid_reserve(m, rows, out_rows, B, T);
   if (rows > m->act_rows) {
@@ -463,7 +465,7 @@ int ensure_activations(ruai_model* m, uint32_t rows, uint32_t out_rows, uint32_t
 
 // y = Linear(norm(x)) without a producer's sums of squares.  RMSNorm of more than 16 rows rides in the GEMM's pre-kernel, which
 // reads every row of x anyway (64 rows of 2048: 3.9 us a norm, 2000 of 4096: 21 us).
-int normed_linear(ruai_model* m, const ruai_qweight* w, const float* x, const float* nw, const float* nb, uint32_t rows, float* out, const GemvEpilogue& e) {
+int model_normed_linear(ruai_model* m, const ruai_qweight* w, const float* x, const float* nw, const float* nb, uint32_t rows, float* out, const GemvEpilogue& e) {
   ruai_ctx* c = m->ctx;
   float* xn = m->xn.as<float>();
   const bool dot = ruai_gemv_dot_takes(c, w, rows);
@@ -476,6 +478,8 @@ int normed_linear(ruai_model* m, const ruai_qweight* w, const float* x, const fl
   else RUAI_TRY(ruai_layer_norm(c, x, nw, nb, rows, m->d, 1e-5f, xn));
   return ruai_gemv_launch(c, w, xn, RUAI_F32, m->d, rows, out, e);
 }
+
+namespace {
 
 // Issues every kernel of one forward over rows = B*T new tokens whose ids are in d_ids and
 // whose first position is *d_len.  Logits for the last position of each sequence (or all
@@ -508,7 +512,7 @@ int issue_step(ruai_model* m, uint32_t B, uint32_t T, const HeadRows& head, bool
       pr.norm_w = Ly.n1w.as<float>(); pr.sumsq = ss; pr.tiles = ss_tiles; pr.eps = m->eps;
       RUAI_TRY(ruai_gemv_launch(c, Ly.qkv.w, x, RUAI_F32, d, rows, qkv, e, pr));
     } else {
-      RUAI_TRY(normed_linear(m, Ly.qkv.w, x, Ly.n1w.as<float>(), Ly.n1b.as<float>(), rows, qkv, e));
+      RUAI_TRY(model_normed_linear(m, Ly.qkv.w, x, Ly.n1w.as<float>(), Ly.n1b.as<float>(), rows, qkv, e));
     }
     const float2* table = m->llama ? m->rope_table.as<float2>() : nullptr;
     const bool fuse = T == 1;  // rotate + append inside the attention kernel
@@ -545,7 +549,7 @@ int issue_step(ruai_model* m, uint32_t B, uint32_t T, const HeadRows& head, bool
       pr.norm_w = Ly.n2w.as<float>(); pr.sumsq = ss; pr.tiles = ss_tiles; pr.eps = m->eps;
       RUAI_TRY(ruai_gemv_launch(c, Ly.up.w, x, RUAI_F32, d, rows, hb, eu, pr));
     } else {
-      RUAI_TRY(normed_linear(m, Ly.up.w, x, Ly.n2w.as<float>(), Ly.n2b.as<float>(), rows, hb, eu));
+      RUAI_TRY(model_normed_linear(m, Ly.up.w, x, Ly.n2w.as<float>(), Ly.n2b.as<float>(), rows, hb, eu));
     }
     GemvEpilogue ed;
     ed.bias = Ly.down.bias.as<float>();
@@ -583,7 +587,7 @@ int issue_step(ruai_model* m, uint32_t B, uint32_t T, const HeadRows& head, bool
     pr.norm_w = m->final_w.as<float>(); pr.sumsq = ss; pr.tiles = ss_tiles; pr.eps = m->eps;
     RUAI_TRY(ruai_gemv_launch(c, m->head.w, hx, RUAI_F32, d, out_rows, m->logits.as<float>(), eh, pr));
   } else {
-    RUAI_TRY(normed_linear(m, m->head.w, hx, m->final_w.as<float>(), m->final_b.as<float>(), out_rows, m->logits.as<float>(), eh));
+    RUAI_TRY(model_normed_linear(m, m->head.w, hx, m->final_w.as<float>(), m->final_b.as<float>(), out_rows, m->logits.as<float>(), eh));
   }
   if (!fused_pick) {
     RUAI_TRY(ruai_add_scalar(c, len, (int32_t)T));
@@ -597,9 +601,11 @@ int issue_step(ruai_model* m, uint32_t B, uint32_t T, const HeadRows& head, bool
 
 int pstep_reset(ruai_model* m);
 
+}  // namespace
+
 // Waits for the step; its error words and the first n token ids come back with it, through pinned memory, so that the host waits once:
 // a copy into pageable memory is a wait of its own.  (The model's own: models of one context may be stepped by several threads.)
-int read_back(ruai_model* m, int32_t* ids_host, uint32_t n) {
+int model_read_back(ruai_model* m, int32_t* ids_host, uint32_t n) {
   ruai_ctx* c = m->ctx;
   int32_t* h = m->pinned;  // the model's error word, the context's, the ids
   const bool staged = n + 2 <= kPinnedWords;
@@ -618,7 +624,9 @@ int read_back(ruai_model* m, int32_t* ids_host, uint32_t n) {
   if (e == 1) return model_fail(m, RUAI_ERR_ARG, "token id out of range [0, %u)", m->V);
   return model_fail(m, RUAI_ERR_TIMEOUT, "tensor-parallel exchange timed out waiting for a peer (status %d)", e);
 }
-int check_device_status(ruai_model* m) { return read_back(m, nullptr, 0); }
+namespace {
+
+int check_device_status(ruai_model* m) { return model_read_back(m, nullptr, 0); }
 
 // ---- the persistent decode step (pstep.cu) ---------------------------------------------------
 
@@ -743,7 +751,7 @@ int prepare_step(ruai_model* m, uint32_t B, uint32_t T, const HeadRows& head) {
   if (m->len + T > m->max_pos)
     return model_fail(m, RUAI_ERR_SHAPE, "context %u exceeds %s %u", m->len + T, m->hy ? "max_positions" : m->llama ? "max_position_embeddings" : "n_positions", m->max_pos);
   RUAI_TRY(ensure_cache(m, B, m->len + T));
-  RUAI_TRY(ensure_activations(m, B * T, head.count(B, T), B, T));
+  RUAI_TRY(model_activations(m, B * T, head.count(B, T), B, T));
   if (m->world > 1) RUAI_TRY(ruai_tp_check_ready(m->ctx, &m->tp, B * T, m->d));
   return RUAI_OK;
 }
@@ -852,6 +860,7 @@ RUAI_API int ruai_model_destroy(ruai_model* m) {
   m->d_rows.release();
   cudaFreeHost(m->pinned);
   hybrid_destroy(m);
+  serve_destroy(m);
   delete m;
   return RUAI_OK;
 }
@@ -1154,7 +1163,7 @@ RUAI_API int ruai_model_decode_step(ruai_model* m, const int32_t* ids_dev, uint3
     m->len_dirty = false;
   }
   RUAI_TRY(run_decode_graph(m, B));
-  return next_host ? read_back(m, next_host, B) : RUAI_OK;
+  return next_host ? model_read_back(m, next_host, B) : RUAI_OK;
 }
 
 // Times `iters` passes over every quantized Linear of the model (the weight-streaming
@@ -1164,7 +1173,7 @@ RUAI_API int ruai_model_time_linears(ruai_model* m, uint32_t B, uint32_t iters, 
   if (!m->quantized) return model_fail(m, RUAI_ERR_UNSUPPORTED, "the model is not quantized");
   ruai_ctx* c = m->ctx;
   DeviceGuard g(c->ordinal);
-  RUAI_TRY(ensure_activations(m, B, B, B, 1));
+  RUAI_TRY(model_activations(m, B, B, B, 1));
   if (m->hy) return hybrid_time_linears(m, B, iters, ms_total, launches, bytes_per_pass);
   float *xn = m->xn.as<float>(), *qkv = m->qkv.as<float>(), *att = m->att.as<float>(), *hb = m->hbuf.as<float>(), *xl = m->xl.as<float>();
   RUAI_CUDA(c, cudaMemsetAsync(xn, 0, (size_t)B * m->d * sizeof(float), c->stream));
@@ -1279,11 +1288,11 @@ static int generate_impl(ruai_model* m, const int32_t* prompt, uint32_t T, uint3
       m->len_dirty = false;
       RUAI_TRY(issue_step(m, 1, Tn, HeadRows(), true));
       m->len += Tn;
-      RUAI_TRY(read_back(m, &next, 1));
+      RUAI_TRY(model_read_back(m, &next, 1));
     }
     if (sampler) {  // the step left the argmax in d_ids; the sampled token replaces it there
       RUAI_TRY(ruai_sample_device(c, m->logits.as<float>(), m->V, sampler->temperature, sampler->top_k, sampler->top_p, &sampler->state, m->d_ids.as<int32_t>()));
-      RUAI_TRY(read_back(m, &next, 1));
+      RUAI_TRY(model_read_back(m, &next, 1));
     }
     on_device = true;
     ids.push_back(next);

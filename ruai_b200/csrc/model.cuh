@@ -62,6 +62,7 @@ struct PStep {
 };
 
 struct Hybrid;  // hybrid.cuh
+struct Serve;   // serve.cu
 
 struct ruai_model {
   ruai_ctx* ctx = nullptr;
@@ -94,6 +95,7 @@ struct ruai_model {
   bool len_dirty = true;  // the device copy of `len` may differ from the host's
   PStep ps;
   ruai_tp_state tp;
+  Serve* serve = nullptr;  // requests over a pool of pages
 };
 
 int model_fail(ruai_model* m, int code, const char* fmt, ...);
@@ -102,6 +104,14 @@ void drop_graph(ruai_model* m);
 int staged_get(ruai_model* m, uint64_t id, DevBuf** out);
 void staged_drop(ruai_model* m, uint64_t id);
 int stage_alloc(ruai_model* m, uint64_t id, size_t count, DevBuf** out);
+
+// The model's buffers for a step of `rows` tokens, out_rows of them with logits (B sequences of T; T 1: a decode step's scratch too).
+int model_activations(ruai_model* m, uint32_t rows, uint32_t out_rows, uint32_t B, uint32_t T);
+// y = Linear(norm(x)), RMSNorm or LayerNorm by the model.
+int model_normed_linear(ruai_model* m, const ruai_qweight* w, const float* x, const float* nw, const float* nb, uint32_t rows, float* out, const GemvEpilogue& e);
+// Waits for the step, its error words and the first n of d_ids.
+int model_read_back(ruai_model* m, int32_t* ids_host, uint32_t n);
+void serve_destroy(ruai_model* m);
 
 // Which rows of a step get logits: all B*T, the last of each sequence, or a list.
 struct HeadRows {

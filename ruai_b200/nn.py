@@ -500,6 +500,46 @@ class _Model:
                                                               float(top_p), int(seed), out.ctypes.data_as(C.c_void_p)))
         return out
 
+    def serve_start(self, pages, requests, page=16, request_pages=None, dtype=F32):
+        """Serve up to `requests` requests of different lengths over a pool of `pages` pages of `page` positions, kept in
+        `dtype` (F32, F16 or BF16).  A request holds request_pages pages at most (default: what the model's positions take)."""
+        if request_pages is None:
+            request_pages = max(1, min(pages, -(-self.max_positions // page)))
+        self.dev.check(self.dev.L.ruai_model_serve_start(self.h, pages, page, requests, request_pages, dtype))
+        self._requests = requests
+
+    def serve_step(self, new, ended=(), want_logits=True):
+        """One step of the requests in `new` ({request: its new token ids}); those in `ended` give their pages back.  Returns
+        (requests with new tokens in ascending order, logits [n, V] after the last of them or None, greedy next ids [n])."""
+        requests = getattr(self, "_requests", 0)
+        fresh = np.zeros(requests, np.int32)
+        order, ids = sorted(new), []
+        for r in order:
+            ids.append(np.ascontiguousarray(new[r], np.int32).reshape(-1))
+            if not 0 <= r < requests or not ids[-1].size:
+                raise ValueError(f"request {r} of {requests} with {ids[-1].size} new tokens")
+            fresh[r] = ids[-1].size
+        for r in ended:
+            if not 0 <= r < requests or fresh[r]:
+                raise ValueError(f"request {r} of {requests} cannot end in this step")
+            fresh[r] = -1
+        ids = np.concatenate(ids) if ids else np.zeros(0, np.int32)
+        logits = np.empty((len(order), self.vocab), np.float32) if want_logits else None
+        nxt = np.empty(len(order), np.int32)
+        self.dev.check(self.dev.L.ruai_model_serve_step(self.h, fresh.ctypes.data_as(C.c_void_p), ids.ctypes.data_as(C.c_void_p),
+                                                        logits.ctypes.data_as(C.c_void_p) if want_logits else None, nxt.ctypes.data_as(C.c_void_p)))
+        return order, logits, nxt
+
+    def serve_free(self):
+        """Free pages of the pool that the requests share."""
+        n = C.c_uint32()
+        self.dev.check(self.dev.L.ruai_model_serve_free(self.h, C.byref(n)))
+        return n.value
+
+    def serve_stop(self):
+        self.dev.check(self.dev.L.ruai_model_serve_stop(self.h))
+        self._requests = 0
+
     def decode_step(self, B, ids_dev=None, fetch=True):
         """One greedy step for B sequences that stays on the device; returns the next ids if fetch."""
         out = np.empty(B, np.int32) if fetch else None

@@ -1,0 +1,124 @@
+"""Llama and GPT-2 serving requests of different lengths over pages, against the same requests one by one over the model's own cache."""
+import numpy as np
+import pytest
+
+from ruai_b200 import nn
+
+pytestmark = pytest.mark.gpu
+
+# Pages in f32 differ from the model's own cache in the order of sums only: the project's tolerance on logits.  In 16 bits every key, value,
+# query and attention output is rounded to half a step (2^-11 or 2^-8) once in a layer; the logits of these two-layer models are sums of
+# hundreds of such terms, whose errors add up like their squares: a few half steps of the logits' scale.
+REL = {nn.F32: 1e-3, nn.F16: 8 * 2.0 ** -11, nn.BF16: 8 * 2.0 ** -8}
+
+
+@pytest.fixture(scope="module")
+def dev():
+    assert nn.Device.is_available(), "these tests need a CUDA device"
+    return nn.Device.cuda(0)
+
+
+def llama(dev, H=8, KV=2, hd=64, V=500, d=256, ff=512, L=2, bits=8, positions=512):
+    m = nn.Llama(dev, nn.LlamaConfig(V, d, ff, L, H, KV, hd, positions, 1e-5, 10000.0, 0))
+    m.load_synthetic(5, bits, 32)
+    return m
+
+
+def gpt2(dev, V=500, positions=400, d=256, L=2, H=4):
+    m = nn.GPT2(dev, nn.GPT2Config(V, positions, d, L, H))
+    m.load_synthetic(6, 8, 32)
+    return m
+
+
+MODELS = {"llama": llama, "llama int4 hd 128": lambda dev: llama(dev, H=4, KV=1, hd=128, bits=4), "llama hd 80": lambda dev: llama(dev, H=6, KV=3, hd=80), "gpt2": gpt2}
+
+
+def alone(m, ids):
+    """Logits after the last of a request's tokens, by the model's own cache."""
+    m.cache_clear()
+    return m.forward_cached(np.asarray(ids)[None])[0]
+
+
+@pytest.mark.parametrize("dtype", [nn.F32, nn.F16, nn.BF16])
+@pytest.mark.parametrize("name", MODELS)
+def test_steps_of_mixed_requests(dev, name, dtype):
+    """Prompts, parts of a prompt and single tokens in one step; requests end, and others take their pages."""
+    m = MODELS[name](dev)
+    rng = np.random.default_rng(1)
+    m.serve_start(40, 4, page=16, dtype=dtype)
+    said = {}
+    steps = [({0: 37, 2: 5}, ()), ({0: 1, 1: 130, 2: 1}, ()), ({0: 1, 2: 3, 3: 16}, ()), ({0: 20, 3: 1}, (1,)), ({1: 70, 3: 1}, (2,)), ({0: 1, 1: 1, 2: 1, 3: 1}, ())]
+    for new, ended in steps:
+        for r in ended:
+            said.pop(r)
+        ids = {r: rng.integers(0, 500, n) for r, n in new.items()}
+        order, logits, nxt = m.serve_step(ids, ended)
+        assert order == sorted(new)
+        for r in order:
+            said[r] = np.concatenate([said.get(r, np.zeros(0, np.int64)), ids[r]])
+        for i, r in enumerate(order):
+            want = alone(m, said[r])
+            assert np.abs(logits[i] - want).max() <= REL[dtype] * np.abs(want).max(), (r, np.abs(logits[i] - want).max(), np.abs(want).max())
+            assert logits[i][nxt[i]] == logits[i].max()
+    assert m.serve_free() == 40 - sum(-(-len(s) // 16) for s in said.values())
+    m.serve_step({}, ended=list(said))
+    assert m.serve_free() == 40
+    m.close()
+
+
+def test_greedy_serving_repeats_generate(dev):
+    m = llama(dev, positions=256)
+    rng = np.random.default_rng(2)
+    prompts = [rng.integers(0, 500, n) for n in (3, 40, 17)]
+    want = [m.generate(p, 12)[len(p):] for p in prompts]
+    m.cache_clear()
+    m.serve_start(24, 3, page=16)
+    _, _, nxt = m.serve_step(dict(enumerate(prompts)), want_logits=False)
+    got = [nxt]
+    for _ in range(11):
+        got.append(m.serve_step({r: [got[-1][r]] for r in range(3)}, want_logits=False)[2])
+    assert np.array_equal(np.array(got).T, np.array(want))
+    m.close()
+
+
+def test_refusals_leave_the_requests_as_they_were(dev):
+    m = llama(dev, positions=100)
+    with pytest.raises(nn.RuaiError, match="serve_start first"):
+        m._requests = 2
+        m.serve_step({0: [1]})
+    for args in (dict(pages=0, requests=1), dict(pages=4, requests=0), dict(pages=4, requests=1, page=24), dict(pages=4, requests=1, dtype=7), dict(pages=4, requests=9000)):
+        with pytest.raises(nn.RuaiError):
+            m.serve_start(**args)
+    m.serve_start(6, 3, page=16, request_pages=4)
+    ids = np.arange(30)
+    a = m.serve_step({0: ids})[1]
+    for new, text in (({0: np.arange(80)}, "max_position"), ({0: np.arange(36)}, "exceeds its 4 pages"), ({1: np.arange(50), 2: np.arange(20)}, "more pages")):
+        with pytest.raises(nn.RuaiError, match=text):
+            m.serve_step(new)
+    with pytest.raises(nn.RuaiError, match="token id out of range"):
+        m.serve_step({1: [3, 500]})
+    for new, ended in (({3: [1]}, ()), ({1: []}, ()), ({1: [1]}, (1,)), ({}, (5,))):
+        with pytest.raises(ValueError):
+            m.serve_step(new, ended)
+    assert m.serve_free() == 4
+    b = m.serve_step({0: [7], 1: ids})[1]
+    assert np.abs(b[1] - a[0]).max() <= 1e-3 * np.abs(a).max()
+    want = alone(m, np.concatenate([ids, [7]]))
+    assert np.abs(b[0] - want).max() <= 1e-3 * np.abs(want).max()
+    m.serve_stop()
+    with pytest.raises(nn.RuaiError, match="serve_start first"):
+        m._requests = 1
+        m.serve_step({0: [1]})
+    m.close()
+
+
+def test_layer_lists_do_not_serve(dev):
+    import zazasun_cases as zcases
+    cfg = zcases.config([zcases.attention()])
+    m = nn.Zazasun(dev, nn.ZazasunConfig(cfg, 0))
+    for name, t in zcases.weights(cfg).items():
+        m.set_tensor(name, t)
+    m.build("float32")
+    with pytest.raises(nn.RuaiError, match="serving over pages"):
+        m.serve_start(8, 1)
+    m.close()
