@@ -4,12 +4,14 @@
 // sums over the requests (new tokens, pages they need beyond those they hold, pages given back) say where everything lies: token t
 // belongs to the request whose range of the first sum holds it, the k-th page that is needed is the ring's (first + k)-th, and the
 // j-th that is given back goes behind the free ones.  Latency bounds it (two dependent loads, a scan, a search in shared memory), not
-// bytes: a cluster of up to eight CTAs works every sum out in each of them, so that nothing is exchanged, shares the tokens and pages, and
-// meets once before the pool's words are written, which all of them have read (they may be written in place).
+// bytes: every CTA works the sums out for itself, so that nothing is exchanged, and they share the tokens and pages, a token per thread.
+// Where the pool's words are written in place all CTAs must have read them before: they are one cluster then, of eight, and meet.
 //
 // append_kernel.  A CTA per token; a thread takes eight elements of a head, the two fours that rotate into each other where there is a
 // rotation: y_i = x_i cos - x_(i+h) sin, y_(i+h) = x_(i+h) cos + x_i sin, in f32, rounded once to the cache's type.  Bound by HBM: every
 // element is read and written once.
+#include <algorithm>
+
 #include "attn_paged.cuh"
 #include "pipeline.cuh"
 
@@ -20,7 +22,7 @@ struct PlanArgs {
   int32_t *table, *ring;
   const int32_t* words_in;
   int32_t *words_out, *starts, *positions, *slots;
-  uint32_t R, tokens, page_log2, table_ld, pages;
+  uint32_t R, tokens, page_log2, table_ld, pages, in_place;
   int* status;
 };
 
@@ -38,16 +40,17 @@ __device__ __forceinline__ uint32_t owner_of(const uint32_t* sums, uint32_t n, u
 constexpr uint32_t kPlanCluster = 8;
 
 __global__ void __launch_bounds__(1024) plan_kernel(const PlanArgs a) {
-  extern __shared__ uint32_t sums[];  // three exclusive sums over the requests, R + 1 each
+  extern __shared__ uint32_t sums[];  // three exclusive sums over the requests, R + 1 each, and their lengths
   __shared__ uint32_t part[3][32];
   const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, ld = a.R + 1, page = 1u << a.page_log2;
-  uint32_t *s_n = sums, *s_need = sums + ld, *s_back = sums + 2 * ld;
+  uint32_t *s_n = sums, *s_need = sums + ld, *s_back = sums + 2 * ld, *s_cached = sums + 3 * ld;
   grid_dependency_wait();
   grid_launch_dependents();
   const uint32_t first = (uint32_t)a.words_in[0], free = (uint32_t)a.words_in[1];
   const uint32_t per = (a.R + blockDim.x - 1) / blockDim.x, r0 = min(tid * per, a.R), r1 = min(r0 + per, a.R);
   uint32_t sum[3] = {0, 0, 0};
   bool bad = false;
+#pragma unroll 4
   for (uint32_t r = r0; r < r1; ++r) {
     const int32_t past = a.cached[r], f = a.fresh[r];
     uint32_t n = 0, need = 0, back = 0;
@@ -60,7 +63,7 @@ __global__ void __launch_bounds__(1024) plan_kernel(const PlanArgs a) {
       if (all > a.table_ld) bad = true;
       else need = all - held;
     }
-    s_n[r] = n; s_need[r] = need; s_back[r] = back;
+    s_n[r] = n; s_need[r] = need; s_back[r] = back; s_cached[r] = (uint32_t)past;
     sum[0] += n; sum[1] += need; sum[2] += back;
   }
   uint32_t inc[3];
@@ -103,7 +106,7 @@ __global__ void __launch_bounds__(1024) plan_kernel(const PlanArgs a) {
   for (uint32_t t = me; t < a.tokens; t += step) {
     int32_t pos = -1, slot = -1;
     if (ok && t < total[0]) {
-      const uint32_t r = owner_of(s_n, a.R, t), past = (uint32_t)a.cached[r], held = (past + page - 1) >> a.page_log2;
+      const uint32_t r = owner_of(s_n, a.R, t), past = s_cached[r], held = (past + page - 1) >> a.page_log2;
       const uint32_t p = past + t - s_n[r], i = p >> a.page_log2;
       const int32_t pg = i < held ? a.table[(size_t)r * a.table_ld + i] : a.ring[ring_at(s_need[r] + i - held)];
       pos = (int32_t)p;
@@ -115,7 +118,7 @@ __global__ void __launch_bounds__(1024) plan_kernel(const PlanArgs a) {
   }
   if (ok) {
     for (uint32_t k = me; k < total[1]; k += step) {
-      const uint32_t r = owner_of(s_need, a.R, k), held = ((uint32_t)a.cached[r] + page - 1) >> a.page_log2;
+      const uint32_t r = owner_of(s_need, a.R, k), held = (s_cached[r] + page - 1) >> a.page_log2;
       a.table[(size_t)r * a.table_ld + held + k - s_need[r]] = a.ring[ring_at(k)];
     }
     for (uint32_t k = me; k < total[2]; k += step) {
@@ -123,7 +126,7 @@ __global__ void __launch_bounds__(1024) plan_kernel(const PlanArgs a) {
       a.ring[ring_at(free + k)] = a.table[(size_t)r * a.table_ld + k - s_back[r]];
     }
   }
-  if (gridDim.x > 1) pipe::cluster_sync_all();  // every CTA has read the words
+  if (a.in_place && gridDim.x > 1) pipe::cluster_sync_all();  // every CTA has read the words
   else __syncthreads();
   if (me == 0) {
     a.words_out[0] = (int32_t)(ok ? ring_at(total[1]) : first);
@@ -245,20 +248,22 @@ RUAI_API int ruai_page_plan(ruai_ctx* c, const int32_t* cached, const int32_t* f
                             int32_t* positions, int32_t* slots) {
   if (!c || !cached || !fresh || !table || !ring || !words_in || !words_out || !starts || (tokens && (!positions || !slots)))
     return ruai_fail(c, RUAI_ERR_ARG, "ruai_page_plan: NULL argument");
-  PlanArgs a = {cached, fresh, table, ring, words_in, words_out, starts, positions, slots, R, tokens, 0, table_ld, pages, c->status};
+  PlanArgs a = {cached, fresh, table, ring, words_in, words_out, starts, positions, slots, R, tokens, 0, table_ld, pages, words_in == words_out ? 1u : 0u, c->status};
   if (!page_log2(page, &a.page_log2)) return ruai_fail(c, RUAI_ERR_SHAPE, "ruai_page_plan: pages of %u: a power of two from 16 to 256", page);
+  if (words_in != words_out && (const char*)words_in < (const char*)(words_out + 3) && (const char*)words_out < (const char*)(words_in + 3))
+    return ruai_fail(c, RUAI_ERR_ARG, "ruai_page_plan: words_out is words_in or lies apart from it");
   if (!R || R > kPlanRowsMax || tokens > kPlanTokensMax)
     return ruai_fail(c, RUAI_ERR_SHAPE, "ruai_page_plan: %u requests and %u tokens: 1 to %u and up to %u", R, tokens, kPlanRowsMax, kPlanTokensMax);
   if (!table_ld || table_ld > (1u << 18)) return ruai_fail(c, RUAI_ERR_SHAPE, "ruai_page_plan: rows of %u pages: 1 to %u", table_ld, 1u << 18);
   if (!pages || ((unsigned long long)pages << a.page_log2) >= (1ull << 31)) return ruai_fail(c, RUAI_ERR_SHAPE, "ruai_page_plan: a pool of %u pages of %u", pages, page);
   DeviceGuard g(c->ordinal);
   const uint32_t most = R > tokens ? R : tokens;
-  const dim3 block(most <= 256 ? 256 : 1024), grid(most <= 2048 ? 1 : kPlanCluster);
-  const size_t smem = 3 * (size_t)(R + 1) * sizeof(uint32_t);
+  const dim3 block(most <= 256 ? 256 : 1024), grid(most <= 1024 ? 1 : a.in_place ? kPlanCluster : std::min((most + 1023) / 1024, (uint32_t)c->sm_count));
+  const size_t smem = 4 * (size_t)(R + 1) * sizeof(uint32_t);
   if (smem > 48 * 1024) {
     static bool done[64] = {};
     if (!done[c->ordinal & 63]) {
-      RUAI_CUDA(c, cudaFuncSetAttribute(plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(3 * (kPlanRowsMax + 1) * sizeof(uint32_t))));
+      RUAI_CUDA(c, cudaFuncSetAttribute(plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(4 * (kPlanRowsMax + 1) * sizeof(uint32_t))));
       done[c->ordinal & 63] = true;
     }
   }
@@ -270,7 +275,7 @@ RUAI_API int ruai_page_plan(ruai_ctx* c, const int32_t* cached, const int32_t* f
     attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[n++].val.programmaticStreamSerializationAllowed = 1;
   }
-  if (grid.x > 1) {
+  if (a.in_place && grid.x > 1) {
     attr[n].id = cudaLaunchAttributeClusterDimension;
     attr[n].val.clusterDim.x = kPlanCluster; attr[n].val.clusterDim.y = 1; attr[n++].val.clusterDim.z = 1;
   }

@@ -248,14 +248,20 @@ class PagePlan(NamedTuple):
     words: Tensor      # int32 [3]: place of the first free page in the ring, free pages, missing pages
 
 
-def _ints(name, t, shape):
-    if t.np_dtype != np.int32 or t.shape != shape:
+_INT32 = np.dtype(np.int32)
+
+
+def _ints(dev, name, t, shape):
+    if t.shape != shape or t.np_dtype is not _INT32 and t.np_dtype != _INT32:
         raise ValueError(f"{name} must be int32 {list(shape)}, got {t.np_dtype} {list(t.shape)}")
+    if t.dev is not dev:
+        _same_device(dev, t)
 
 
 def _same_device(dev, *tensors):
-    if any(t is not None and t.dev.ordinal != dev.ordinal for t in tensors):
-        raise ValueError("tensors of different devices")
+    for t in tensors:
+        if t is not None and t.dev is not dev and t.dev.ordinal != dev.ordinal:
+            raise ValueError("tensors of different devices")
 
 
 def _pages(k, v):
@@ -268,20 +274,25 @@ def page_plan(cached, fresh, table, ring, words, page, tokens=None, out=None):
     """Block tables and slots of a step over a cache in pages (see `ruai_page_plan`): request r has cached[r] positions and
     brings fresh[r] new tokens, or has ended (negative).  `tokens` is the number of the step's rows, padding included."""
     dev = cached.dev
-    R, pages = cached.shape[0], ring.shape[0]
+    if len(table.shape) != 2 or len(ring.shape) != 1 or len(cached.shape) != 1:
+        raise ValueError("cached must be [requests], table [requests, pages] and ring [pages]")
+    R, pages, width = cached.shape[0], ring.shape[0], table.shape[1]
     if out is None:
         if tokens is None:
             raise ValueError("page_plan: the step's number of rows is needed where no buffers are given")
         out = PagePlan(Tensor(dev, (R + 1,), np.int32), Tensor(dev, (tokens,), np.int32), Tensor(dev, (tokens,), np.int32), Tensor(dev, (3,), np.int32))
-    tokens = out.slots.shape[0] if tokens is None else int(tokens)
-    if len(table.shape) != 2 or len(ring.shape) != 1:
-        raise ValueError("table must be [requests, pages] and ring [pages]")
-    for name, t, shape in (("cached", cached, (R,)), ("fresh", fresh, (R,)), ("table", table, (R, table.shape[1])), ("ring", ring, (pages,)), ("words", words, (3,)),
-                           ("starts", out.starts, (R + 1,)), ("positions", out.positions, (tokens,)), ("slots", out.slots, (tokens,)), ("words", out.words, (3,))):
-        _ints(name, t, shape)
-    _same_device(dev, fresh, table, ring, words, *out)
-    dev.check(dev.L.ruai_page_plan(dev.ctx, cached.ptr, fresh.ptr, R, tokens, page, table.ptr, table.shape[1], ring.ptr, pages, words.ptr, out.words.ptr, out.starts.ptr,
-                                   out.positions.ptr, out.slots.ptr))
+    starts, positions, slots, words_out = out
+    tokens = slots.shape[0] if tokens is None else int(tokens)
+    _ints(dev, "cached", cached, (R,))
+    _ints(dev, "fresh", fresh, (R,))
+    _ints(dev, "table", table, (R, width))
+    _ints(dev, "ring", ring, (pages,))
+    _ints(dev, "words", words, (3,))
+    _ints(dev, "starts", starts, (R + 1,))
+    _ints(dev, "positions", positions, (tokens,))
+    _ints(dev, "slots", slots, (tokens,))
+    _ints(dev, "words", words_out, (3,))
+    dev.check(dev.L.ruai_page_plan(dev.ctx, cached.ptr, fresh.ptr, R, tokens, page, table.ptr, width, ring.ptr, pages, words.ptr, words_out.ptr, starts.ptr, positions.ptr, slots.ptr))
     return out
 
 
@@ -292,19 +303,20 @@ def paged_append(qkv, positions, slots, k_pages, v_pages, rope=None, out=None):
     dev = qkv.dev
     if qkv.rdtype is None or len(qkv.shape) != 2 or qkv.shape[1] % dim or qkv.shape[1] // dim <= 2 * kv:
         raise ValueError(f"qkv must be a float tensor [tokens, (heads + {2 * kv}) * {dim}], got {list(qkv.shape)}")
-    tokens, heads = qkv.shape[0], qkv.shape[1] // dim - 2 * kv
-    _ints("positions", positions, (tokens,))
-    _ints("slots", slots, (tokens,))
+    tokens, width = qkv.shape
+    heads = width // dim - 2 * kv
+    _ints(dev, "positions", positions, (tokens,))
+    _ints(dev, "slots", slots, (tokens,))
     if rope is not None and (rope.rdtype != F32 or len(rope.shape) != 3 or rope.shape[2] != 2):
         raise ValueError("rope must be f32 [positions, rot / 2, 2]")
     if out is None:
         out = Tensor(dev, (tokens, heads, dim), k_pages.np_dtype, k_pages.rdtype)
     if out.rdtype != k_pages.rdtype or out.shape != (tokens, heads, dim):
         raise ValueError(f"out must be [{tokens}, {heads}, {dim}] of the pages' type")
-    _same_device(dev, positions, slots, k_pages, v_pages, rope, out)
-    dev.check(dev.L.ruai_paged_append(dev.ctx, qkv.rdtype, qkv.ptr, qkv.shape[1], heads * dim, (heads + kv) * dim, tokens, heads, 2 * rope.shape[1] if rope is not None else 0,
-                                      rope.ptr if rope is not None else None, rope.shape[0] if rope is not None else 0, positions.ptr, slots.ptr, k_pages.rdtype, k_pages.ptr,
-                                      v_pages.ptr, pages, kv, page, dim, out.ptr, heads * dim))
+    _same_device(dev, k_pages, v_pages, rope, out)
+    turns, most, half = (None, 0, 0) if rope is None else (rope.ptr, rope.shape[0], rope.shape[1])
+    dev.check(dev.L.ruai_paged_append(dev.ctx, qkv.rdtype, qkv.ptr, width, heads * dim, (heads + kv) * dim, tokens, heads, 2 * half, turns, most, positions.ptr, slots.ptr, k_pages.rdtype,
+                                      k_pages.ptr, v_pages.ptr, pages, kv, page, dim, out.ptr, heads * dim))
     return out
 
 
@@ -315,19 +327,20 @@ def paged_attention(q, k_pages, v_pages, table, cached, starts, most_fresh, most
     dev = q.dev
     if q.rdtype != k_pages.rdtype or len(q.shape) != 3 or q.shape[2] != dim:
         raise ValueError(f"q must be [tokens, heads, {dim}] of the pages' type, got {list(q.shape)}")
+    if len(table.shape) != 2 or len(cached.shape) != 1:
+        raise ValueError("cached must be [requests] and table [requests, pages]")
     tokens, heads, _ = q.shape
-    R = cached.shape[0]
-    if len(table.shape) != 2:
-        raise ValueError("table must be [requests, pages]")
-    for name, t, shape in (("table", table, (R, table.shape[1])), ("cached", cached, (R,)), ("starts", starts, (R + 1,))):
-        _ints(name, t, shape)
+    R, width = cached.shape[0], table.shape[1]
+    _ints(dev, "table", table, (R, width))
+    _ints(dev, "cached", cached, (R,))
+    _ints(dev, "starts", starts, (R + 1,))
     if out is None:
         out = Tensor(dev, q.shape, q.np_dtype, q.rdtype)
     if out.rdtype != q.rdtype or out.shape != q.shape:
         raise ValueError(f"out must be {list(q.shape)} of the pages' type")
-    _same_device(dev, k_pages, v_pages, table, cached, starts, out)
-    dev.check(dev.L.ruai_paged_attention(dev.ctx, q.rdtype, q.ptr, heads * dim, k_pages.ptr, v_pages.ptr, pages, kv, page, dim, table.ptr, table.shape[1], cached.ptr, starts.ptr, R,
-                                         tokens, heads, dim ** -0.5 if scale is None else float(scale), int(window), int(most_fresh), int(most_len), out.ptr, heads * dim))
+    _same_device(dev, k_pages, v_pages, out)
+    dev.check(dev.L.ruai_paged_attention(dev.ctx, q.rdtype, q.ptr, heads * dim, k_pages.ptr, v_pages.ptr, pages, kv, page, dim, table.ptr, width, cached.ptr, starts.ptr, R, tokens, heads,
+                                         dim ** -0.5 if scale is None else float(scale), int(window), int(most_fresh), int(most_len), out.ptr, heads * dim))
     return out
 
 

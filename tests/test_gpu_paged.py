@@ -414,7 +414,7 @@ def test_entry_points_check_their_arguments(dev):
     plan = dict(cached=p, fresh=p, R=1, tokens=1, page=16, table=p, ld=1, ring=p, pages=4, win=p, wout=p, starts=p, pos=p, slots=p)
     append = dict(xd=0, x=p, ld=48, k=16, v=32, tokens=1, H=1, rot=16, rope=p, most=4, pos=p, slots=p, d=0, kp=p, vp=p, pages=1, KV=1, page=16, hd=16, q=p, q_ld=16)
     attn = dict(d=0, q=p, q_ld=16, kp=p, vp=p, pages=1, KV=1, page=16, hd=16, table=p, ld=1, cached=p, starts=p, R=1, tokens=1, H=1, scale=1.0, window=0, fresh=1, len=1, out=p, out_ld=16)
-    for fn, base, changes in ((L.ruai_page_plan, plan, [dict(page=24), dict(page=8), dict(page=512), dict(R=0), dict(R=8193), dict(tokens=262145), dict(ld=0), dict(pages=0), dict(pages=1 << 28), dict(slots=None), dict(win=None)]),
+    for fn, base, changes in ((L.ruai_page_plan, plan, [dict(page=24), dict(page=8), dict(page=512), dict(R=0), dict(R=8193), dict(tokens=262145), dict(ld=0), dict(pages=0), dict(pages=1 << 28), dict(slots=None), dict(win=None), dict(wout=odd)]),
                               (L.ruai_paged_append, append, [dict(xd=3), dict(d=-1), dict(page=20), dict(hd=12), dict(hd=264), dict(hd=0), dict(KV=0), dict(pages=0), dict(pages=1 << 28), dict(rot=0), dict(rot=12),
                                                             dict(rot=24), dict(most=0), dict(ld=46), dict(ld=40), dict(k=18), dict(q_ld=12), dict(x=odd), dict(q=odd), dict(kp=odd), dict(rope=odd), dict(slots=None),
                                                             dict(pos=None)]),
