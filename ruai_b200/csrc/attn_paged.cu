@@ -547,11 +547,10 @@ __global__ void __launch_bounds__(kThreads, Shape<T, HP, WR>::ONE ? 1 : 2) rows_
         for (int j = 0; j < HP / 32; ++j)
           if (lane + 32 * j < hd) dst[lane + 32 * j] = from_f32<T>(l == 0.0f ? 0.0f : v[j] * inv);
       } else {
-        float* dst = part + row * (HP + 2);
+        float* dst = part + row * HP;
 #pragma unroll
-        for (int j = 0; j < HP / 32; ++j)
-          if (lane + 32 * j < hd) dst[lane + 32 * j] = v[j];
-        if (lane == 0) { dst[HP] = m; dst[HP + 1] = l; }
+        for (int j = 0; j < HP / 32; ++j) dst[lane + 32 * j] = v[j];
+        if (lane == 0) { part[RB * HP + row] = m; part[RB * HP + RB + row] = l; }
       }
     }
     if (cut) {
@@ -562,28 +561,52 @@ __global__ void __launch_bounds__(kThreads, Shape<T, HP, WR>::ONE ? 1 : 2) rows_
       gather();
       if (s_last) {
         __threadfence();
+        auto part_of = [&](uint32_t p) { return plan.parts + ((size_t)p * 2 + (p == first ? 1 : 0)) * (RB * (HP + 2)); };
+        constexpr int C = HP / 32 < 4 ? HP / 32 : 4, VECS = HP / 32 / C;  // columns of a load, loads of a row, per lane
         for (uint32_t row = warp; row < s.rows; row += kSoftWarps) {
-          auto part_of = [&](uint32_t p) { return plan.parts + ((size_t)p * 2 + (p == first ? 1 : 0)) * (RB * (HP + 2)) + row * (HP + 2); };
-          float m = -INFINITY;
-          for (uint32_t p = first + lane; p <= last; p += 32) m = fmaxf(m, __ldcg(part_of(p) + HP));
+          float m = -INFINITY, l = 0.0f, v[VECS][C];
 #pragma unroll
-          for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, off));
-          float l = 0.0f, v[HP / 32];
+          for (int x = 0; x < VECS; ++x)
 #pragma unroll
-          for (int j = 0; j < HP / 32; ++j) v[j] = 0.0f;
-#pragma unroll 4
-          for (uint32_t p = first; p <= last; ++p) {
-            const float* src = part_of(p);
-            const float mp = __ldcg(src + HP), lp = __ldcg(src + HP + 1), f = mp == -INFINITY ? 0.0f : exp2_of(mp - m);
-            l = fmaf(lp, f, l);
+            for (int y = 0; y < C; ++y) v[x][y] = 0.0f;
+          for (uint32_t p0 = first; p0 <= last; p0 += 32) {  // 32 parts' maxima and sums at a time, a lane each
+            const uint32_t np = min(32u, last + 1 - p0);
+            const float mp = lane < np ? __ldcg(part_of(p0 + lane) + RB * HP + row) : -INFINITY, lp = lane < np ? __ldcg(part_of(p0 + lane) + RB * HP + RB + row) : 0.0f;
+            float top = mp;
 #pragma unroll
-            for (int j = 0; j < HP / 32; ++j)
-              if (lane + 32 * j < hd) v[j] = fmaf(__ldcg(src + lane + 32 * j), f, v[j]);
+            for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, off));
+            const float m_new = fmaxf(m, top), corr = m == -INFINITY ? 0.0f : exp2_of(m - m_new), f = mp == -INFINITY ? 0.0f : exp2_of(mp - m_new);
+            float add = lp * f;
+#pragma unroll
+            for (int off = 16; off > 0; off >>= 1) add += __shfl_xor_sync(0xFFFFFFFFu, add, off);
+            l = fmaf(l, corr, add);
+            m = m_new;
+#pragma unroll
+            for (int x = 0; x < VECS; ++x)
+#pragma unroll
+              for (int y = 0; y < C; ++y) v[x][y] *= corr;
+#pragma unroll 8
+            for (uint32_t i = 0; i < np; ++i) {
+              const float fi = __shfl_sync(0xFFFFFFFFu, f, (int)i);
+              const float* src = part_of(p0 + i) + row * HP + lane * C;
+#pragma unroll
+              for (int x = 0; x < VECS; ++x) {
+                float w[C];
+                if constexpr (C == 4) *reinterpret_cast<float4*>(w) = __ldcg(reinterpret_cast<const float4*>(src + x * 128));
+                else *reinterpret_cast<float2*>(w) = __ldcg(reinterpret_cast<const float2*>(src));
+#pragma unroll
+                for (int y = 0; y < C; ++y) v[x][y] = fmaf(w[y], fi, v[x][y]);
+              }
+            }
           }
           T* dst = out_at(s.row0 + row);
 #pragma unroll
-          for (int j = 0; j < HP / 32; ++j)
-            if (lane + 32 * j < hd) dst[lane + 32 * j] = from_f32<T>(l == 0.0f ? 0.0f : v[j] / l);
+          for (int x = 0; x < VECS; ++x)
+#pragma unroll
+            for (int y = 0; y < C; ++y) {
+              const uint32_t e = x * 128 + lane * C + y;
+              if (e < hd) dst[e] = from_f32<T>(l == 0.0f ? 0.0f : v[x][y] / l);
+            }
         }
         if (tid == 0) plan.arrived[first] = 0;
       }

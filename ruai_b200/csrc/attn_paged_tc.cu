@@ -653,7 +653,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const PagedAttn a, c
 }
 
 // grid (CTAs of chunk_kernel, groups of 32 rows): the parts of an item, in their order.
-constexpr int kJoinThreads = 128;
+constexpr int kJoinThreads = 512;
 template <typename T>
 __global__ void __launch_bounds__(kJoinThreads) join_kernel(const PagedAttn a, const TcPlan plan) {
   grid_dependency_wait();
@@ -664,22 +664,36 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const PagedAttn a, c
   const uint32_t tile = row / kRows, mine = row % kRows / rep, token = tile * plan.tile_tokens + mine;
   if (mine >= plan.tile_tokens || token >= cut.tokens) return;
   auto part_of = [&](uint32_t i) { return plan.parts + ((size_t)i * 2 + (i == blockIdx.x ? 1 : 0)) * plan.part_floats; };
-  float m = -INFINITY, l = 0.0f;
-#pragma unroll 8
-  for (uint32_t i = blockIdx.x; i <= cut.last; ++i) m = fmaxf(m, part_of(i)[hd * kItemRows + row]);
-#pragma unroll 8
-  for (uint32_t i = blockIdx.x; i <= cut.last; ++i) {
-    const float mp = part_of(i)[hd * kItemRows + row];
-    l = fmaf(part_of(i)[(hd + 1) * kItemRows + row], mp == -INFINITY ? 0.0f : exp2_of(mp - m), l);
-  }
+  constexpr int kAhead = 4;  // parts whose loads are under way together
   T* dst = static_cast<T*>(a.out) + (size_t)(cut.token + token) * a.out_ld + (size_t)(cut.g * rep + row % kRows % rep) * hd;
-  for (uint32_t e = 4 * warp; e < hd; e += 16) {
-    float o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 8
-    for (uint32_t i = blockIdx.x; i <= cut.last; ++i) {
-      const float mp = part_of(i)[hd * kItemRows + row], f = mp == -INFINITY ? 0.0f : exp2_of(mp - m);
-      const float4 v = *reinterpret_cast<const float4*>(part_of(i) + ((size_t)(e / 4) * kItemRows + row) * 4);
-      o[0] = fmaf(v.x, f, o[0]); o[1] = fmaf(v.y, f, o[1]); o[2] = fmaf(v.z, f, o[2]); o[3] = fmaf(v.w, f, o[3]);
+  for (uint32_t e = 4 * warp; e < hd; e += kJoinThreads / 8) {
+    float m = -INFINITY, l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (uint32_t i0 = blockIdx.x; i0 <= cut.last; i0 += kAhead) {
+      float mp[kAhead], lp[kAhead], top = m;
+      float4 v[kAhead];
+#pragma unroll
+      for (int x = 0; x < kAhead; ++x) {
+        if (i0 + x > cut.last) { mp[x] = -INFINITY; continue; }
+        const float* part = part_of(i0 + x);
+        mp[x] = part[hd * kItemRows + row];
+        lp[x] = part[(hd + 1) * kItemRows + row];
+        v[x] = *reinterpret_cast<const float4*>(part + ((size_t)(e / 4) * kItemRows + row) * 4);
+      }
+#pragma unroll
+      for (int x = 0; x < kAhead; ++x) top = fmaxf(top, mp[x]);
+      const float corr = m == -INFINITY ? 0.0f : exp2_of(m - top);
+      l *= corr;
+#pragma unroll
+      for (int y = 0; y < 4; ++y) o[y] *= corr;
+      m = top;
+#pragma unroll
+      for (int x = 0; x < kAhead; ++x) {
+        if (mp[x] != -INFINITY) {
+          const float f = exp2_of(mp[x] - m);
+          l = fmaf(lp[x], f, l);
+          o[0] = fmaf(v[x].x, f, o[0]); o[1] = fmaf(v[x].y, f, o[1]); o[2] = fmaf(v[x].z, f, o[2]); o[3] = fmaf(v[x].w, f, o[3]);
+        }
+      }
     }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
     *reinterpret_cast<uint2*>(dst + e) = make_uint2(pack2<T>(o[0] * inv, o[1] * inv), pack2<T>(o[2] * inv, o[3] * inv));
