@@ -670,7 +670,7 @@ int ruai_paged_attention_launch(ruai_ctx* c, const PagedAttn& a) {
   uint32_t rows = a.most_fresh * (a.H / a.pool.KV), rows_most = 0xFFFFFFFFu;  // below 2^31: most_fresh is checked against the tokens
   if (rows > kRowsAlone) {
     const uint32_t rep = a.H / a.pool.KV, over = a.R > 1 && rep <= kRowsBeside ? kRowsBeside : 0u;
-    const int took = ruai_paged_attention_tc(c, a, over);
+    const int took = a.pool.dtype == RUAI_F32 ? ruai_paged_attention_pieces(c, a, over) : ruai_paged_attention_tc(c, a, over);
     if (took < 0) return RUAI_ERR_CUDA;
     if (took && !over) return RUAI_OK;
     if (took) rows = rows_most = over;

@@ -66,6 +66,8 @@ __device__ void row_again(const PagedAttn& a, const Segment& s, uint32_t rep, ui
 // attn_paged_tc.cu: the requests with more than `rows_over` rows (tokens x query heads of a key head) on the tensor cores, 256 rows at a
 // time.  1: launched; 0: this shape is not taken; < 0: error.
 int ruai_paged_attention_tc(ruai_ctx* c, const PagedAttn& a, uint32_t rows_over);
+// The same in f32, with operands as two fp16 pieces (attn_prefill_tc.cu).
+int ruai_paged_attention_pieces(ruai_ctx* c, const PagedAttn& a, uint32_t rows_over);
 
 typedef CUresult (*ruai_tensor_map_encode)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
                                            const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);

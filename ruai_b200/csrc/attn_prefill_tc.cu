@@ -16,6 +16,9 @@
 // attn_split_kernel writes the pieces of keys and values once, in the form the tensor core reads (K-major, 128-byte swizzle; values
 // transposed), so that a tile is one bulk copy for each of the query tiles that see it.
 //
+// PAGED: the same for requests of different lengths over pages (paged.cuh; b is a request, its keys and values come through its block table,
+// and it may see a window of them only).  A request with few rows is left to attn_paged.cu.
+//
 // attn_tc_kernel: a CTA owns 128 rows (queries x the query heads of a KV head).  One thread copies tiles, one issues
 // the MMAs (scores of tile t + 1 ahead of the values of tile t), and 4 CS warps are the softmax: thread = row and a CS-th of the
 // tile's keys, and of the output's columns.  Scores lie in tensor memory twice, probabilities (the A operand of the second product)
@@ -33,6 +36,7 @@
 // most 64 wide, else four: the registers that hold the output then leave room for the products' read-out.
 #include <algorithm>
 
+#include "attn_paged.cuh"
 #include "common.cuh"
 #include "decode_ops.cuh"
 #include "pipeline.cuh"
@@ -91,20 +95,42 @@ __device__ __forceinline__ uint32_t block_max(uint32_t v, uint32_t* red) {
 
 constexpr int kSplitThreads = 256;
 
+// Requests over pages, and the first tile that a request's rows see.
+struct Paged { PagedAttn a; uint32_t rows_over; };
+__device__ __forceinline__ bool paged_taken(const Paged& g, uint32_t r, uint32_t rep, PagedRequest& q) {
+  return paged_request(g.a, r, q) && q.fresh * rep > g.rows_over;
+}
+__device__ __forceinline__ uint32_t paged_tile0(const Paged& g, const PagedRequest& q, uint32_t first) { return paged_low(q.cached + first, g.a.window) / kKeys; }
+
 // grid (tiles, sequences * KV): 64 keys and their values.
-__global__ void __launch_bounds__(kSplitThreads) attn_split_kernel(const AttnParams p, const Pieces s) {
+template <bool PAGED>
+__global__ void __launch_bounds__(kSplitThreads) attn_split_kernel(const AttnParams p, const Pieces s, const Paged pg) {
   extern __shared__ float vs[];  // [64][hd + 1]
   __shared__ uint32_t red[kSplitThreads / 32];
   grid_dependency_wait();
   grid_launch_dependents();
-  const uint32_t tile = blockIdx.x, k0 = tile * kKeys, tid = threadIdx.x, n = (uint32_t)*p.len + p.T;
-  if (k0 >= n || n > p.cap) return;  // beyond the cache: the attention kernel reports it
-  const uint32_t nk = min((uint32_t)kKeys, n - k0), hd = p.hd;
+  const uint32_t tile = blockIdx.x, k0 = tile * kKeys, tid = threadIdx.x, hd = p.hd;
   const uint32_t b = s.b0 + blockIdx.y / p.KV, kvh = blockIdx.y % p.KV;
+  uint32_t n;
+  if constexpr (PAGED) {
+    PagedRequest rq;
+    if (!paged_taken(pg, b, s.rep, rq) || tile < paged_tile0(pg, rq, 0)) return;
+    n = rq.len;
+  } else {
+    n = (uint32_t)*p.len + p.T;
+  }
+  if (k0 >= n || n > p.cap) return;  // beyond the cache: the attention kernel reports it
+  const uint32_t nk = min((uint32_t)kKeys, n - k0);
   const size_t bk = (size_t)b * p.KV + kvh;
-  const float* kbase = p.kcache + bk * p.cap * hd;
-  const float* vbase = p.vcache + bk * p.cap * hd;
-  auto key4 = [&](uint32_t k, uint32_t e) { return *reinterpret_cast<const float4*>(kbase + (size_t)(k0 + k) * hd + e); };  // of key k0 + k
+  const float* kbase = p.kcache + (PAGED ? 0 : bk * p.cap * hd);
+  const float* vbase = p.vcache + (PAGED ? 0 : bk * p.cap * hd);
+  // where key k0 + k lies, in rows of hd; a page out of range: the pool's first row
+  auto row_of = [&](uint32_t k) -> size_t {
+    if constexpr (!PAGED) return k0 + k;
+    const int32_t page = paged_page(pg.a, b, k0 + k);
+    return page < 0 ? 0 : (((size_t)page * p.KV + kvh) << pg.a.pool.page_log2) + ((k0 + k) & ((1u << pg.a.pool.page_log2) - 1u));
+  };
+  auto key4 = [&](uint32_t k, uint32_t e) { return *reinterpret_cast<const float4*>(kbase + row_of(k) * hd + e); };  // of key k0 + k
   auto mag4 = [](const float4& v) { return max(max(magnitude(v.x), magnitude(v.y)), max(magnitude(v.z), magnitude(v.w))); };
   uint32_t km = 0, vm = 0;
   bool odd = false;
@@ -115,7 +141,7 @@ __global__ void __launch_bounds__(kSplitThreads) attn_split_kernel(const AttnPar
   }
   for (uint32_t i = tid; i < kKeys * (hd / 4); i += kSplitThreads) {
     const uint32_t k = i / (hd / 4), e = 4 * (i % (hd / 4));
-    const float4 v = k < nk ? *reinterpret_cast<const float4*>(vbase + (size_t)(k0 + k) * hd + e) : make_float4(0.f, 0.f, 0.f, 0.f);
+    const float4 v = k < nk ? *reinterpret_cast<const float4*>(vbase + row_of(k) * hd + e) : make_float4(0.f, 0.f, 0.f, 0.f);
     float* d = vs + k * (hd + 1) + e;
     d[0] = v.x; d[1] = v.y; d[2] = v.z; d[3] = v.w;
     vm = max(vm, mag4(v));
@@ -235,12 +261,29 @@ __device__ void rows_in_f32(const AttnParams& p, uint32_t b, uint32_t kvh, uint3
   }
 }
 
+// The same over pages.
+__device__ void rows_over_pages(const Paged& g, uint32_t b, uint32_t kvh, uint32_t rep, uint32_t q0, uint32_t nq, uint32_t first, uint32_t step) {
+  Segment sg = {};
+  paged_request(g.a, b, sg.rq);
+  sg.r = b;
+  sg.g = kvh;
+  const uint32_t lane = threadIdx.x & 31u, hd = g.a.pool.hd;
+  for (uint32_t r = first; r < nq * rep; r += step) {
+    const uint32_t row = q0 * rep + r;
+    float* dst = static_cast<float*>(g.a.out) + (size_t)(sg.rq.t0 + row / rep) * g.a.out_ld + (size_t)(kvh * rep + row % rep) * hd;
+    float m, l;
+    row_again<float>(g.a, sg, rep, row, 0, sg.rq.len, dst, m, l);
+    __syncwarp();
+    for (uint32_t e = lane; e < hd; e += 32) dst[e] = l == 0.0f ? 0.0f : dst[e] / l;
+  }
+}
+
 // Tensor memory: scores [2][64 columns], probabilities (hi 32 columns, lo 32), weighted values.
 constexpr uint32_t kProbCol = 2 * kKeys, kValueCol = kProbCol + kKeys;
 
 // CS: warps that share a row (keys of a tile, columns of the output).  OC: columns of the output per thread.
-template <int CS, int OC>
-__global__ void __launch_bounds__((kControl + 4 * CS) * 32, CS == 2 && OC == 32 ? 2 : 1) attn_tc_kernel(const AttnParams p, const Pieces s) {
+template <int CS, int OC, bool PAGED>
+__global__ void __launch_bounds__((kControl + 4 * CS) * 32, CS == 2 && OC == 32 ? 2 : 1) attn_tc_kernel(const AttnParams p, const Pieces s, const Paged pg) {
   constexpr int kSoftWarps = 4 * CS, SC = kKeys / CS;
   extern __shared__ unsigned char smem_raw[];
   __shared__ __align__(8) uint64_t q_ready, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], s_free[2], p_ready, o_full, fin;
@@ -256,6 +299,11 @@ __global__ void __launch_bounds__((kControl + 4 * CS) * 32, CS == 2 && OC == 32 
   const uint32_t bk = blockIdx.y, b = s.b0 + bk / p.KV, kvh = bk % p.KV;
   const uint32_t q0 = (gridDim.x - 1u - blockIdx.x) * qt;  // the tiles with the most keys first: they are the long ones
   const uint32_t head0 = kvh * rep;
+  PagedRequest rq;
+  if constexpr (PAGED) {  // nothing to do here for most CTAs of a mixed step: away before anything is set up
+    grid_dependency_wait();
+    if (!paged_taken(pg, b, rep, rq) || q0 >= rq.fresh) return;
+  }
 
   if (tid == 0) {
     mbar_init(&q_ready, kSoftWarps); mbar_init(&p_ready, kSoftWarps); mbar_init(&o_full, 1); mbar_init(&fin, 1);
@@ -274,20 +322,27 @@ __global__ void __launch_bounds__((kControl + 4 * CS) * 32, CS == 2 && OC == 32 
   const uint32_t tmem = s_tmem;
   grid_dependency_wait();
   grid_launch_dependents();
-  const uint32_t past = (uint32_t)*p.len, nq = min(qt, p.T - q0);
+  uint32_t past, T, t0, tile0 = 0;  // positions before the new tokens, their number, their first row; the first tile that any of the CTA's rows sees
+  if constexpr (PAGED) {
+    past = rq.cached; T = rq.fresh; t0 = rq.t0;
+    tile0 = paged_tile0(pg, rq, q0);
+  } else {
+    past = (uint32_t)*p.len; T = p.T; t0 = b * p.T;
+  }
+  const uint32_t nq = min(qt, T - q0);
   uint32_t kmax = past + q0 + nq;  // keys 0 .. kmax - 1 are seen by the tile's last query
-  const bool over = past + p.T > p.cap;  // the device's position is not the host's: touch nothing beyond the cache, tell the host
+  const bool over = past + T > p.cap;  // the device's position is not the host's: touch nothing beyond the cache, tell the host
   if (over) {
     kmax = 0;
     if (tid == 0 && p.status) atomicCAS(p.status, 0, 5);
   }
-  const uint32_t ntiles = (kmax + kKeys - 1) / kKeys;
+  const uint32_t ntiles = kmax ? (kmax + kKeys - 1) / kKeys - tile0 : 0u;
 
   if (warp < kControl) {
     if (warp == 0 && elect_one()) {
       // ===== copies =====
-      const unsigned char* kbase = s.k + (size_t)bk * s.tiles * k_slot;
-      const unsigned char* vbase = s.v + (size_t)bk * s.tiles * v_slot;
+      const unsigned char* kbase = s.k + ((size_t)bk * s.tiles + tile0) * k_slot;
+      const unsigned char* vbase = s.v + ((size_t)bk * s.tiles + tile0) * v_slot;
       // the keys of tile i, then the values of tile i - 1: keys are needed sooner and freed sooner
       uint32_t k = 0, v = 0;  // requested
       for (uint32_t i = 0; i <= ntiles && !s_abort && ntiles; ++i) {
@@ -362,7 +417,7 @@ __global__ void __launch_bounds__((kControl + 4 * CS) * 32, CS == 2 && OC == 32 
     for (uint32_t r = warp - kControl; r < (uint32_t)kRows; r += kSoftWarps) {
       const uint32_t qi = r / rep, h = r % rep;
       const bool in = r < qt * rep && qi < nq;
-      const float* src = p.q + (size_t)(b * p.T + q0 + qi) * p.q_ld + (size_t)(head0 + h) * hd;
+      const float* src = p.q + (size_t)(t0 + q0 + qi) * p.q_ld + (size_t)(head0 + h) * hd;
       float4 v[2];
       uint32_t mx = 0;
 #pragma unroll
@@ -396,6 +451,7 @@ __global__ void __launch_bounds__((kControl + 4 * CS) * 32, CS == 2 && OC == 32 
     const float qback = s_qback[row];
     const uint32_t qi = row / rep, h = row % rep;
     const uint32_t qpos = past + q0 + min(qi, nq - 1u);  // the last key this row's query sees (rows without a query: any)
+    const uint32_t qlow = PAGED ? paged_low(qpos, pg.a.window) : 0u;  // and the first
     const uint32_t lanes = (quarter * 32u) << 16;
     float m_run = -INFINITY, l_run = 0.0f, corr_prev = 0.0f, vf_prev = 0.0f;
     bool odd = false;  // a tile's factor was NaN: the same for the whole CTA
@@ -425,10 +481,10 @@ __global__ void __launch_bounds__((kControl + 4 * CS) * 32, CS == 2 && OC == 32 
         }
       }
     };
-    const float* factor = s.factor + (size_t)bk * s.tiles * 2;
+    const float* factor = s.factor + ((size_t)bk * s.tiles + tile0) * 2;
     float2 fac = ntiles ? *reinterpret_cast<const float2*>(factor) : make_float2(0.f, 0.f);
     for (uint32_t i = 0; i < ntiles; ++i) {
-      const uint32_t sb = i & 1u, key0 = i * kKeys + cp * SC;  // this thread's first key
+      const uint32_t sb = i & 1u, key0 = (tile0 + i) * kKeys + cp * SC;  // this thread's first key
       const float2 cur = fac;
       odd = odd || cur.x != cur.x;
       if (i + 1 < ntiles) fac = *reinterpret_cast<const float2*>(factor + 2 * (i + 1));
@@ -446,7 +502,8 @@ __global__ void __launch_bounds__((kControl + 4 * CS) * 32, CS == 2 && OC == 32 
       if (lane == 0) mbar_arrive(&s_free[sb]);
       // which of the keys the row sees: bit j = key0 + j <= qpos
       const uint32_t all = SC == 32 ? 0xFFFFFFFFu : (1u << (SC & 31)) - 1u;
-      const uint32_t seen = qpos < key0 ? 0u : qpos - key0 >= 31u ? all : ((2u << (qpos - key0)) - 1u) & all;
+      uint32_t seen = qpos < key0 ? 0u : qpos - key0 >= 31u ? all : ((2u << (qpos - key0)) - 1u) & all;
+      if (PAGED && qlow > key0) seen &= qlow - key0 >= 32u ? 0u : ~((1u << (qlow - key0)) - 1u);
       const bool whole = __all_sync(0xFFFFFFFFu, seen == all);
       if (!whole) {
 #pragma unroll
@@ -499,9 +556,13 @@ __global__ void __launch_bounds__((kControl + 4 * CS) * 32, CS == 2 && OC == 32 
 #pragma unroll
     for (int j = 0; j < OC; ++j) o[j] = __uint_as_float((uint32_t)(sums[j / 2] >> (32 * (j & 1))));
     if (odd) {
-      if (!over && !s_abort) rows_in_f32(p, b, kvh, rep, past, q0, nq, (uint32_t)(warp - kControl), kSoftWarps);
+      if constexpr (PAGED) {
+        if (!over && !s_abort) rows_over_pages(pg, b, kvh, rep, q0, nq, (uint32_t)(warp - kControl), kSoftWarps);
+      } else {
+        if (!over && !s_abort) rows_in_f32(p, b, kvh, rep, past, q0, nq, (uint32_t)(warp - kControl), kSoftWarps);
+      }
     } else if (!over && !s_abort && row < qt * rep && qi < nq) {
-      const size_t token = (size_t)b * p.T + q0 + qi;
+      const size_t token = (size_t)t0 + q0 + qi;
       const uint32_t c0 = cp * OC;
       const float inv = 1.0f / l;
       float* dst = p.out + token * p.out_ld + (size_t)(head0 + h) * hd;
@@ -516,15 +577,15 @@ __global__ void __launch_bounds__((kControl + 4 * CS) * 32, CS == 2 && OC == 32 
   if (warp == 1) tmem_dealloc(tmem, s.tmem);
 }
 
-template <int CS, int OC>
-cudaError_t launch_tc(ruai_ctx* c, const AttnParams& p, const Pieces& s, dim3 grid, uint32_t smem) {
+template <int CS, int OC, bool PAGED>
+cudaError_t launch_tc(ruai_ctx* c, const AttnParams& p, const Pieces& s, const Paged& pg, dim3 grid, uint32_t smem) {
   static bool done[64] = {};
   if (!done[c->ordinal & 63]) {
-    cudaError_t e = cudaFuncSetAttribute(attn_tc_kernel<CS, OC>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kSmemMax + 1024));
+    cudaError_t e = cudaFuncSetAttribute(attn_tc_kernel<CS, OC, PAGED>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kSmemMax + 1024));
     if (e != cudaSuccess) return e;
     done[c->ordinal & 63] = true;
   }
-  return ruai_launch(c, attn_tc_kernel<CS, OC>, grid, dim3((kControl + 4 * CS) * 32), smem, true, p, s);
+  return ruai_launch(c, attn_tc_kernel<CS, OC, PAGED>, grid, dim3((kControl + 4 * CS) * 32), smem, true, p, s, pg);
 }
 
 constexpr size_t kScratchMost = 256u << 20;  // a step's pieces at a time
@@ -533,12 +594,9 @@ constexpr size_t kScratchMost = 256u << 20;  // a step's pieces at a time
 // the 1.1B shape's 6 803 | 836, of GPT-2 1056 | 1126; 160 tokens 1080 | 1123, 833 | 937, 1105 | 1197, 1226 | 1410.
 constexpr uint32_t kFromTokens = 96;
 
-}  // namespace
-
-// 1: launched; 0: this shape is not taken; < 0: error.  `p`: as ruai_attention_prefill has completed it.
-int ruai_attention_prefill_tc(ruai_ctx* c, const AttnParams& p, uint32_t B, uint32_t rep) {
-  if (!c->use_tc || !p.pieces || p.T < kFromTokens || rep > 64) return 0;
-  if (p.maps != 1 || p.window || p.keep || p.vd != p.hd || p.vd_out != p.hd || p.out_dtype != RUAI_F32 || p.k_pos || p.sink || p.gate) return 0;
+// B sequences (PAGED: requests) whose new tokens are T at the most.
+template <bool PAGED>
+int launch_pieces(ruai_ctx* c, const AttnParams& p, const Paged& pg, uint32_t B, uint32_t rep) {
   Pieces s = {};
   s.rep = rep;
   s.blocks = (p.hd + 63) / 64;
@@ -573,17 +631,40 @@ int ruai_attention_prefill_tc(ruai_ctx* c, const AttnParams& p, uint32_t B, uint
   static bool done[64] = {};
   cudaError_t e = cudaSuccess;
   if (!done[c->ordinal & 63]) {
-    e = cudaFuncSetAttribute(attn_split_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kKeys * 257 * 4);
+    e = cudaFuncSetAttribute(attn_split_kernel<PAGED>, cudaFuncAttributeMaxDynamicSharedMemorySize, kKeys * 257 * 4);
     done[c->ordinal & 63] = e == cudaSuccess;
   }
   const uint32_t qt = kRows / rep;
   for (uint32_t b0 = 0; b0 < B && e == cudaSuccess; b0 += per) {
     const uint32_t nb = std::min(per, B - b0);
     s.b0 = b0;
-    e = ruai_launch(c, attn_split_kernel, dim3(s.tiles, nb * p.KV), dim3(kSplitThreads), (size_t)kKeys * (p.hd + 1) * 4, true, p, s);
+    e = ruai_launch(c, attn_split_kernel<PAGED>, dim3(s.tiles, nb * p.KV), dim3(kSplitThreads), (size_t)kKeys * (p.hd + 1) * 4, true, p, s, pg);
     const dim3 grid((p.T + qt - 1) / qt, nb * p.KV);
-    if (e == cudaSuccess) e = p.hd <= 64 ? launch_tc<2, 32>(c, p, s, grid, smem) : p.hd <= 128 ? launch_tc<4, 32>(c, p, s, grid, smem) : launch_tc<4, 64>(c, p, s, grid, smem);
+    if (e == cudaSuccess)
+      e = p.hd <= 64    ? launch_tc<2, 32, PAGED>(c, p, s, pg, grid, smem)
+          : p.hd <= 128 ? launch_tc<4, 32, PAGED>(c, p, s, pg, grid, smem)
+                        : launch_tc<4, 64, PAGED>(c, p, s, pg, grid, smem);
   }
   if (e != cudaSuccess) { ruai_fail(c, RUAI_ERR_CUDA, "prefill attention launch: %s", cudaGetErrorString(e)); return -1; }
   return 1;
+}
+
+}  // namespace
+
+// 1: launched; 0: this shape is not taken; < 0: error.  `p`: as ruai_attention_prefill has completed it.
+int ruai_attention_prefill_tc(ruai_ctx* c, const AttnParams& p, uint32_t B, uint32_t rep) {
+  if (!c->use_tc || !p.pieces || p.T < kFromTokens || rep > 64) return 0;
+  if (p.maps != 1 || p.window || p.keep || p.vd != p.hd || p.vd_out != p.hd || p.out_dtype != RUAI_F32 || p.k_pos || p.sink || p.gate) return 0;
+  return launch_pieces<false>(c, p, Paged(), B, rep);
+}
+
+int ruai_paged_attention_pieces(ruai_ctx* c, const PagedAttn& a, uint32_t rows_over) {
+  const uint32_t rep = a.H / a.pool.KV;
+  if (!c->use_tc || a.pool.dtype != RUAI_F32 || rep > 64 || a.pool.hd > 192 || !(a.scale > 0.0f)) return 0;  // (a row's largest score is that of its largest product)
+  AttnParams p = {};
+  p.q = static_cast<const float*>(a.q); p.q_ld = a.q_ld;
+  p.kcache = static_cast<float*>(a.pool.k); p.vcache = static_cast<float*>(a.pool.v);
+  p.T = a.most_fresh; p.KV = a.pool.KV; p.hd = a.pool.hd; p.cap = a.most_len; p.scale = a.scale;
+  p.out = static_cast<float*>(a.out); p.out_ld = a.out_ld; p.status = a.status;
+  return launch_pieces<true>(c, p, Paged{a, rows_over}, a.R, rep);
 }
