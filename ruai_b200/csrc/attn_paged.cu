@@ -75,18 +75,19 @@ constexpr int kSegments = 3;   // segments that the copying warp is ahead
 constexpr int kItemCost = 1;   // tiles that an item's queries and results take as long as
 constexpr int kTilesLeast = 3; // of a run, that cost included
 
-// HP: the head's width, up to 64, 128 or 256.  WR: warps that have rows of their own.
+// HP: the head's width, up to 64, 128 or 256.  WR: warps that have rows of their own, 16 each; 0: eight rows in all (f32).
 template <typename T, int HP, int WR>
 struct Shape {
-  static constexpr bool F32 = sizeof(T) == 4;
-  static constexpr int WK = 4 / WR, RB = 16 * WR, TK = !F32 ? 64 : HP == 256 && WR == 2 ? 16 : 32, KW = TK / WK;
+  static constexpr bool F32 = sizeof(T) == 4, NARROW = WR == 0;
+  static constexpr int WK = NARROW ? 4 : 4 / (NARROW ? 1 : WR), RW = NARROW ? 8 : 16, RB = RW * 4 / WK, TK = !F32 || NARROW ? 64 : HP == 256 && WR == 2 ? 16 : 32, KW = TK / WK;
+  static_assert(!NARROW || (F32 && HP <= 128), "eight rows: f32, heads of up to 128");
   static constexpr int PANEL_ELEMS = 128 / (int)sizeof(T), PANELS = HP / PANEL_ELEMS, PANEL = TK * 128;  // 128 bytes of every key of a tile
   static constexpr int HALF = PANELS * PANEL, STAGE = 2 * HALF;                                          // keys, values
-  static constexpr bool QSMEM = F32 || HP == 256;  // queries in shared memory, not in registers
+  static constexpr bool QSMEM = (F32 && !NARROW) || HP == 256;  // queries in shared memory, not in registers
   static constexpr int QPITCH = HP * (int)sizeof(T) + 16, QBYTES = QSMEM ? RB * QPITCH : 0;
-  static constexpr int MERGE = kSoftWarps * 16 * (HP + 4) * 4;  // the warps' results at the end, in the queries' place
+  static constexpr int MERGE = kSoftWarps * RW * (HP + 4) * 4;  // the warps' results at the end, in the queries' place
   static constexpr int KEPT = MERGE > QBYTES ? MERGE : QBYTES;
-  static constexpr bool ONE = HP == 256 || (HP == 128 && WR == 4);  // one CTA per SM: two have too few registers
+  static constexpr bool ONE = HP == 256 || (HP == 128 && (WR == 4 || NARROW));  // one CTA per SM: two have too few registers (eight rows: too little shared memory)
   static constexpr int ROOM = (ONE ? 216 : 108) * 1024 - KEPT, STAGES = ROOM / STAGE < 6 ? ROOM / STAGE : 6;
   static constexpr int SMEM = STAGES * STAGE + KEPT + 1024;
   static_assert(STAGES >= 2 && PANELS >= 1, "two stages at least");
@@ -114,7 +115,7 @@ struct Work {
 template <typename T, int HP, int WR>
 __global__ void __launch_bounds__(kThreads, Shape<T, HP, WR>::ONE ? 1 : 2) rows_kernel(const PagedAttn a, const RowsPlan plan, const __grid_constant__ Maps maps) {
   using S = Shape<T, HP, WR>;
-  constexpr int WK = S::WK, RB = S::RB, TK = S::TK, KW = S::KW, ST = S::STAGES;
+  constexpr int WK = S::WK, RB = S::RB, RW = S::RW, TK = S::TK, KW = S::KW, ST = S::STAGES, WRN = S::NARROW ? 1 : WR;
   extern __shared__ unsigned char smem_raw[];
   __shared__ __align__(8) uint64_t full[ST], empty[ST], work_full[kSegments], work_empty[kSegments], meet;
   __shared__ Work s_work[kSegments];
@@ -263,7 +264,7 @@ __global__ void __launch_bounds__(kThreads, Shape<T, HP, WR>::ONE ? 1 : 2) rows_
   }
 
   // ===== products and softmax
-  const uint32_t g4 = lane >> 2, t4 = lane & 3, wr = WR == 1 ? 0 : warp % WR, wk = warp / WR;
+  const uint32_t g4 = lane >> 2, t4 = lane & 3, wr = WRN == 1 ? 0 : warp % WRN, wk = warp / WRN;
   const float c = a.scale * kLog2e;
   uint32_t st = 0, meets = 0;
   auto gather = [&]() {  // the four warps meet
@@ -281,8 +282,16 @@ __global__ void __launch_bounds__(kThreads, Shape<T, HP, WR>::ONE ? 1 : 2) rows_
     // ---- queries
     const uint32_t row_lo = s.row0 + wr * 16 + g4, row_hi = row_lo + 8;
     auto q_at = [&](uint32_t row) { return static_cast<const T*>(a.q) + (size_t)(t0 + row / rep) * a.q_ld + (size_t)(s.g * rep + row % rep) * hd; };
-    uint32_t qf[S::QSMEM ? 1 : HP / 16][4];
-    if constexpr (S::QSMEM) {
+    uint32_t qf[S::QSMEM ? 1 : S::NARROW ? HP / 8 : HP / 16][4];
+    if constexpr (S::NARROW) {  // row g4: (hi, hi, lo, lo) of elements t4 and t4 + 4 of every eight
+      const float* q = g4 < s.rows ? reinterpret_cast<const float*>(q_at(s.row0 + g4)) + t4 : nullptr;
+#pragma unroll
+      for (int e = 0; e < HP / 8; ++e) {
+        const bool in = q && e * 8 < (int)hd;
+        split_tf32(in ? q[e * 8] : 0.0f, qf[e][0], qf[e][2]);
+        split_tf32(in ? q[e * 8 + 4] : 0.0f, qf[e][1], qf[e][3]);
+      }
+    } else if constexpr (S::QSMEM) {
       constexpr uint32_t kChunks = HP * sizeof(T) / 16;
       for (uint32_t x = tid; x < RB * kChunks; x += 32 * kSoftWarps) {
         const uint32_t row = x / kChunks, col = x % kChunks;
@@ -303,12 +312,14 @@ __global__ void __launch_bounds__(kThreads, Shape<T, HP, WR>::ONE ? 1 : 2) rows_
           qf[e][2 * h + 1] = q1 && col < hd ? *reinterpret_cast<const uint32_t*>(q1 + col) : 0u;
         }
     }
-    const uint32_t p_lo = cached + min(row_lo, row_end - 1) / rep, p_hi = cached + min(row_hi, row_end - 1) / rep;
+    // the positions of this thread's two rows: g4 and g4 + 8 of its warp's, or 2 t4 and 2 t4 + 1 of eight
+    const uint32_t p_lo = cached + min(S::NARROW ? s.row0 + 2 * t4 : row_lo, row_end - 1) / rep, p_hi = cached + min(S::NARROW ? s.row0 + 2 * t4 + 1 : row_hi, row_end - 1) / rep;
     const uint32_t l_lo = paged_low(p_lo, a.window), l_hi = paged_low(p_hi, a.window), whole0 = w.whole0, whole1 = w.whole1;
 
-    float o[HP / 8][4], m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
+    constexpr int OT = S::NARROW ? HP / 16 : HP / 8;  // tiles of the output: 16 rows x 8 columns, or 16 columns x 8 rows
+    float o[OT][4], m0 = -INFINITY, m1 = -INFINITY, l0 = 0.0f, l1 = 0.0f;
 #pragma unroll
-    for (int i = 0; i < HP / 8; ++i)
+    for (int i = 0; i < OT; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) o[i][j] = 0.0f;
 
@@ -326,6 +337,115 @@ __global__ void __launch_bounds__(kThreads, Shape<T, HP, WR>::ONE ? 1 : 2) rows_
         pipe::fence_proxy_async_smem();
         __syncwarp();
       }
+      if constexpr (S::NARROW) {
+        // S^T = K Q^T, 16 keys x 8 rows: key g4 (and g4 + 8) of rows 2 t4 and 2 t4 + 1; half the products of 16 rows with 8 of them empty
+        float sc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        const unsigned char* kf = ks + g4 * 128 + t4 * 4;
+#pragma unroll
+        for (int p0 = 0; p0 < S::PANELS; p0 += 2) {
+          if (p0 * 32 >= (int)hd) break;
+          float part[2][2][4];
+#pragma unroll
+          for (int y = 0; y < 2; ++y)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) part[y][0][x] = part[y][1][x] = 0.0f;
+#pragma unroll
+          for (int f = 0; f < 4; ++f) {
+            uint32_t ah[2][4], al[2][4];
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+              const unsigned char* kj = kf + (p0 + y) * S::PANEL;
+              const uint32_t c0 = ((2 * f) ^ g4) << 4, c1 = ((2 * f + 1) ^ g4) << 4;
+              split_tf32(*reinterpret_cast<const float*>(kj + c0), ah[y][0], al[y][0]);
+              split_tf32(*reinterpret_cast<const float*>(kj + 8 * 128 + c0), ah[y][1], al[y][1]);
+              split_tf32(*reinterpret_cast<const float*>(kj + c1), ah[y][2], al[y][2]);
+              split_tf32(*reinterpret_cast<const float*>(kj + 8 * 128 + c1), ah[y][3], al[y][3]);
+            }
+#pragma unroll
+            for (int z = 0; z < 3; ++z)
+#pragma unroll
+              for (int y = 0; y < 2; ++y) {
+                const uint32_t* q = qf[(p0 + y) * 4 + f];
+                mma8(part[y][z == 2], z == 0 ? al[y] : ah[y], z == 1 ? q[2] : q[0], z == 1 ? q[3] : q[1]);
+              }
+          }
+#pragma unroll
+          for (int y = 0; y < 2; ++y)
+            if ((p0 + y) * 32 < (int)hd) {  // a panel behind the head's end may hold anything
+#pragma unroll
+              for (int x = 0; x < 4; ++x) sc[x] += part[y][0][x] + part[y][1][x];
+            }
+        }
+        const bool whole = key0 >= whole0 && key0 + KW <= whole1;
+        float x0 = -INFINITY, x1 = -INFINITY;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const uint32_t key = key0 + g4 + (x & 2) * 4;
+          sc[x] = whole || (key <= (x & 1 ? p_hi : p_lo) && key >= (x & 1 ? l_hi : l_lo)) ? sc[x] * c : -INFINITY;
+          if (x & 1) x1 = fmaxf(x1, sc[x]);
+          else x0 = fmaxf(x0, sc[x]);
+        }
+#pragma unroll
+        for (int off = 4; off < 32; off <<= 1) {
+          x0 = fmaxf(x0, __shfl_xor_sync(0xFFFFFFFFu, x0, off));
+          x1 = fmaxf(x1, __shfl_xor_sync(0xFFFFFFFFu, x1, off));
+        }
+        const float n0 = fmaxf(m0, x0), n1 = fmaxf(m1, x1);
+        if (__any_sync(0xFFFFFFFFu, n0 > m0 || n1 > m1)) {
+          const float c0 = m0 == -INFINITY ? 0.0f : exp2_of(m0 - n0), c1 = m1 == -INFINITY ? 0.0f : exp2_of(m1 - n1);
+          l0 *= c0;
+          l1 *= c1;
+#pragma unroll
+          for (int d = 0; d < OT; ++d) { o[d][0] *= c0; o[d][1] *= c1; o[d][2] *= c0; o[d][3] *= c1; }
+          m0 = n0;
+          m1 = n1;
+        }
+        const float b0 = m0 == -INFINITY ? 0.0f : m0, b1 = m1 == -INFINITY ? 0.0f : m1;
+        sc[0] = exp2_of(sc[0] - b0); sc[1] = exp2_of(sc[1] - b1);
+        sc[2] = exp2_of(sc[2] - b0); sc[3] = exp2_of(sc[3] - b1);
+        l0 += sc[0] + sc[2];
+        l1 += sc[1] + sc[3];
+        // O^T += V^T P^T, 16 columns x 8 rows; the product's k is key 2 t4 for t4, 2 t4 + 1 for t4 + 4
+        uint32_t ph[2][2], pl[2][2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            const int from = (int)((2 * t4 + y) * 4 + (g4 >> 1));
+            const float even = __shfl_sync(0xFFFFFFFFu, sc[2 * h], from), odd = __shfl_sync(0xFFFFFFFFu, sc[2 * h + 1], from);
+            split_tf32(g4 & 1 ? odd : even, ph[h][y], pl[h][y]);
+          }
+        const unsigned char* v0 = vs + 2 * t4 * 128 + (g4 & 3) * 4;
+#pragma unroll
+        for (int d0 = 0; d0 < OT; d0 += 2) {
+          if (d0 * 16 >= (int)hd) break;
+          float part[2][2][4];
+#pragma unroll
+          for (int y = 0; y < 2; ++y)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) part[y][0][x] = part[y][1][x] = 0.0f;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const unsigned char* vj = v0 + (d0 / 2) * S::PANEL + h * 8 * 128;
+            uint32_t ah[2][4], al[2][4];
+#pragma unroll
+            for (int y = 0; y < 2; ++y)
+#pragma unroll
+              for (int x = 0; x < 4; ++x) {  // columns g4 and g4 + 8, keys 2 t4 and 2 t4 + 1
+                const uint32_t ch = 4 * y + (g4 >> 2) + (x & 1) * 2, key = 2 * t4 + (x >> 1);
+                split_tf32(*reinterpret_cast<const float*>(vj + (x >> 1) * 128 + ((ch ^ key) << 4)), ah[y][x], al[y][x]);
+              }
+#pragma unroll
+            for (int z = 0; z < 3; ++z)
+#pragma unroll
+              for (int y = 0; y < 2; ++y) mma8(part[y][z == 2], z == 0 ? al[y] : ah[y], z == 1 ? pl[h][0] : ph[h][0], z == 1 ? pl[h][1] : ph[h][1]);
+          }
+#pragma unroll
+          for (int y = 0; y < 2; ++y)
+#pragma unroll
+            for (int x = 0; x < 4; ++x) o[d0 + y][x] += part[y][0][x] + part[y][1][x];
+        }
+      } else {
       float sc[KW / 8][4];
 #pragma unroll
       for (int j = 0; j < KW / 8; ++j) sc[j][0] = sc[j][1] = sc[j][2] = sc[j][3] = 0.0f;
@@ -484,18 +604,28 @@ __global__ void __launch_bounds__(kThreads, Shape<T, HP, WR>::ONE ? 1 : 2) rows_
             for (int x = 0; x < 4; ++x) o[d0 + y][x] += part[y][x];
         }
       }
+      }
       __syncwarp();
       if (lane == 0) pipe::mbar_arrive(&empty[slot]);
     }
 
     // ---- the warps' results meet
 #pragma unroll
-    for (int off = 1; off < 4; off <<= 1) {
+    for (int off = S::NARROW ? 4 : 1; off < (S::NARROW ? 32 : 4); off <<= 1) {
       l0 += __shfl_xor_sync(0xFFFFFFFFu, l0, off);
       l1 += __shfl_xor_sync(0xFFFFFFFFu, l1, off);
     }
     if constexpr (S::QSMEM) gather();  // the queries have been read
-    {
+    if constexpr (S::NARROW) {
+      float* d0 = res + (warp * 8 + 2 * t4) * (HP + 4) + g4;
+#pragma unroll
+      for (int d = 0; d < OT; ++d) {
+        if (d * 16 >= (int)hd) break;
+        d0[d * 16] = o[d][0]; d0[HP + 4 + d * 16] = o[d][1];
+        d0[d * 16 + 8] = o[d][2]; d0[HP + 4 + d * 16 + 8] = o[d][3];
+      }
+      if (g4 == 0) { s_m[warp][2 * t4] = m0; s_l[warp][2 * t4] = l0; s_m[warp][2 * t4 + 1] = m1; s_l[warp][2 * t4 + 1] = l1; }
+    } else {
       float* d0 = res + (warp * 16 + g4) * (HP + 4) + 2 * t4;
       float* d1 = d0 + 8 * (HP + 4);
 #pragma unroll
@@ -512,15 +642,15 @@ __global__ void __launch_bounds__(kThreads, Shape<T, HP, WR>::ONE ? 1 : 2) rows_
     auto out_at = [&](uint32_t row) { return static_cast<T*>(a.out) + (size_t)(t0 + row / rep) * a.out_ld + (size_t)(s.g * rep + row % rep) * hd; };
     // a warp per row
     for (uint32_t row = warp; row < s.rows; row += kSoftWarps) {
-      const uint32_t w0 = row / 16, rr = row % 16;  // the row's warps are w0, w0 + WR, ...
+      const uint32_t w0 = row / RW, rr = row % RW;  // the row's warps are w0, w0 + WR, ...
       float m = -INFINITY, l = 0.0f, f[WK], v[HP / 32];
 #pragma unroll
-      for (int x = 0; x < WK; ++x) m = fmaxf(m, s_m[w0 + x * WR][rr]);
+      for (int x = 0; x < WK; ++x) m = fmaxf(m, s_m[w0 + x * WRN][rr]);
 #pragma unroll
       for (int x = 0; x < WK; ++x) {
-        const float mw = s_m[w0 + x * WR][rr];
+        const float mw = s_m[w0 + x * WRN][rr];
         f[x] = mw == -INFINITY ? 0.0f : exp2_of(mw - m);
-        l = fmaf(s_l[w0 + x * WR][rr], f[x], l);
+        l = fmaf(s_l[w0 + x * WRN][rr], f[x], l);
       }
       bool fine = isfinite(l);
 #pragma unroll
@@ -529,12 +659,12 @@ __global__ void __launch_bounds__(kThreads, Shape<T, HP, WR>::ONE ? 1 : 2) rows_
         v[j] = 0.0f;
         if (e < hd) {
 #pragma unroll
-          for (int x = 0; x < WK; ++x) v[j] = fmaf(res[((w0 + x * WR) * 16 + rr) * (HP + 4) + e], f[x], v[j]);
+          for (int x = 0; x < WK; ++x) v[j] = fmaf(res[((w0 + x * WRN) * RW + rr) * (HP + 4) + e], f[x], v[j]);
           fine = fine && isfinite(v[j]);
         }
       }
       if (!__all_sync(0xFFFFFFFFu, fine)) {
-        float* again = res + (w0 * 16 + rr) * (HP + 4);
+        float* again = res + (w0 * RW + rr) * (HP + 4);
         row_again<T>(a, s, rep, s.row0 + row, s.tile0 * TK, s.tile1 * TK, again, m, l);
         __syncwarp();
 #pragma unroll
@@ -649,6 +779,9 @@ int launch_rows(ruai_ctx* c, const PagedAttn& a, uint32_t rows_most) {
 
 template <typename T, int HP>
 int launch_width(ruai_ctx* c, const PagedAttn& a, uint32_t rows, uint32_t rows_most) {
+  if constexpr (sizeof(T) == 4 && HP <= 128) {
+    if (rows <= 8) return launch_rows<T, HP, 0>(c, a, rows_most);
+  }
   if (rows <= 16) return launch_rows<T, HP, 1>(c, a, rows_most);
   if (rows <= 32 || HP == 256) return launch_rows<T, HP, 2>(c, a, rows_most);
   return launch_rows<T, HP == 256 ? 128 : HP, 4>(c, a, rows_most);
