@@ -18,6 +18,7 @@
 #include <cuda.h>
 
 #include <algorithm>
+#include <cmath>
 
 #include "attn_paged.cuh"
 #include "pipeline.cuh"
@@ -794,14 +795,26 @@ int launch_type(ruai_ctx* c, const PagedAttn& a, uint32_t rows, uint32_t rows_mo
                             : launch_width<T, 256>(c, a, rows, rows_most);
 }
 
-// A step whose requests have no more than this many rows stays on the kernel here; else it keeps those of kRowsBeside at the most.
-constexpr uint32_t kRowsAlone = 64, kRowsBeside = 16;
+// A step whose requests all have few rows stays on the kernel here; else it keeps those of up to kRowsBeside rows.
+constexpr uint32_t kRowsBeside = 16;
+// f16 and bf16: up to 24 rows.  us, here | attn_paged_tc.cu, heads of 128, 8 of keys: 20 rows of 4 requests of 1000 28 | 24, of 32 47 | 47, 24 rows (heads of
+// 64) of 64 requests of 200 12 | 23; 32 rows of 8 requests of 4000 60 | 44, of 64 of 200 44 | 35, of one of 8000 55 | 26; 64 rows of 8 of 4000 110 | 43.
+constexpr uint32_t kRowsAlone = 24;
+// f32: from 33 rows on whichever is the shorter by the times of both, which go by the pairs of a row and a key here, and there by the splitting
+// of all keys and the longest row of key tiles, which one CTA walks.  us, here | attn_prefill_tc.cu (the same heads): 64 rows of 8 requests of 4000 269 |
+// 245, of 64 of 200 185 | 138, of one of 8000 114 | 263; 48 rows of 32 requests of 1000 271 | 262; 32 rows of 32 requests of 1000 (heads of 64) 58 | 75.
+bool in_pieces(const PagedAttn& a, uint32_t rows) {
+  if (rows <= 32) return false;
+  const double len = a.most_len, rep = a.H / a.pool.KV, items = a.pool.KV * ceil(a.tokens * rep / 128.0);
+  const double here = a.tokens * (double)a.H * len / 36e3, split = a.R * len * a.pool.KV * a.pool.hd * 16.0 / 3e6, there = split + 15.0 + 2.0 * ceil(len / 64.0) * ceil(items / 148.0);
+  return there < here;
+}
 
 }  // namespace
 
 int ruai_paged_attention_launch(ruai_ctx* c, const PagedAttn& a) {
   uint32_t rows = a.most_fresh * (a.H / a.pool.KV), rows_most = 0xFFFFFFFFu;  // below 2^31: most_fresh is checked against the tokens
-  if (rows > kRowsAlone) {
+  if (a.pool.dtype == RUAI_F32 ? in_pieces(a, rows) : rows > kRowsAlone) {
     const uint32_t rep = a.H / a.pool.KV, over = a.R > 1 && rep <= kRowsBeside ? kRowsBeside : 0u;
     const int took = a.pool.dtype == RUAI_F32 ? ruai_paged_attention_pieces(c, a, over) : ruai_paged_attention_tc(c, a, over);
     if (took < 0) return RUAI_ERR_CUDA;
