@@ -74,7 +74,7 @@ __device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap* map, int
 constexpr int kSoftWarps = 4, kThreads = 32 * (kSoftWarps + 1);
 constexpr int kSegments = 3;   // segments that the copying warp is ahead
 constexpr int kItemCost = 1;   // tiles that an item's queries and results take as long as
-constexpr int kTilesLeast = 3; // of a run, that cost included
+constexpr int kTilesLeast = 3; // of a run, that cost included (three for one warp's rows, more for more: parts are as large as the rows are many)
 
 // HP: the head's width, up to 64, 128 or 256.  WR: warps that have rows of their own, 16 each; 0: eight rows in all (f32).
 template <typename T, int HP, int WR>
@@ -166,7 +166,7 @@ __global__ void __launch_bounds__(kThreads, Shape<T, HP, WR>::ONE ? 1 : 2) rows_
     if (w < warp) before += s_part[w];
     total += s_part[w];
   }
-  const unsigned long long per = max((total + gridDim.x - 1) / gridDim.x, (unsigned long long)kTilesLeast);
+  const unsigned long long per = max((total + gridDim.x - 1) / gridDim.x, (unsigned long long)(kTilesLeast + 2 * (WRN - 1)));
   const unsigned long long u0 = per * blockIdx.x, u1 = min(u0 + per, total);
   if (u0 >= u1) return;
   if (before <= u0 && u0 < before + mine) {
@@ -806,7 +806,8 @@ constexpr uint32_t kRowsAlone = 24;
 bool in_pieces(const PagedAttn& a, uint32_t rows) {
   if (rows <= 32) return false;
   const double len = a.most_len, rep = a.H / a.pool.KV, items = a.pool.KV * ceil(a.tokens * rep / 128.0);
-  const double here = a.tokens * (double)a.H * len / 36e3, split = a.R * len * a.pool.KV * a.pool.hd * 16.0 / 3e6, there = split + 15.0 + 2.0 * ceil(len / 64.0) * ceil(items / 148.0);
+  const double many = ceil((double)(a.tokens > a.R ? a.tokens - a.R : 0) / (a.most_fresh > 1 ? a.most_fresh - 1 : 1));  // requests with as many rows as the most
+  const double here = 10.0 + a.tokens * (double)a.H * len / 36e3, split = std::min(many, (double)a.R) * len * a.pool.KV * a.pool.hd * 16.0 / 3e6, there = split + 15.0 + 2.0 * ceil(len / 64.0) * ceil(items / 148.0);
   return there < here;
 }
 

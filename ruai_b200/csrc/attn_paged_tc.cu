@@ -8,7 +8,8 @@
 // probabilities (written over the scores, rounded once to the values' type) and outputs stay in tensor memory: 2 x (128 + 128)
 // columns.  Outputs are rescaled only where a row's maximum has grown by more than 2^8 since the last time: weights of up to 256 are as exact
 // as those of up to 1, and nearly every tile leaves the outputs where they are.
-//   Split: the key tiles of all items, in a row, in equal runs, one per CTA.  An item cut by a run's end leaves (m, l, o) of its parts in
+//   Split: the key tiles of all items, in a row, in equal runs, one per CTA, their ends moved to an item's edge where one is near (four
+// prompts of 2000: 175 -> 158 us; one of 2000: 74 -> 64; one of 500 after 8192: 85 -> 78).  An item cut by a run's end leaves (m, l, o) of its parts in
 // scratch, and join_kernel adds them up, many CTAs to an item (the last CTA to arrive alone took 90 us for 17 parts).
 //   Values of the positions behind a request's end are cleared in shared memory (0 x NaN), and a row that is not finite at the end is worked
 // out again key by key.  Every mbarrier wait is bounded.
@@ -28,7 +29,8 @@ constexpr int kThreads = 384;
 constexpr uint32_t kOutCol = 256;  // tensor memory: scores of both tiles, then their outputs
 constexpr float kGrowth = 8.0f;
 constexpr int kItemCost = 2;    // units of a run that an item takes beside its tiles: its queries' and outputs' way, 5500 clocks where a tile takes 3100
-constexpr int kTilesLeast = 6;  // units of a run: a part costs as much as a few tiles
+constexpr int kTilesLeast = 6;  // units of a run
+constexpr int kSnap = 1, kSnapShare = 32;  // units, or a share of a run, that a run's end may move to an item's edge (up to 4 units: 500 after 8192 78 -> 84 us)
 
 struct alignas(64) Maps { CUtensorMap q, k, v, o; };
 
@@ -39,6 +41,7 @@ struct TcPlan {
   Cut* cuts;     // [CTAs], or NULL: items stay whole
   uint32_t rows_over, box_rows, part_floats;
   uint32_t tile_tokens;  // tokens of a row tile
+  uint32_t whole;        // no item is long enough to be cut
   uint32_t boxed;        // 32 rows of a tile are a box of the output's map
 };
 
@@ -138,7 +141,7 @@ template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, fl
 struct Piece {
   Segment s;                 // row0: the item's first row; tiles of keys [tile0, tile1)
   unsigned long long item_u;
-  uint32_t tiles;            // of the whole item
+  uint32_t tiles, last;      // of the whole item; the CTA that has its end, where that is cut off here
   uint32_t token, tokens;    // of the request
   uint32_t n[2], n_all;      // how many tiles from tile0 on each row tile sees
   bool cut_begin, cut_end;
@@ -146,14 +149,20 @@ struct Piece {
 struct Walk {
   unsigned long long u, base;  // the next unit; the first unit of the requests' row block b
   uint32_t r, b;
+  bool begun;
 };
 
+// Runs of `per` units, whose boundaries move to an item's edge where that is within `snap` units: a part costs as much as a few tiles.
 struct Runs {
-  unsigned long long u1;
+  unsigned long long u1, per, snap;
   uint32_t rep, rows_over, tokens;  // tokens of an item
   __device__ __forceinline__ uint32_t tiles(const PagedAttn& a, const PagedRequest& q, uint32_t b, uint32_t& skip) const {
     skip = paged_low(q.cached + b * tokens, a.window) / kKeys;
     return (q.cached + min((b + 1) * tokens, q.fresh) - 1) / kKeys + 1 - skip;
+  }
+  // Where a boundary at u of runs lies that falls on an item's units, slot .. stop - 1.
+  __device__ __forceinline__ unsigned long long edge(unsigned long long u, unsigned long long slot, unsigned long long stop) const {
+    return u - slot <= kItemCost + snap ? slot : stop - u <= snap ? stop : u;
   }
   __device__ unsigned long long units(const PagedAttn& a, const PagedRequest& q) const {
     if (q.fresh * rep <= rows_over) return 0;
@@ -172,20 +181,29 @@ struct Runs {
       const unsigned long long all = (unsigned long long)(n + kItemCost) * a.pool.KV;
       if (w.u >= w.base + all) { w.base += all; ++w.b; continue; }
       const uint32_t g = (uint32_t)(w.u - w.base) / (n + kItemCost);  // fewer than 2^32 units in a block of rows: keys / 128 x key heads
-      p.item_u = w.base + (unsigned long long)g * (n + kItemCost) + kItemCost;
-      if (w.u < p.item_u) { w.u = p.item_u; continue; }
-      if (!plan.cuts && w.u != p.item_u) { w.u = p.item_u + n; continue; }  // the CTA before has the whole item
+      const unsigned long long slot = w.base + (unsigned long long)g * (n + kItemCost), stop = slot + kItemCost + n;
+      p.item_u = slot + kItemCost;
+      if (!w.begun) {  // where the run's own beginning lies
+        w.begun = true;
+        w.u = edge(w.u, slot, stop);
+        if (w.u >= stop) continue;
+      }
+      const unsigned long long from = max(w.u, p.item_u), to = u1 >= stop ? stop : edge(u1, slot, stop);
+      if (to <= from) return false;  // the rest is the next CTA's
       p.tiles = n;
       p.s.rq = q; p.s.r = w.r; p.s.g = g;
       p.token = w.b * tokens;
       p.tokens = min(tokens, q.fresh - p.token);
       p.s.row0 = p.token * rep;
       p.s.rows = p.tokens * rep;
-      p.s.tile0 = skip + (uint32_t)(w.u - p.item_u);
-      const unsigned long long end = plan.cuts ? min(u1, p.item_u + n) : p.item_u + n;
-      p.s.tile1 = skip + (uint32_t)(end - p.item_u);
-      p.cut_begin = w.u != p.item_u;
-      p.cut_end = end != p.item_u + n;
+      p.s.tile0 = skip + (uint32_t)(from - p.item_u);
+      p.s.tile1 = skip + (uint32_t)(to - p.item_u);
+      p.cut_begin = from != p.item_u;
+      p.cut_end = to != stop;
+      if (p.cut_end) {  // the CTA that has the item's end: the last boundary inside it that is not moved to its end
+        const unsigned long long k = (stop - 1) / per, moved = (stop - snap + per - 1) / per;  // boundaries before the end; the first within `snap` of it
+        p.last = (uint32_t)(min(k + 1, moved) - 1);
+      }
 #pragma unroll
       for (uint32_t t = 0; t < 2; ++t) {
         p.n[t] = 0;
@@ -195,7 +213,7 @@ struct Runs {
         }
       }
       p.n_all = max(p.n[0], p.n[1]);
-      w.u = end;
+      w.u = to;
       return true;
     }
     return false;
@@ -240,9 +258,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const PagedAttn a, c
   grid_launch_dependents();
 
   // ---- this CTA's run of units (a unit: a tile of keys of an item)
-  Runs runs = {0, a.H / a.pool.KV, plan.rows_over, 2 * plan.tile_tokens};
-  Walk walk = {0, 0, 0, 0};
-  unsigned long long per;
+  Runs runs = {0, 0, 0, a.H / a.pool.KV, plan.rows_over, 2 * plan.tile_tokens};
+  Walk walk = {0, 0, 0, 0, false};
   {
     const uint32_t each = (a.R + kThreads - 1) / kThreads, ra = min(tid * each, a.R), rb = min(ra + each, a.R);
     unsigned long long mine = 0;
@@ -264,9 +281,10 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const PagedAttn a, c
       if (w < warp) before += s_part[w];
       total += s_part[w];
     }
-    per = max((total + gridDim.x - 1) / gridDim.x, (unsigned long long)kTilesLeast);
-    walk.u = per * blockIdx.x;
-    runs.u1 = min(walk.u + per, total);
+    runs.per = max((total + gridDim.x - 1) / gridDim.x, (unsigned long long)kTilesLeast);
+    runs.snap = !plan.cuts ? 1ull << 40 : plan.whole ? kSnap : max((unsigned long long)kSnap, runs.per / kSnapShare);  // without scratch for parts: every item whole
+    walk.u = runs.per * blockIdx.x;
+    runs.u1 = min(walk.u + runs.per, total);
     if (walk.u < runs.u1 && before <= walk.u && walk.u < before + mine) {
       unsigned long long base = before;
       for (uint32_t r = ra; r < rb; ++r) {
@@ -443,7 +461,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const PagedAttn a, c
           Piece p;
           p.tiles = 0;
           more = runs.next(a, plan, walk, p);
-          if (more && p.cut_end && !p.cut_begin) cut = {(uint32_t)((p.item_u + p.tiles - 1) / per), p.s.rq.t0 + p.token, p.tokens, p.s.g};
+          if (more && p.cut_end && !p.cut_begin) cut = {p.last, p.s.rq.t0 + p.token, p.tokens, p.s.g};
           if (i >= kPieces && (s_abort || !mbar_wait(&piece_empty[i % kPieces], (i / kPieces - 1) & 1u))) { s_abort = 1; break; }
           s_piece[i % kPieces] = p;
           mbar_arrive(&piece_full[i % kPieces]);
@@ -727,7 +745,7 @@ cudaError_t launch_chunk(ruai_ctx* c, const PagedAttn& a, const TcPlan& plan, co
   }
   // one CTA per SM: each takes all of tensor memory
   const cudaError_t e = ruai_launch(c, chunk_kernel<T>, dim3(c->sm_count), dim3(kThreads), (size_t)std::max(smem, 120 * 1024), true, a, plan, maps);
-  if (e != cudaSuccess || !plan.cuts) return e;
+  if (e != cudaSuccess || !plan.cuts || plan.whole) return e;
   return ruai_launch(c, join_kernel<T>, dim3(c->sm_count, kItemRows / 32), dim3(kJoinThreads), 0, true, a, plan);
 }
 
@@ -766,6 +784,8 @@ int ruai_paged_attention_tc(ruai_ctx* c, const PagedAttn& a, uint32_t rows_over)
     }
   }
   plan.parts = c->partial;
+  // items of so few tiles are never cut, whatever the runs are (one end or the other is within kSnap): nothing to join
+  plan.whole = (a.most_len + kKeys - 1) / kKeys <= 2 * kSnap + 1;
   plan.cuts = cuts ? reinterpret_cast<Cut*>(reinterpret_cast<unsigned char*>(c->partial) + parts) : nullptr;
   const cudaError_t e = p.dtype == RUAI_F16 ? launch_chunk<__half>(c, a, plan, maps) : launch_chunk<__nv_bfloat16>(c, a, plan, maps);
   if (e != cudaSuccess) { ruai_fail(c, RUAI_ERR_CUDA, "attention over pages: %s", cudaGetErrorString(e)); return -1; }
