@@ -224,7 +224,9 @@ int ruai_paged_append(ruai_ctx* ctx, int x_dtype, const void* x_dev, uint32_t ld
  * and values already: token i of request r sits at position p = cached[r] + i and sees positions p - window + 1 .. p (window 0:
  * 0 .. p).  q [tokens, q_ld] and out [tokens, out_ld] are of the pages' type; rows behind the last token stay as they were.
  * Scores, softmax and sums are f32.  most_fresh and most_len are bounds on a request's new tokens and on its length with them; they
- * choose the kernels, and a request beyond them is left out (reported as above).  H / KV up to 256, H up to 8191. */
+ * choose the kernels, and a request beyond them is left out (reported as above).  H / KV up to 256, H up to 8191.  May be
+ * captured: the graph is replayed in order with the context's stream, as long as the context lives (it uses the context's scratch,
+ * as far as that was allocated by earlier calls). */
 int ruai_paged_attention(ruai_ctx* ctx, int dtype, const void* q_dev, uint32_t q_ld, const void* k_pages_dev, const void* v_pages_dev,
                          uint32_t pages, uint32_t KV, uint32_t page, uint32_t hd, const int32_t* table_dev, uint32_t table_ld,
                          const int32_t* cached_dev, const int32_t* starts_dev, uint32_t R, uint32_t tokens, uint32_t H, float scale,

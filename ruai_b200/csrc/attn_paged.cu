@@ -814,6 +814,11 @@ bool in_pieces(const PagedAttn& a, uint32_t rows) {
 }  // namespace
 
 int ruai_paged_attention_launch(ruai_ctx* c, const PagedAttn& a) {
+  if (!c->scratch_in_graph) {  // parts and counters lie in the context's scratch, whose address a graph keeps
+    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+    RUAI_CUDA(c, cudaStreamIsCapturing(c->stream, &capture));
+    c->scratch_in_graph = capture != cudaStreamCaptureStatusNone;
+  }
   uint32_t rows = a.most_fresh * (a.H / a.pool.KV), rows_most = 0xFFFFFFFFu;  // below 2^31: most_fresh is checked against the tokens
   if (a.pool.dtype == RUAI_F32 ? in_pieces(a, rows) : rows > kRowsAlone) {
     const uint32_t rep = a.H / a.pool.KV, over = a.R > 1 && rep <= kRowsBeside ? kRowsBeside : 0u;

@@ -29,6 +29,8 @@ struct ruai_ctx {
   unsigned long long scratch_epoch = 0;  // counts reallocations of the scratch: captured graphs hold its address
   unsigned* counters = nullptr;
   size_t counters_n = 0;
+  bool scratch_in_graph = false;  // a caller's graph may hold the scratch's address: blocks that it outgrows are kept
+  struct KeptScratch { void* p; size_t counter_bytes; KeptScratch* next; }* kept_scratch = nullptr;
   cudaEvent_t ev0 = nullptr, ev1 = nullptr;
   bool use_pdl = true;  // programmatic dependent launch between consecutive kernels
   bool use_bulk = true; // bulk-copy staged GEMV (gemv_bulk.cu) where the weight allows it

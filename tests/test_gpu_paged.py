@@ -472,3 +472,51 @@ def test_calls_repeat_their_bits(dev):
         s = shapes[i]
         again = attend(dev, np.random.default_rng(i), *s[:5], s[5], 16)[0]
         assert np.array_equal(first[i], again), i
+
+
+# ---- what calls may be ------------------------------------------------------------------------------------------------------
+
+
+@pytest.fixture()
+def capturing(dev):
+    from test_gpu_ops import Capturing
+    c = Capturing()
+    yield c
+    c.close()
+
+
+@pytest.mark.parametrize("warm", [False, True])
+@pytest.mark.parametrize("cached,fresh,H,KV,hd,dtype", [(3000, 1, 8, 2, 128, "bf16"), (900, 200, 4, 1, 128, "bf16"), (2000, 3, 8, 2, 64, "f32"), (10, 400, 8, 2, 64, "f32")])
+def test_attention_in_a_graph_whose_scratch_has_moved(capturing, cached, fresh, H, KV, hd, dtype, warm):
+    """Captured on a fresh context and on one whose scratch has grown for the kernel; replayed with other queries after the scratch has moved."""
+    d, rng = capturing.dev, np.random.default_rng(17)
+    width = ref.up(cached + fresh, 16)
+    (k, kn), (v, vn) = (put(d, rng.normal(size=(width + 1, KV, 16, hd)), dtype) for _ in range(2))
+    (q, qn), on = put(d, rng.normal(size=(fresh, H, hd)), dtype), ref.stored(rng.normal(size=(fresh, H, hd)), dtype)[1]
+    table, lens, starts = rng.permutation(width + 1)[None, :width], np.array([cached]), np.array([0, fresh])
+    args = (k, v, ints(d, table), ints(d, lens), ints(d, starts), fresh, cached + fresh)
+    out, before = put(d, np.full((fresh, H, hd), 7.0), dtype)
+    if warm:
+        nn.paged_attention(q, *args, out=out)
+        d.synchronize()
+    capturing.begin()
+    try:
+        nn.paged_attention(q, *args, out=out)
+    finally:
+        assert capturing.end() == 0
+
+    def replayed(queries):
+        capturing.replay()
+        want, tol = ref.attention(queries, kn, vn, table, lens, starts, hd ** -0.5, 0, dtype)
+        hold(numbers(out), want, tol, before, fresh)
+
+    replayed(qn)
+    # a prompt in f32 whose pieces take more scratch than any call before
+    far, pages = nn.Tensor.from_numpy(d, np.zeros((4000, 8, 128), np.float32)), nn.Tensor.from_numpy(d, np.zeros((500, 8, 16, 128), np.float32))
+    nn.paged_attention(far, pages, pages, ints(d, np.arange(500)[None]), ints(d, [4000]), ints(d, [0, 4000]), 4000, 8000)
+    d.synchronize()
+    changed = ref.stored(on, dtype)[0]
+    d.check(d.L.ruai_memcpy_h2d(d.ctx, q.ptr, changed.ctypes.data_as(C.c_void_p), q.nbytes))
+    replayed(on)
+    for t in (k, v, q, out, far, pages, *args[2:5]):
+        t.free()
