@@ -6,6 +6,7 @@
 // runs; the device's words are taken over from the plan only when the step has ended well.
 #include <algorithm>
 #include <cmath>
+#include <new>
 #include <vector>
 
 #include "decode_ops.cuh"
@@ -157,9 +158,15 @@ RUAI_API int ruai_model_serve_start(ruai_model* m, uint32_t pages, uint32_t page
   if ((unsigned long long)m->Hl * kPlanTokensMax >= (1ull << 31) || m->Hl / m->KVl > 256) return model_fail(m, RUAI_ERR_UNSUPPORTED, "%u heads over %u", m->Hl, m->KVl);
   RUAI_CUDA(c, cudaStreamSynchronize(c->stream));
   serve_destroy(m);
-  Serve* s = new Serve();
+  Serve* s = new (std::nothrow) Serve();
+  if (!s) return model_fail(m, RUAI_ERR_CUDA, "no host memory to serve with");
   s->pages = pages; s->page_log2 = pool.page_log2; s->requests = requests; s->row_pages = request_pages; s->dtype = dtype;
-  const int rc = start(m, s);
+  int rc;
+  try {
+    rc = start(m, s);
+  } catch (const std::bad_alloc&) {
+    rc = model_fail(m, RUAI_ERR_CUDA, "no host memory for %u requests over %u pages", requests, pages);
+  }
   if (rc != RUAI_OK) {
     (void)cudaGetLastError();
     release(s);
@@ -217,7 +224,11 @@ RUAI_API int ruai_model_serve_step(ruai_model* m, const int32_t* fresh, const in
   if (need > s->free) return model_fail(m, RUAI_ERR_SHAPE, "the step needs %u more pages, %u are free", need, s->free);
   RUAI_TRY(reserve(m, s, std::max((uint32_t)T, 1u)));
   if (T) RUAI_TRY(model_activations(m, (uint32_t)T, n_out, 1, 2));
-  s->sent.assign(3 * (size_t)R + T, 0);
+  try {
+    s->sent.assign(3 * (size_t)R + T, 0);
+  } catch (const std::bad_alloc&) {
+    return model_fail(m, RUAI_ERR_CUDA, "no host memory for a step of %llu tokens", T);
+  }
   uint32_t t = 0, o = 0;
   for (uint32_t r = 0; r < R; ++r) {
     s->sent[r] = (int32_t)s->len[r];
