@@ -198,7 +198,8 @@ int ruai_dequant_int4_ref(ruai_ctx* ctx, const int8_t* q_dev, const float* scale
  * request r.  Free pages wait in a ring of `pages` entries; words[0] is the first one's place, words[1] their number.  A page
  * belongs to one request.  All of it lives in device memory, and so do the requests' lengths: nothing here waits for the host.
  * Indices out of range are never followed: what they belong to is left out and the next ruai_ctx_synchronize reports
- * RUAI_ERR_SHAPE.  The reference keeps one contiguous buffer per batch (KvBuf, transformer.rs:10-53). */
+ * RUAI_ERR_SHAPE; a request with such a page in its table has results without meaning, the others theirs.  The reference keeps
+ * one contiguous buffer per batch (KvBuf, transformer.rs:10-53). */
 
 /* Block tables and slots of a step.  Request r < R has cached[r] positions in its pages and brings fresh[r] new tokens
  * (0: none this time; negative: it has ended and its pages go back, to be given out from the next plan on).  Written: the new
@@ -213,17 +214,17 @@ int ruai_page_plan(ruai_ctx* ctx, const int32_t* cached_dev, const int32_t* fres
                    int32_t* words_out_dev, int32_t* starts_dev, int32_t* positions_dev, int32_t* slots_dev);
 /* KvBuf::append and apply_rope (transformer.rs:27-53, functional.rs:197-204) of a step's rows: row t of x [tokens, ld] holds H
  * query heads, KV key heads from column k_off and KV value heads from v_off.  Keys and values go to slots[t] (negative: the row
- * is left out), queries to row t of q_out [tokens, q_ld], all in the pages' type; q_out may be x itself where the types are
- * equal, or NULL.  With rope [max_pos, rot / 2] (cos, sin), elements i and i + rot / 2 of every query and key head turn by the
- * angle of positions[t]; rot a multiple of 8 up to hd.  Computed in f32, rounded once. */
+ * is left out; no two rows have the same slot), queries to row t of q_out [tokens, q_ld], all in the pages' type; q_out may be x
+ * itself where types and rows are equal, lie apart from it, or be NULL.  With rope [max_pos, rot / 2] (cos, sin), elements i and
+ * i + rot / 2 of every query and key head turn by the angle of positions[t]; rot a multiple of 8 up to hd.  Computed in f32, rounded once. */
 int ruai_paged_append(ruai_ctx* ctx, int x_dtype, const void* x_dev, uint32_t ld, uint32_t k_off, uint32_t v_off, uint32_t tokens,
                       uint32_t H, uint32_t rot, const float* rope_dev_or_null, uint32_t max_pos, const int32_t* positions_dev,
                       const int32_t* slots_dev, int dtype, void* k_pages_dev, void* v_pages_dev, uint32_t pages, uint32_t KV,
                       uint32_t page, uint32_t hd, void* q_out_dev_or_null, uint32_t q_ld);
 /* Scaled dot-product attention (functional.rs:264-296) of a step's new tokens over their requests' pages, which hold their keys
  * and values already: token i of request r sits at position p = cached[r] + i and sees positions p - window + 1 .. p (window 0:
- * 0 .. p).  q [tokens, q_ld] and out [tokens, out_ld] are of the pages' type; rows behind the last token stay as they were.
- * Scores, softmax and sums are f32.  most_fresh and most_len are bounds on a request's new tokens and on its length with them; they
+ * 0 .. p).  q [tokens, q_ld] and out [tokens, out_ld] are of the pages' type and lie apart; rows behind the last token
+ * stay as they were.  Scores, softmax and sums are f32.  most_fresh and most_len are bounds on a request's new tokens and on its length with them; they
  * choose the kernels, and a request beyond them is left out (reported as above).  H / KV up to 256, H up to 8191.  May be
  * captured: the graph is replayed in order with the context's stream, as long as the context lives (it uses the context's scratch,
  * as far as that was allocated by earlier calls). */
@@ -386,7 +387,8 @@ int ruai_model_serve_free(const ruai_model* m, uint32_t* free_pages);
  * prompts and single tokens in one step.  logits_host_or_null receives [n, V] and next_ids_host_or_null [n] (greedy, the
  * last maximum), for the n requests with new tokens, in their order, after the last of them.  What does not fit (pages, a
  * request's pages, the model's positions) is refused before anything runs, and a step that fails leaves the requests as they
- * were before it. */
+ * were before it.  A decode step without ids goes on from the last step's argmax, this one's too: give it its ids after a serve
+ * step. */
 int ruai_model_serve_step(ruai_model* m, const int32_t* fresh_host, const int32_t* ids_host, float* logits_host_or_null,
                           int32_t* next_ids_host_or_null);
 

@@ -97,7 +97,7 @@ __global__ void __launch_bounds__(1024) plan_kernel(const PlanArgs a) {
   }
   if (tid == 0) { s_n[a.R] = total[0]; s_need[a.R] = total[1]; s_back[a.R] = total[2]; }
   const uint32_t missing = total[1] > free ? total[1] - free : 0u;
-  bad = bad || first >= a.pages || free > a.pages || total[0] > a.tokens || (!missing && free - total[1] + total[2] > a.pages);
+  bad = bad || first >= a.pages || free > a.pages || total[0] > a.tokens || (free <= a.pages && total[2] > a.pages - free);  // pages go back behind all that are free, given out in this step or not
   const bool ok = !bad && !missing;
   __syncthreads();
   const uint32_t step = gridDim.x * blockDim.x, me = blockIdx.x * blockDim.x + tid;
@@ -296,9 +296,11 @@ RUAI_API int ruai_paged_append(ruai_ctx* c, int x_dtype, const void* x, uint32_t
   if (!known(x_dtype)) return ruai_fail(c, RUAI_ERR_ARG, "ruai_paged_append: unknown type %d of x", x_dtype);
   if (rope && (!rot || rot % 8 || rot > hd || !max_pos))
     return ruai_fail(c, RUAI_ERR_SHAPE, "ruai_paged_append: rotation of %u of %u over %u positions: a multiple of 8", rot, hd, max_pos);
+  if (tokens && q_out == x && (x_dtype != dtype || q_ld != ld)) return ruai_fail(c, RUAI_ERR_ARG, "ruai_paged_append: queries may take the place of x's only in its own type and rows");
   if (ld % 4 || k_off % 4 || v_off % 4 || (q_out && q_ld % 4) || !aligned(x, 4 * bytes_of(x_dtype)) || (q_out && !aligned(q_out, 4 * bytes_of(dtype))) || !aligned(rope, 16))
     return ruai_fail(c, RUAI_ERR_ARG, "ruai_paged_append: rows and heads must start on boundaries of four elements, the rotations on one of 16 bytes");
   const unsigned long long wide = (unsigned long long)H * hd, kv = (unsigned long long)KV * hd;
+  if (wide >= (1ull << 31) || kv >= (1ull << 30)) return ruai_fail(c, RUAI_ERR_SHAPE, "ruai_paged_append: %u and twice %u heads of %u", H, KV, hd);
   if (ld < k_off + kv || ld < v_off + kv || (q_out && (ld < wide || q_ld < wide)))
     return ruai_fail(c, RUAI_ERR_SHAPE, "ruai_paged_append: rows of %u (queries %u) do not hold %u and twice %u heads of %u", ld, q_ld, H, KV, hd);
   if (tokens > 0x7FFFFFFFu) return ruai_fail(c, RUAI_ERR_SHAPE, "ruai_paged_append: %u tokens", tokens);
@@ -319,6 +321,7 @@ RUAI_API int ruai_paged_attention(ruai_ctx* c, int dtype, const void* q, uint32_
   const uint32_t four = 16 / bytes_of(dtype);
   if (q_ld % four || out_ld % four || !aligned(q, 16) || !aligned(out, 16))
     return ruai_fail(c, RUAI_ERR_ARG, "ruai_paged_attention: rows of q and out must start on 16-byte boundaries");
+  if (R && tokens && most_fresh && q == out) return ruai_fail(c, RUAI_ERR_ARG, "ruai_paged_attention: out must lie apart from q");
   if ((unsigned long long)H * hd > q_ld || (unsigned long long)H * hd > out_ld)
     return ruai_fail(c, RUAI_ERR_SHAPE, "ruai_paged_attention: rows of %u and %u do not hold %u heads of %u", q_ld, out_ld, H, hd);
   if (!table_ld || R > kPlanRowsMax || tokens > kPlanTokensMax)

@@ -477,6 +477,27 @@ def test_calls_repeat_their_bits(dev):
 # ---- what calls may be ------------------------------------------------------------------------------------------------------
 
 
+def test_plan_refuses_more_pages_back_than_there_is_room_for(dev):
+    """Free pages and those that come back are more than the ring holds: refused, whatever is given out in the same step."""
+    table, ring = np.array([[0, 1, 2, 3], [4, 5, -1, -1]]), np.arange(10)
+    got = run_plan(dev, [64, 16], [-1, 17], table, ring, [0, 7, 0], 16, 20)
+    with pytest.raises(nn.RuaiError, match="page plan was refused"):
+        dev.synchronize()
+    assert np.array_equal(got[0], table) and np.array_equal(got[1], ring) and got[5].tolist() == [0, 7, 0]
+
+
+def test_entry_points_refuse_overlaps_and_widths(dev):
+    t = nn.Tensor.from_numpy(dev, np.zeros(4096, np.float32))
+    L, p = dev.L, t.ptr
+    append = dict(xd=nn.F32, x=p, ld=48, k=16, v=32, tokens=1, H=1, rot=16, rope=None, most=0, pos=None, slots=p, d=nn.F32, kp=p, vp=p, pages=1, KV=1, page=16, hd=16, q=None, q_ld=0)
+    for change in (dict(q=p, q_ld=16), dict(q=p, q_ld=48, d=nn.F16), dict(H=2**32 - 1), dict(H=2**28)):
+        assert L.ruai_paged_append(dev.ctx, *{**append, **change}.values()) in (1, 6), change
+    with pytest.raises(nn.RuaiError, match="apart"):
+        q, pages = (nn.Tensor.from_numpy(dev, np.zeros(n, np.float32)) for n in ((1, 1, 16), (1, 1, 16, 16)))
+        nn.paged_attention(q, pages, pages, ints(dev, [[0]]), ints(dev, [0]), ints(dev, [0, 1]), 1, 1, out=q)
+    dev.synchronize()
+
+
 @pytest.fixture()
 def capturing(dev):
     from test_gpu_ops import Capturing
