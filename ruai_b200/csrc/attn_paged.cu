@@ -5,6 +5,8 @@
 // query head) pairs of one request and key head, 16 WR of them, so that a cached row is read once for all query heads of its key
 // head.  HBM bounds it; an item's keys pass through once, in tiles of TK, with a running maximum m, sum l and weighted values o per row:
 // o <- o 2^(m - m') + 2^(s - m') v, in f32 registers.
+// 64 requests of 64 to 4096 positions (32 heads of 128, 8 of keys, bf16; 610 MB): 105 us, 5.8 TB/s; one of 32000: 37 us, 3.5 TB/s (the parts' way through
+// scratch and its join are latency); 24 drafts of five tokens in f32 (124 MB): 36 us, the splitting of operands.
 //   Split: the tiles of all items, in a row, are cut into equal runs, one per CTA, whatever the requests' lengths are (they are known to the
 // device only).  An item cut by a run's end leaves (m, l, o) of its part in scratch, and the CTA that arrives last joins the parts, in
 // their order: the same bits every time.

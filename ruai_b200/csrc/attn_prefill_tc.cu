@@ -17,7 +17,8 @@
 // transposed), so that a tile is one bulk copy for each of the query tiles that see it.
 //
 // PAGED: the same for requests of different lengths over pages (paged.cuh; b is a request, its keys and values come through its block table,
-// and it may see a window of them only).  A request with few rows is left to attn_paged.cu.
+// and it may see a window of them only).  A request with few rows is left to attn_paged.cu.  A prompt of 1000
+// (32 heads of 64, 4 of keys): 57 us with the split, 222 in attn_paged.cu.
 //
 // attn_tc_kernel: a CTA owns 128 rows (queries x the query heads of a KV head).  One thread copies tiles, one issues
 // the MMAs (scores of tile t + 1 ahead of the values of tile t), and 4 CS warps are the softmax: thread = row and a CS-th of the
