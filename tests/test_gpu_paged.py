@@ -541,3 +541,14 @@ def test_attention_in_a_graph_whose_scratch_has_moved(capturing, cached, fresh, 
     replayed(on)
     for t in (k, v, q, out, far, pages, *args[2:5]):
         t.free()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("H,KV,hd", [(4, 2, 72), (6, 1, 104), (8, 8, 120), (5, 1, 88), (24, 1, 64), (48, 1, 72), (64, 1, 128), (100, 1, 64), (128, 1, 64), (129, 1, 64), (256, 1, 16)])
+def test_attention_odd_heads_and_many_per_key(dev, H, KV, hd, dtype):
+    """Heads that are no multiple of 16, and as many query heads per key as rows of a tile, fewer and more."""
+    rng = np.random.default_rng(21)
+    for cached, fresh, window in (([130, 0, 33], [1, 1, 1], 0), ([0, 200, 17, 5], [70, 3, 131, 0], 0), ([300], [129], 50)):
+        got, want, tol, before = attend(dev, rng, cached, fresh, H, KV, hd, dtype, 16, window=window)
+        hold(got, want, tol, before, sum(fresh))
+    dev.synchronize()
