@@ -552,3 +552,66 @@ def test_attention_odd_heads_and_many_per_key(dev, H, KV, hd, dtype):
         got, want, tol, before = attend(dev, rng, cached, fresh, H, KV, hd, dtype, 16, window=window)
         hold(got, want, tol, before, sum(fresh))
     dev.synchronize()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("H,KV,hd,cached,fresh", [(8, 2, 64, [700, 3], [1, 1]), (8, 2, 128, [0, 100], [300, 1]), (5, 1, 72, [50], [90])])
+def test_attention_rows_wider_than_the_heads(dev, H, KV, hd, cached, fresh, dtype):
+    """q and out as columns of wider tensors: what lies between the rows is neither read into results nor written."""
+    rng = np.random.default_rng(23)
+    cached, fresh = np.array(cached), np.array(fresh)
+    table, pages = lay_out(rng, cached + fresh, 16)
+    starts = np.concatenate([[0], np.cumsum(fresh)])
+    T, wide = int(starts[-1]), H * hd
+    x = np.full((T, wide + 24), np.nan)
+    x[:, 8:8 + wide] = rng.normal(size=(T, wide))
+    q, qn = put(dev, x, dtype)
+    (k, kn), (v, vn) = (put(dev, rng.normal(size=(pages, KV, 16, hd)), dtype) for _ in range(2))
+    out, _ = put(dev, np.full((T + 1, wide + 40), 7.0), dtype)
+    size, t, c, s = q.np_dtype.itemsize, ints(dev, table), ints(dev, cached), ints(dev, starts)
+    dev.check(dev.L.ruai_paged_attention(dev.ctx, RD[dtype], C.c_void_p(q.ptr.value + 8 * size), wide + 24, k.ptr, v.ptr, pages, KV, 16, hd, t.ptr, table.shape[1], c.ptr, s.ptr, len(cached), T, H,
+                                         hd ** -0.5, 0, int(fresh.max()), int((cached + fresh).max()), C.c_void_p(out.ptr.value + 16 * size), wide + 40))
+    dev.synchronize()
+    got = numbers(out)
+    want, tol = ref.attention(qn[:, 8:8 + wide].reshape(T, H, hd), kn, vn, table, cached, starts, hd ** -0.5, 0, dtype)
+    hold(got[:T, 16:16 + wide].reshape(T, H, hd), want, tol, want[:T], T)
+    got[:T, 16:16 + wide] = 7
+    assert (got == 7).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_two_graphs_of_one_context_in_turn(capturing, dtype):
+    """Two captured calls of other shapes share a workspace; replayed in turn, each gives the bits of its call by itself."""
+    d, rng = capturing.dev, np.random.default_rng(29)
+    calls, want, keep = [], [], []
+    for cached, fresh, H, KV, hd in ((4000, 1, 8, 2, 128), (700, 150, 8, 2, 64)):
+        width = ref.up(cached + fresh, 16)
+        k, v = (put(d, rng.normal(size=(width, KV, 16, hd)), dtype)[0] for _ in range(2))
+        q, out = (put(d, rng.normal(size=(fresh, H, hd)), dtype)[0] for _ in range(2))
+        args = (q, k, v, ints(d, rng.permutation(width)[None]), ints(d, [cached]), ints(d, [0, fresh]), fresh, cached + fresh)
+        nn.paged_attention(*args, out=out)
+        want.append(out.numpy())
+        calls.append((args, out))
+        keep += [k, v, q, out, *args[3:6]]
+    graphs = []
+    for args, out in calls:
+        capturing.begin()
+        try:
+            nn.paged_attention(*args, out=out)
+        finally:
+            assert capturing.end() == 0
+        capturing.replay()
+        graphs.append((capturing.graph, capturing.exec))
+        capturing.graph, capturing.exec = C.c_void_p(), C.c_void_p()
+    for turn in range(6):
+        which = (0, 1, 1, 0, 1, 0)[turn]
+        out = calls[which][1]
+        d.check(d.L.ruai_memcpy_h2d(d.ctx, out.ptr, np.zeros_like(want[which]).ctypes.data_as(C.c_void_p), out.nbytes))
+        assert capturing.cu.cuGraphLaunch(graphs[which][1], capturing.stream) == 0
+        d.synchronize()
+        assert np.array_equal(out.numpy(), want[which]), turn
+    for graph, ex in graphs:
+        capturing.cu.cuGraphExecDestroy(ex)
+        capturing.cu.cuGraphDestroy(graph)
+    for t in keep:
+        t.free()
