@@ -693,7 +693,8 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const PagedAttn a, c
       float4 v[kAhead];
 #pragma unroll
       for (int x = 0; x < kAhead; ++x) {
-        if (i0 + x > cut.last) { mp[x] = -INFINITY; continue; }
+        mp[x] = -INFINITY; lp[x] = 0.0f; v[x] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (i0 + x > cut.last) continue;
         const float* part = part_of(i0 + x);
         mp[x] = part[hd * kItemRows + row];
         lp[x] = part[(hd + 1) * kItemRows + row];
@@ -708,11 +709,9 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const PagedAttn a, c
       m = top;
 #pragma unroll
       for (int x = 0; x < kAhead; ++x) {
-        if (mp[x] != -INFINITY) {
-          const float f = exp2_of(mp[x] - m);
-          l = fmaf(lp[x], f, l);
-          o[0] = fmaf(v[x].x, f, o[0]); o[1] = fmaf(v[x].y, f, o[1]); o[2] = fmaf(v[x].z, f, o[2]); o[3] = fmaf(v[x].w, f, o[3]);
-        }
+        const float f = mp[x] == -INFINITY ? 0.0f : exp2_of(mp[x] - m);  // a part whose every score is NaN has no maximum; its sums are NaN
+        l = fmaf(lp[x], f, l);
+        o[0] = fmaf(v[x].x, f, o[0]); o[1] = fmaf(v[x].y, f, o[1]); o[2] = fmaf(v[x].z, f, o[2]); o[3] = fmaf(v[x].w, f, o[3]);
       }
     }
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;

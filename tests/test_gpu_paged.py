@@ -615,3 +615,44 @@ def test_two_graphs_of_one_context_in_turn(capturing, dtype):
         capturing.cu.cuGraphDestroy(graph)
     for t in keep:
         t.free()
+
+
+def attend_to(dev, q, k, v, table, cached, fresh, dtype, scale, window=0):
+    """One call on these numbers: (what it wrote, what the inputs hold)."""
+    starts = np.concatenate([[0], np.cumsum(fresh)])
+    (q, qn), (k, kn), (v, vn) = (put(dev, x, dtype) for x in (q, k, v))
+    out, _ = put(dev, np.full(qn.shape, 7.0), dtype)
+    nn.paged_attention(q, k, v, ints(dev, table), ints(dev, cached), ints(dev, starts), int(np.max(fresh)), int(np.max(np.add(cached, fresh))), scale=scale, window=window, out=out)
+    return numbers(out), (qn, kn, vn, table, cached, starts, scale, window, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("fresh", [1, 40])
+@pytest.mark.parametrize("what", ["nan query", "inf query", "nan keys", "-inf keys", "inf values", "nan first key"])
+def test_attention_infinities_and_nan_in_parts_of_long_requests(dev, what, fresh, dtype):
+    """A request so long that its keys are shared out: parts without a finite score are not lost where the parts are joined."""
+    rng = np.random.default_rng(fresh)
+    H, KV, hd, cached, page = 8, 2, 64, 2500, 16
+    n = ref.up(cached + fresh, page)
+    q, k, v = (rng.normal(size=s) for s in ((fresh, H, hd), (n, KV, page, hd), (n, KV, page, hd)))
+    table = rng.permutation(n)[None]
+    if what == "nan query":
+        q[fresh // 2, 3] = np.nan
+    if what == "inf query":
+        q[fresh // 2, 3, 5] = np.inf
+    if what == "nan keys":
+        k[table[0, 96:]] = np.nan  # positions 1536 and up
+    if what == "nan first key":
+        k[table[0, 0], 1, 0, 7] = np.nan
+    if what == "-inf keys":  # weigh nothing, whatever their values are
+        q[..., 0], k[table[0, 96:, None], 0, :, 0] = np.abs(q[..., 0]) + 0.1, -np.inf
+        v[table[0, 130], 0] = np.inf
+    if what == "inf values":
+        v[table[0, 100], 1, 3, 9], v[table[0, 20], 0, 3, 9] = np.inf, -np.inf
+    got, args = attend_to(dev, q, k, v, table, np.array([cached]), np.array([fresh]), dtype, hd ** -0.5)
+    dev.synchronize()
+    want, tol = ref.attention(*args)
+    with np.errstate(invalid="ignore"):
+        ok = (np.abs(got - want) <= tol) | (np.isnan(want) & np.isnan(got)) | (got == want)
+    assert ok.all(), (np.argwhere(~ok)[:4].tolist(), (~ok).sum())
+    assert np.isnan(want).any() or "nan" not in what
