@@ -224,7 +224,9 @@ int ruai_paged_append(ruai_ctx* ctx, int x_dtype, const void* x_dev, uint32_t ld
 /* Scaled dot-product attention (functional.rs:264-296) of a step's new tokens over their requests' pages, which hold their keys
  * and values already: token i of request r sits at position p = cached[r] + i and sees positions p - window + 1 .. p (window 0:
  * 0 .. p).  q [tokens, q_ld] and out [tokens, out_ld] are of the pages' type and lie apart; rows behind the last token
- * stay as they were.  Scores, softmax and sums are f32.  most_fresh and most_len are bounds on a request's new tokens and on its length with them; they
+ * stay as they were.  Scores, softmax and sums are f32.  In f16 and bf16 a weight is rounded to the pages' type before it meets its
+ * value (f16: under a power of two, so that weights down to 2^-21 of a row's largest keep all their bits); f32 operands reach the
+ * products as two pieces of 22 bits together.  most_fresh and most_len are bounds on a request's new tokens and on its length with them; they
  * choose the kernels, and a request beyond them is left out (reported as above).  H / KV up to 256, H up to 8191.  May be
  * captured: the graph is replayed in order with the context's stream, as long as the context lives (it uses the context's scratch,
  * as far as that was allocated by earlier calls). */

@@ -536,7 +536,7 @@ __global__ void __launch_bounds__(kThreads, Shape<T, HP, WR>::ONE ? 1 : 2) rows_
         x0 = fmaxf(x0, __shfl_xor_sync(0xFFFFFFFFu, x0, off));
         x1 = fmaxf(x1, __shfl_xor_sync(0xFFFFFFFFu, x1, off));
       }
-      const float n0 = fmaxf(m0, x0), n1 = fmaxf(m1, x1);
+      const float n0 = fmaxf(m0, x0 - weights_up<T>(15.0f)), n1 = fmaxf(m1, x1 - weights_up<T>(15.0f));
       if (__any_sync(0xFFFFFFFFu, n0 > m0 || n1 > m1)) {
         const float c0 = m0 == -INFINITY ? 0.0f : exp2_of(m0 - n0), c1 = m1 == -INFINITY ? 0.0f : exp2_of(m1 - n1);
         l0 *= c0;

@@ -7,7 +7,7 @@
 // for the others; two warpgroups are the softmax, a thread per row.  Scores,
 // probabilities (written over the scores, rounded once to the values' type) and outputs stay in tensor memory: 2 x (128 + 128)
 // columns.  Outputs are rescaled only where a row's maximum has grown by more than 2^8 since the last time: weights of up to 256 are as exact
-// as those of up to 1, and nearly every tile leaves the outputs where they are.
+// as those of up to 1, and nearly every tile leaves the outputs where they are (f16: of up to 2^15, the largest of 2^7 at least: attn_paged.cuh).
 //   Split: the key tiles of all items, in a row, in equal runs, one per CTA, their ends moved to an item's edge where one is near (four
 // prompts of 2000: 175 -> 158 us; one of 2000: 74 -> 64; one of 500 after 8192: 85 -> 78).  An item cut by a run's end leaves (m, l, o) of its parts in
 // scratch, and join_kernel adds them up, many CTAs to an item (the last CTA to arrive alone took 90 us for 17 parts).
@@ -531,7 +531,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const PagedAttn a, c
           for (int z = 0; z < 4; ++z) top[z] = max3(top[z], s[y + z], s[y + z + 4]);
         }
         float mx = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-        mx *= c;  // c > 0
+        mx = fmaf(mx, c, -weights_up<T>(7.0f));  // c > 0
         if (__any_sync(0xFFFFFFFFu, mx > m + kGrowth)) {
           const float m_new = fmaxf(m, mx), f = m == -INFINITY ? 0.0f : exp2_of(m - m_new);
           m = m_new;

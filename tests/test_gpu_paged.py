@@ -656,3 +656,29 @@ def test_attention_infinities_and_nan_in_parts_of_long_requests(dev, what, fresh
         ok = (np.abs(got - want) <= tol) | (np.isnan(want) & np.isnan(got)) | (got == want)
     assert ok.all(), (np.argwhere(~ok)[:4].tolist(), (~ok).sum())
     assert np.isnan(want).any() or "nan" not in what
+
+
+@pytest.mark.parametrize("R,fresh", [(80, 1), (40, 26)])
+@pytest.mark.parametrize("bits", [16, 20, 24])
+@pytest.mark.parametrize("spread", [0.0, 0.3])
+def test_attention_tail_behind_a_key_with_nearly_all_weight(dev, spread, bits, R, fresh):
+    """f16, one key `bits` powers of two above 600 others and without a value: the others are the result, and keep their bits.
+    More requests than the GPU runs at a time, so that the keys of most are not shared out.
+
+    Weights reach the values as f16, the largest as 2^7 at least, so that one is off by half a step, 2^-11 of itself, or by 2^-25 where it is
+    below 2^-14: 2^-32 of the largest.  The scores themselves are off as everywhere (paged_cases.attention)."""
+    rng = np.random.default_rng(bits)
+    KV, hd, cached, page = 4, 64, 600, 16
+    n = ref.up(cached + fresh, page)
+    q, k, v = np.zeros((R * fresh, KV, hd)), np.zeros((R * n, KV, page, hd)), 100 + 20 * rng.normal(size=(R * n, KV, page, hd))
+    q[..., 0], q[..., 1] = 1, 1
+    k[..., 1] = spread * rng.normal(size=(R * n, KV, page))
+    table = rng.permutation(R * n).reshape(R, n)
+    k[table[:, 3], :, 5, 0], k[table[:, 3], :, 5, 1], v[table[:, 3], :, 5] = bits * np.log(2), 0, 0
+    got, args = attend_to(dev, q, k, v, table, np.full(R, cached), np.full(R, fresh), "f16", 1.0)
+    dev.synchronize()
+    want, f32_tol = ref.attention(*args[:-1], "f32")
+    size = np.abs(want)  # the values are positive
+    tail = np.abs(args[2].astype(np.float64))[table].sum((1, 3)).repeat(fresh, 0) * 2.0 ** -32  # the weights' sum is the largest at least
+    tol = f32_tol + size * 2.0 ** -11 + size * 2.0 ** -11 * 1.01 + tail + 2.0 ** -25
+    assert (np.abs(got - want) <= tol).all(), (np.abs(got - want) / size).max()
