@@ -768,7 +768,7 @@ int launch_rows(ruai_ctx* c, const PagedAttn& a, uint32_t rows_most) {
     RUAI_CUDA(c, cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, rows_kernel<T, HP, WR>, kThreads, S::SMEM));
     n = std::max(n, 1);
   }
-  RowsPlan p = {c->partial, c->counters, rows_most, std::min(1u << a.pool.page_log2, (uint32_t)S::TK)};
+  RowsPlan p = {nullptr, nullptr, rows_most, std::min(1u << a.pool.page_log2, (uint32_t)S::TK)};
   Maps maps;
   if (!ruai_tensor_map_fn()) return ruai_fail(c, RUAI_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
   const CUresult rk = encode(&maps.k, a.pool, a.pool.k, p.box_rows), rv = encode(&maps.v, a.pool, a.pool.v, p.box_rows);
@@ -776,6 +776,9 @@ int launch_rows(ruai_ctx* c, const PagedAttn& a, uint32_t rows_most) {
     return ruai_fail(c, RUAI_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d, %d) for %u pages of %u heads of %u", (int)rk, (int)rv, a.pool.pages, a.pool.KV, a.pool.hd);
   // a run per resident CTA, as far as the context's first scratch holds their parts: it never grows for them
   const uint32_t grid = (uint32_t)std::min<size_t>((size_t)c->sm_count * n, kScratchBytes / (2 * S::PART));
+  RUAI_TRY(ruai_ctx_reserve(c, grid * 2 * S::PART, grid));  // it is there, unless an earlier call has run out of memory
+  p.parts = c->partial;
+  p.arrived = c->counters;
   RUAI_CUDA(c, ruai_launch(c, rows_kernel<T, HP, WR>, dim3(grid), dim3(kThreads), S::SMEM, true, a, p, maps));
   return RUAI_OK;
 }

@@ -773,16 +773,12 @@ int ruai_paged_attention_tc(ruai_ctx* c, const PagedAttn& a, uint32_t rows_over)
     return -1;
   }
   // parts of cut items: two per CTA.  Nothing may be allocated while the stream is captured; items then stay whole
-  const size_t parts = 2 * (size_t)c->sm_count * plan.part_floats * sizeof(float), need = parts + c->sm_count * sizeof(Cut), held = c->partial_bytes;
+  const size_t parts = 2 * (size_t)c->sm_count * plan.part_floats * sizeof(float), need = parts + c->sm_count * sizeof(Cut);
   bool cuts = true;
-  if (need > held) {
+  if (need > c->partial_bytes) {
     cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
     if (cudaStreamIsCapturing(c->stream, &capture) != cudaSuccess || capture != cudaStreamCaptureStatusNone) cuts = false;
-    else if (ruai_ctx_reserve(c, need, 0) != RUAI_OK) {  // no memory for the parts: the scratch as it was
-      (void)cudaGetLastError();
-      cuts = false;
-      if (ruai_ctx_reserve(c, held, 0) != RUAI_OK) return -1;
-    }
+    else cuts = ruai_ctx_reserve(c, need, 0) == RUAI_OK;  // no memory for the parts: the scratch as it was
   }
   plan.parts = c->partial;
   // items of so few tiles are never cut, whatever the runs are (one end or the other is within kSnap): nothing to join

@@ -616,14 +616,10 @@ int launch_pieces(ruai_ctx* c, const AttnParams& p, const Paged& pg, uint32_t B,
   if (one > kScratchMost) return 0;
   const uint32_t per = (uint32_t)std::min<size_t>(B, std::min<size_t>(kScratchMost / one, 65535u / p.KV));
   if (!per) return 0;
-  const size_t held = c->partial_bytes;
-  if ((size_t)per * one > held) {
+  if ((size_t)per * one > c->partial_bytes) {
     cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
     if (cudaStreamIsCapturing(c->stream, &capture) != cudaSuccess || capture != cudaStreamCaptureStatusNone) return 0;  // nothing may be allocated
-    if (ruai_ctx_reserve(c, (size_t)per * one, 0) != RUAI_OK) {  // no memory for the pieces: the kernel without them, the scratch as it was
-      (void)cudaGetLastError();
-      return ruai_ctx_reserve(c, held, 0) == RUAI_OK ? 0 : -1;
-    }
+    if (ruai_ctx_reserve(c, (size_t)per * one, 0) != RUAI_OK) return 0;  // no memory for the pieces: the kernel without them
   }
   unsigned char* at = reinterpret_cast<unsigned char*>(c->partial);
   s.k = at; at += up(per * k1);

@@ -11,26 +11,19 @@
 
 #include "../../include/ruai_b200.h"
 #include "../../include/ruai_b200_synth.h"
+#include "scratch.cuh"
 
 #define RUAI_API extern "C" __attribute__((visibility("default")))
 
 // Number of SMs of the target part; grids are sized in multiples of it.
 constexpr int kSmCountB200 = 148;
 
-struct ruai_ctx {
+struct ruai_ctx : Scratch {
   int ordinal = 0;
   cudaStream_t stream = nullptr;
   bool own_stream = false;
   int sm_count = kSmCountB200;
   std::string err;
-  // split-K scratch: partial sums [splits][m][n] and one arrival counter per column tile
-  float* partial = nullptr;
-  size_t partial_bytes = 0;
-  unsigned long long scratch_epoch = 0;  // counts reallocations of the scratch: captured graphs hold its address
-  unsigned* counters = nullptr;
-  size_t counters_n = 0;
-  bool scratch_in_graph = false;  // a caller's graph may hold the scratch's address: blocks that it outgrows are kept
-  struct KeptScratch { void* p; size_t counter_bytes; KeptScratch* next; }* kept_scratch = nullptr;
   cudaEvent_t ev0 = nullptr, ev1 = nullptr;
   bool use_pdl = true;  // programmatic dependent launch between consecutive kernels
   bool use_bulk = true; // bulk-copy staged GEMV (gemv_bulk.cu) where the weight allows it
@@ -109,7 +102,7 @@ cudaError_t ruai_device_malloc(void** out, size_t bytes);
 // each, 9.7 MB), so that it never grows for them.
 constexpr size_t kScratchBytes = 10u << 20;
 
-// Grows the split-K scratch when a launch needs more (never inside a graph capture).
+// Grows the scratch when a launch needs more (never inside a graph capture); after an error it is as it was.
 int ruai_ctx_reserve(ruai_ctx* ctx, size_t partial_bytes, size_t counters);
 
 // ---- launches ---------------------------------------------------------------

@@ -78,13 +78,7 @@ RUAI_API int ruai_ctx_destroy(ruai_ctx* c) {
   DeviceGuard g(c->ordinal);
   cudaStreamSynchronize(c->stream);
   block_pool::detach(c, c->ordinal);  // before its stream goes
-  cudaFree(c->partial);
-  cudaFree(c->counters);
-  while (ruai_ctx::KeptScratch* k = c->kept_scratch) {
-    c->kept_scratch = k->next;
-    cudaFree(k->p);
-    delete k;
-  }
+  scratch::release(*c);
   cudaFree(c->status);
   cudaFree(c->ps_sync);
   cudaFree(c->sample_buf);
@@ -95,38 +89,12 @@ RUAI_API int ruai_ctx_destroy(ruai_ctx* c) {
   return RUAI_OK;
 }
 
-// What the scratch has outgrown: freed, or kept for the graphs that write to it.  (Out of host memory it is left to the process's end.)
-static void outgrown(ruai_ctx* c, void* p, size_t counter_bytes) {
-  if (!p) return;
-  if (!c->scratch_in_graph) {
-    cudaFree(p);
-    return;
-  }
-  if (ruai_ctx::KeptScratch* k = new (std::nothrow) ruai_ctx::KeptScratch{p, counter_bytes, c->kept_scratch}) c->kept_scratch = k;
-}
-
 int ruai_ctx_reserve(ruai_ctx* c, size_t partial_bytes, size_t counters) {
   DeviceGuard g(c->ordinal);
-  if (partial_bytes > c->partial_bytes) {
-    RUAI_CUDA(c, cudaStreamSynchronize(c->stream));
-    outgrown(c, c->partial, 0);
-    c->partial = nullptr;
-    c->partial_bytes = 0;
-    RUAI_CUDA(c, ruai_device_malloc((void**)&c->partial, partial_bytes));
-    c->partial_bytes = partial_bytes;
-    c->scratch_epoch++;
-  }
-  if (counters > c->counters_n) {
-    RUAI_CUDA(c, cudaStreamSynchronize(c->stream));
-    outgrown(c, c->counters, c->counters_n * sizeof(unsigned));
-    c->counters = nullptr;
-    c->counters_n = 0;
-    RUAI_CUDA(c, cudaMalloc(&c->counters, counters * sizeof(unsigned)));
-    RUAI_CUDA(c, cudaMemset(c->counters, 0, counters * sizeof(unsigned)));
-    c->counters_n = counters;
-    c->scratch_epoch++;
-  }
-  return RUAI_OK;
+  const cudaError_t e = scratch::grow(*c, c->stream, partial_bytes, counters);
+  if (e == cudaSuccess) return RUAI_OK;
+  (void)cudaGetLastError();
+  return ruai_fail(c, RUAI_ERR_CUDA, "a scratch of %zu bytes and %zu counters: %s", partial_bytes, counters, cudaGetErrorString(e));
 }
 
 int ruai_ctx_check_status(ruai_ctx* c) {
@@ -139,11 +107,7 @@ int ruai_ctx_check_status(ruai_ctx* c) {
 int ruai_ctx_status_result(ruai_ctx* c, int st) {
   if (st == 0) return RUAI_OK;
   cudaMemsetAsync(c->status, 0, sizeof(int), c->stream);
-  if (st == 3) {  // a launch that gave up may have left some counted
-    cudaMemsetAsync(c->counters, 0, c->counters_n * sizeof(unsigned), c->stream);
-    for (ruai_ctx::KeptScratch* k = c->kept_scratch; k; k = k->next)
-      if (k->counter_bytes) cudaMemsetAsync(k->p, 0, k->counter_bytes, c->stream);
-  }
+  if (st == 3) scratch::clear_counters(*c, c->stream);
   if (c->ps_sync) {  // a persistent launch that gave up leaves its barrier count undefined: start over
     cudaMemsetAsync(c->ps_sync, 0, 64, c->stream);
     c->ps_bar_base = 0;
