@@ -418,8 +418,12 @@ int ensure_cache(ruai_model* m, uint32_t B, uint32_t need) {
 int model_activations(ruai_model* m, uint32_t rows, uint32_t out_rows, uint32_t B, uint32_t T) {
   ruai_ctx* c = m->ctx;
   if (m->hy) return hybrid_reserve(m, rows, out_rows, B, T);
+  // Buffers go before their successors come: the graph that holds their addresses goes first, and after an allocation that failed the
+  // next step, of however few rows, makes all of them anew.
   if (rows > m->act_rows) {
     RUAI_CUDA(c, cudaStreamSynchronize(c->stream));
+    drop_graph(m);
+    m->act_rows = 0;
     const size_t nqkv = (size_t)(m->Hl + 2 * m->KVl) * m->hd;
     RUAI_TRY(m->d_ids.alloc(c, (size_t)rows * sizeof(int32_t)));
     RUAI_TRY(m->x.alloc(c, (size_t)rows * m->d * sizeof(float)));
@@ -436,13 +440,13 @@ int model_activations(ruai_model* m, uint32_t rows, uint32_t out_rows, uint32_t 
       RUAI_CUDA(c, cudaMemsetAsync(m->arg_counter.p, 0, sizeof(unsigned), c->stream));
     }
     m->act_rows = rows;
-    drop_graph(m);
   }
   if (out_rows > m->logit_rows) {
     RUAI_CUDA(c, cudaStreamSynchronize(c->stream));
+    drop_graph(m);
+    m->logit_rows = 0;
     RUAI_TRY(m->logits.alloc(c, (size_t)out_rows * m->Vl * sizeof(float)));
     m->logit_rows = out_rows;
-    drop_graph(m);
   }
   const uint32_t rep = m->Hl / m->KVl;
   const AttnPlan plan = T == 1 ? ruai_attention_plan(c, B, T, m->KVl, rep, m->hd, m->cap) : AttnPlan();
@@ -450,12 +454,12 @@ int model_activations(ruai_model* m, uint32_t rows, uint32_t out_rows, uint32_t 
     const size_t items = (size_t)B * m->KVl, need = items * plan.splits * rep * (m->hd + 4) * sizeof(float), cnt = items * sizeof(unsigned);
     if (need > m->attn_scratch.bytes || cnt > m->attn_counters.bytes) {
       RUAI_CUDA(c, cudaStreamSynchronize(c->stream));
+      drop_graph(m);
       RUAI_TRY(m->attn_scratch.reserve(c, need));
       if (cnt > m->attn_counters.bytes) {
         RUAI_TRY(m->attn_counters.alloc(c, cnt));
         RUAI_CUDA(c, cudaMemsetAsync(m->attn_counters.p, 0, cnt, c->stream));
       }
-      drop_graph(m);
     }
   }
   return RUAI_OK;

@@ -12,7 +12,12 @@ struct DevBuf {
   size_t bytes = 0;
   int alloc(ruai_ctx* c, size_t n) {
     release();
-    RUAI_CUDA(c, ruai_device_malloc((void**)&p, n ? n : 1));
+    const cudaError_t e = ruai_device_malloc((void**)&p, n ? n : 1);
+    if (e != cudaSuccess) {
+      (void)cudaGetLastError();  // not sticky: later launch checks must not see it
+      p = nullptr;
+      return ruai_fail(c, RUAI_ERR_CUDA, "%zu bytes of device memory: %s", n, cudaGetErrorString(e));
+    }
     bytes = n;
     return RUAI_OK;
   }

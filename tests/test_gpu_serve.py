@@ -122,3 +122,30 @@ def test_layer_lists_do_not_serve(dev):
     with pytest.raises(nn.RuaiError, match="serving over pages"):
         m.serve_start(8, 1)
     m.close()
+
+
+def test_a_step_that_memory_does_not_hold_leaves_the_model_usable(dev):
+    """A step whose activations take more than the device has (275 GB, refused at once) ends with an error; smaller steps, the model's own
+    prompts and its decoding steps then answer as before."""
+    m = llama(dev, ff=1 << 18, L=1, positions=1 << 18)
+    ids, prompt = np.arange(20), np.arange(7)
+    want = m.generate(prompt, 6)
+    m.cache_clear()
+    m.serve_start(1100, 2, page=256)
+    a = m.serve_step({0: ids})[1]
+    m.forward_cached(prompt[None])
+    first = [m.decode_step(1) for _ in range(3)]
+    with pytest.raises(nn.RuaiError, match="memory"):
+        m.serve_step({1: np.zeros(1 << 18, np.int32)})
+    assert m.serve_free() == 1099
+    m.cache_clear()
+    m.forward_cached(prompt[None])
+    assert np.array_equal([m.decode_step(1) for _ in range(3)], first)
+    b = m.serve_step({1: ids})[1]
+    assert np.array_equal(a, b)
+    m.cache_clear()
+    with pytest.raises(nn.RuaiError, match="memory"):
+        m.forward_cached(np.zeros((1, 1 << 18), np.int32))
+    m.cache_clear()
+    assert np.array_equal(m.generate(prompt, 6), want)
+    m.close()
