@@ -819,10 +819,10 @@ bool in_pieces(const PagedAttn& a, uint32_t rows) {
 }  // namespace
 
 int ruai_paged_attention_launch(ruai_ctx* c, const PagedAttn& a) {
-  if (!c->scratch_in_graph) {  // parts and counters lie in the context's scratch, whose address a graph keeps
+  if (!c->partial_in_graph || !c->counters_in_graph) {  // parts and counters lie in the context's scratch, whose address a graph keeps
     cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
     RUAI_CUDA(c, cudaStreamIsCapturing(c->stream, &capture));
-    c->scratch_in_graph = capture != cudaStreamCaptureStatusNone;
+    if (capture != cudaStreamCaptureStatusNone) c->partial_in_graph = c->counters_in_graph = true;
   }
   uint32_t rows = a.most_fresh * (a.H / a.pool.KV), rows_most = 0xFFFFFFFFu;  // below 2^31: most_fresh is checked against the tokens
   if (a.pool.dtype == RUAI_F32 ? in_pieces(a, rows) : rows > kRowsAlone) {

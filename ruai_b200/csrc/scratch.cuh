@@ -15,7 +15,7 @@ struct Scratch {
   unsigned* counters = nullptr;
   size_t counters_n = 0;
   unsigned long long scratch_epoch = 0;  // counts the changes of address: captured graphs hold them
-  bool scratch_in_graph = false;  // a caller's graph may hold the scratch's address: blocks that it outgrows are kept
+  bool partial_in_graph = false, counters_in_graph = false;  // a caller's graph may hold the block's address: it is kept when it is outgrown
   struct Kept { void* p; size_t counter_bytes; Kept* next; }* kept_scratch = nullptr;
 };
 
@@ -23,16 +23,18 @@ namespace scratch {
 
 // What the scratch has outgrown, nothing on the stream uses it: freed, or kept for the graphs that write to it.  (Out of host memory it is
 // left to the process's end.)
-inline void outgrown(Scratch& s, void* p, size_t counter_bytes) {
+inline void outgrown(Scratch& s, void* p, size_t counter_bytes, bool in_graph) {
   if (!p) return;
-  if (!s.scratch_in_graph) {
+  if (!in_graph) {
     (void)cudaFree(p);
     return;
   }
   if (Scratch::Kept* k = new (std::nothrow) Scratch::Kept{p, counter_bytes, s.kept_scratch}) s.kept_scratch = k;
 }
 
-// At least these.  After an error the scratch is as it was: the new block is there before the old one goes, and where memory holds
+// At least these; more by half than before, as long as memory holds it, since a new block is a wait for the stream, and a new capture of
+// every model's decoding step: a caller whose sizes rise little by little (a long prompt in chunks) has a few of them, and what graphs keep
+// of outgrown blocks is no more than three times the last.  After an error the scratch is as it was: the new block is there before the old one goes, and where memory holds
 // them one at a time only, the old one comes back.
 inline cudaError_t grow(Scratch& s, cudaStream_t stream, size_t partial_bytes, size_t counters) {
   if (partial_bytes <= s.partial_bytes && counters <= s.counters_n) return cudaSuccess;
@@ -40,14 +42,19 @@ inline cudaError_t grow(Scratch& s, cudaStream_t stream, size_t partial_bytes, s
   if (e != cudaSuccess) return e;
   if (partial_bytes > s.partial_bytes) {
     void* p = nullptr;
-    e = block_pool::device_malloc(&p, partial_bytes);
-    if (e == cudaErrorMemoryAllocation && s.partial && !s.scratch_in_graph) {
+    size_t got = s.partial_bytes + s.partial_bytes / 2;
+    if (got < partial_bytes) got = partial_bytes;
+    e = block_pool::device_malloc(&p, got);
+    if (e == cudaErrorMemoryAllocation && got > partial_bytes) {
+      (void)cudaGetLastError();
+      e = cudaMalloc(&p, got = partial_bytes);
+    }
+    if (e == cudaErrorMemoryAllocation && s.partial && !s.partial_in_graph) {
       (void)cudaGetLastError();
       (void)cudaFree(s.partial);
       s.partial = nullptr;
       s.scratch_epoch++;
-      size_t got = partial_bytes;
-      e = cudaMalloc(&p, partial_bytes);
+      e = cudaMalloc(&p, got = partial_bytes);
       if (e != cudaSuccess) {
         (void)cudaGetLastError();
         got = cudaMalloc(&p, s.partial_bytes) == cudaSuccess ? s.partial_bytes : 0;
@@ -59,14 +66,16 @@ inline cudaError_t grow(Scratch& s, cudaStream_t stream, size_t partial_bytes, s
     } else if (e != cudaSuccess) {
       return e;
     } else {
-      outgrown(s, s.partial, 0);
+      outgrown(s, s.partial, 0, s.partial_in_graph);
       s.partial = static_cast<float*>(p);
-      s.partial_bytes = partial_bytes;
+      s.partial_bytes = got;
+      s.partial_in_graph = false;
       s.scratch_epoch++;
     }
   }
   if (counters > s.counters_n) {
     void* p = nullptr;
+    if (counters < s.counters_n + s.counters_n / 2) counters = s.counters_n + s.counters_n / 2;
     e = cudaMalloc(&p, counters * sizeof(unsigned));
     if (e != cudaSuccess) return e;
     e = cudaMemsetAsync(p, 0, counters * sizeof(unsigned), stream);
@@ -74,9 +83,10 @@ inline cudaError_t grow(Scratch& s, cudaStream_t stream, size_t partial_bytes, s
       (void)cudaFree(p);
       return e;
     }
-    outgrown(s, s.counters, s.counters_n * sizeof(unsigned));
+    outgrown(s, s.counters, s.counters_n * sizeof(unsigned), s.counters_in_graph);
     s.counters = static_cast<unsigned*>(p);
     s.counters_n = counters;
+    s.counters_in_graph = false;
     s.scratch_epoch++;
   }
   return cudaSuccess;

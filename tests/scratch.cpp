@@ -91,7 +91,7 @@ int main(int argc, char** argv) {
       fake::limit = fake::used + 5 * MB;
       CHECK(scratch::grow(s, kStream, 14 * MB, 0) == cudaSuccess && s.sound() && s.partial_bytes == 14 * MB && s.scratch_epoch > epoch);
     } else if (what == "out of memory and kept for a graph") {
-      s.scratch_in_graph = true;
+      s.partial_in_graph = true;
       fake::limit = fake::used + 5 * MB;
       CHECK(scratch::grow(s, kStream, 14 * MB, 0) == cudaErrorMemoryAllocation && s.sound() && s.partial == p && s.scratch_epoch == epoch);
     } else if (what == "out of memory for counters") {
@@ -104,12 +104,30 @@ int main(int argc, char** argv) {
       CHECK(s.sound() && s.partial == p && s.counters == n && s.scratch_epoch == epoch);
       fake::capturing = false;
     } else if (what == "kept for a graph") {
-      s.scratch_in_graph = true;
+      s.partial_in_graph = s.counters_in_graph = true;
       CHECK(scratch::grow(s, kStream, 30 * MB, 9000) == cudaSuccess && s.sound() && s.partial != p && s.counters != n);
       CHECK(fake::has(p, 10 * MB) && fake::has(n, 4096 * sizeof(unsigned)));
       fake::zeroed.clear();
       scratch::clear_counters(s, kStream);
       CHECK(fake::zeroed.size() == 2 && fake::zeroed[(char*)n] == 4096 * sizeof(unsigned) && fake::zeroed[(char*)s.counters] == s.counters_n * sizeof(unsigned));
+    } else if (what == "kept only if captured") {
+      s.partial_in_graph = s.counters_in_graph = true;
+      CHECK(scratch::grow(s, kStream, 30 * MB, 9000) == cudaSuccess);
+      float* const p2 = s.partial;  // no graph has seen these two
+      unsigned* const n2 = s.counters;
+      CHECK(scratch::grow(s, kStream, 90 * MB, 30000) == cudaSuccess && s.sound());
+      CHECK(fake::has(p, 10 * MB) && fake::has(n, 4096 * sizeof(unsigned)) && !fake::has(p2, 1) && !fake::has(n2, 1));
+    } else if (what == "rising little by little") {
+      size_t most = 0;
+      for (size_t want = 11 * MB; want < 300 * MB; want += MB) {
+        s.partial_in_graph = s.counters_in_graph = true;  // captured every time
+        CHECK(scratch::grow(s, kStream, want, want / 4096) == cudaSuccess && s.sound() && s.partial_bytes >= want);
+        most = s.partial_bytes;
+      }
+      CHECK(most <= 450 * MB && s.scratch_epoch - epoch <= 25 && fake::used <= 3 * most + 2 * MB);
+    } else if (what == "half as much again does not fit") {
+      fake::limit = fake::used + 12 * MB;
+      CHECK(scratch::grow(s, kStream, 11 * MB, 0) == cudaSuccess && s.sound() && s.partial_bytes == 11 * MB);
     } else {
       std::printf("no such scenario: %s\n", what.c_str());
       return 1;

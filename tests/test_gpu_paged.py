@@ -682,3 +682,40 @@ def test_attention_tail_behind_a_key_with_nearly_all_weight(dev, spread, bits, R
     tail = np.abs(args[2].astype(np.float64))[table].sum((1, 3)).repeat(fresh, 0) * 2.0 ** -32  # the weights' sum is the largest at least
     tol = f32_tol + size * 2.0 ** -11 + size * 2.0 ** -11 * 1.01 + tail + 2.0 ** -25
     assert (np.abs(got - want) <= tol).all(), (np.abs(got - want) / size).max()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_graphs_captured_between_growths_of_the_scratch(capturing, dtype):
+    """Calls captured one after the other while the scratch grows in between, some of its blocks captured and some not: each replays its bits."""
+    d, rng = capturing.dev, np.random.default_rng(31)
+    cached, fresh, H, KV, hd = 3000, 1, 8, 2, 64
+    width = ref.up(cached + fresh, 16)
+    k, v = (put(d, rng.normal(size=(width, KV, 16, hd)), dtype)[0] for _ in range(2))
+    q, out = (put(d, rng.normal(size=(fresh, H, hd)), dtype)[0] for _ in range(2))
+    args = (q, k, v, ints(d, rng.permutation(width)[None]), ints(d, [cached]), ints(d, [0, fresh]), fresh, cached + fresh)
+    nn.paged_attention(*args, out=out)
+    want, graphs, keep = out.numpy(), [], [k, v, q, out, *args[3:6]]
+    for i, rows in enumerate((700, 1100, 1700, 2600, 4000)):
+        far, pages = nn.Tensor.from_numpy(d, np.zeros((rows, 8, 128), np.float32)), nn.Tensor.from_numpy(d, np.zeros((ref.up(rows, 16), 8, 16, 128), np.float32))
+        nn.paged_attention(far, pages, pages, ints(d, np.arange(ref.up(rows, 16))[None]), ints(d, [0]), ints(d, [0, rows]), rows, rows)
+        d.synchronize()
+        keep += [far, pages]
+        if i % 2 == 0:
+            capturing.begin()
+            try:
+                nn.paged_attention(*args, out=out)
+            finally:
+                assert capturing.end() == 0
+            capturing.replay()
+            graphs.append((capturing.graph, capturing.exec))
+            capturing.graph, capturing.exec = C.c_void_p(), C.c_void_p()
+        for _, ex in graphs:
+            d.check(d.L.ruai_memcpy_h2d(d.ctx, out.ptr, np.zeros_like(want).ctypes.data_as(C.c_void_p), out.nbytes))
+            assert capturing.cu.cuGraphLaunch(ex, capturing.stream) == 0
+            d.synchronize()
+            assert np.array_equal(out.numpy(), want), i
+    for graph, ex in graphs:
+        capturing.cu.cuGraphExecDestroy(ex)
+        capturing.cu.cuGraphDestroy(graph)
+    for t in keep:
+        t.free()
