@@ -819,6 +819,7 @@ bool in_pieces(const PagedAttn& a, uint32_t rows) {
 }  // namespace
 
 int ruai_paged_attention_launch(ruai_ctx* c, const PagedAttn& a) {
+  const ScratchLock held(c->scratch_lock);
   if (!c->partial_in_graph || !c->counters_in_graph) {  // parts and counters lie in the context's scratch, whose address a graph keeps
     cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
     RUAI_CUDA(c, cudaStreamIsCapturing(c->stream, &capture));

@@ -616,6 +616,7 @@ int launch_pieces(ruai_ctx* c, const AttnParams& p, const Paged& pg, uint32_t B,
   if (one > kScratchMost) return 0;
   const uint32_t per = (uint32_t)std::min<size_t>(B, std::min<size_t>(kScratchMost / one, 65535u / p.KV));
   if (!per) return 0;
+  const ScratchLock held(c->scratch_lock);
   if ((size_t)per * one > c->partial_bytes) {
     cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
     if (cudaStreamIsCapturing(c->stream, &capture) != cudaSuccess || capture != cudaStreamCaptureStatusNone) return 0;  // nothing may be allocated

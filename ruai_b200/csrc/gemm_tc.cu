@@ -703,6 +703,7 @@ int ruai_gemm_tc_launch(ruai_ctx* c, const ruai_qweight* w, const void* x, int x
   const uint32_t row_blocks = (m + sh.nt - 1) / sh.nt, col_tiles = (w->n + sh.cb * 128 - 1) / (sh.cb * 128);
   // the split activations and the rows' factors live in the context's scratch
   const size_t xs_bytes = (size_t)row_blocks * stages * pieces * sh.nt * 128;
+  const ScratchLock held(c->scratch_lock);
   RUAI_TRY(ruai_ctx_reserve(c, xs_bytes + (size_t)m * sizeof(float), 0));
   SplitParams sp;
   sp.x = x; sp.x_dtype = x_dtype; sp.pieces = pieces; sp.x_ld = x_ld; sp.m = m; sp.k = w->k; sp.stages = stages; sp.nt = sh.nt;

@@ -511,6 +511,7 @@ int ruai_gemv_wide_launch(ruai_ctx* c, const ruai_qweight* w, const void* x, int
   if (epi.argmax_out && epi.act == ACT_SWIGLU) return ruai_fail(c, RUAI_ERR_UNSUPPORTED, "argmax with the SwiGLU epilogue");
   const uint32_t groups = (w->k + 31) / 32, col_tiles = (w->n + kCols - 1) / kCols;
   // the split activations live in the context's scratch
+  const ScratchLock held(c->scratch_lock);
   RUAI_TRY(ruai_ctx_reserve(c, (size_t)((groups + 1u) & ~1u) * kXsGroupBytes, 0));
   unsigned char* xs = reinterpret_cast<unsigned char*>(c->partial);
   RUAI_CUDA(c, ruai_launch(c, xsplit16_kernel, dim3((((groups + 1u) & ~1u) * 4u * kRows + 255u) / 256u), dim3(256), 0, true, x, x_dtype, x_ld, m, w->k, pro.norm_w, groups, xs));

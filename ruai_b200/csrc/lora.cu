@@ -326,6 +326,7 @@ RUAI_API int ruai_matmul_q_grad_input(ruai_ctx* c, const float* g_dev, const rua
     if (shares < 1) shares = 1;
     const uint32_t cols = (steps + shares - 1) / shares * kGradCols;
     shares = (w->n + cols - 1) / cols;
+    const ScratchLock held(c->scratch_lock);
     float* dst = dx_dev;
     if (shares > 1) {
       RUAI_TRY(ruai_ctx_reserve(c, shares * out_bytes, 0));
@@ -356,6 +357,7 @@ RUAI_API int ruai_linear_lora_forward(ruai_ctx* c, const float* x_dev, const rua
   DeviceGuard g(c->ordinal);
   // the frozen base first (no bias: the reference adds it after the adapter), then the low-rank path into the scratch
   RUAI_TRY(ruai_matmul_q(c, RUAI_F32, x_dev, w, nullptr, out_dev, m));
+  const ScratchLock held(c->scratch_lock);
   RUAI_TRY(ruai_ctx_reserve(c, (size_t)m * rank * sizeof(float), 0));
   float* t = c->partial;
   lora_xa_kernel<<<dim3((m + kXaRows - 1) / kXaRows, (rank + 7) / 8), kThreads, 0, c->stream>>>(x_dev, lora_a_dev, m, w->k, rank, t);

@@ -1120,6 +1120,7 @@ RUAI_API int ruai_model_cache_assume(ruai_model* m, uint32_t B, uint32_t len) {
 static int run_decode_graph(ruai_model* m, uint32_t B) {
   ruai_ctx* c = m->ctx;
   if (pstep_eligible(m, B)) return pstep_run(m, B);
+  const ScratchLock held(c->scratch_lock);  // the graph works in the context's scratch
   if (!m->graph || m->graph_B != B || m->graph_cap != m->cap || m->graph_epoch != c->scratch_epoch) {
     drop_graph(m);
     // split-K partials of one GEMV never exceed (3 * SMs + column tiles) * 256 floats per row;

@@ -1666,6 +1666,7 @@ RUAI_API int ruai_matmul_q_stream(ruai_ctx* c, const float* x_dev, const ruai_qw
     const int rc = ruai_sweight_create(c, w, w->stream);
     if (rc != RUAI_OK) { delete w->stream; w->stream = nullptr; return rc; }
   }
+  const ScratchLock held(c->scratch_lock);
   if (!c->ps_sync) {
     RUAI_CUDA(c, cudaMalloc(&c->ps_sync, 64));
     RUAI_CUDA(c, cudaMemsetAsync(c->ps_sync, 0, 64, c->stream));

@@ -100,6 +100,7 @@ int ruai_sample_device(ruai_ctx* c, const float* logits_dev, uint32_t vocab, flo
   RUAI_CUDA(c, cub::DeviceRadixSort::SortKeys(nullptr, temp_bytes, nullkeys, nullkeys, (int)vocab, 0, 64, c->stream));
   const size_t keys_bytes = ((size_t)vocab * 8 + 255) & ~(size_t)255, probs_bytes = ((size_t)vocab * 4 + 255) & ~(size_t)255;
   const size_t need = 2 * keys_bytes + probs_bytes + temp_bytes;
+  const ScratchLock held(c->scratch_lock);
   if (need > c->sample_bytes) {
     RUAI_CUDA(c, cudaStreamSynchronize(c->stream));
     cudaFree(c->sample_buf);

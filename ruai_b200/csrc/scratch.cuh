@@ -5,11 +5,15 @@
 #include <cuda_runtime_api.h>
 
 #include <cstddef>
+#include <mutex>
 #include <new>
 
 #include "block_pool.cuh"
 
 struct Scratch {
+  // Held from the reading of an address (or the growth) to the last launch that uses what it found: threads that step models of one
+  // context share its stream too, and neither a block that goes nor another thread's launches may come between.  Taken before block_pool's locks.
+  std::recursive_mutex scratch_lock;
   float* partial = nullptr;
   size_t partial_bytes = 0;
   unsigned* counters = nullptr;
@@ -18,6 +22,8 @@ struct Scratch {
   bool partial_in_graph = false, counters_in_graph = false;  // a caller's graph may hold the block's address: it is kept when it is outgrown
   struct Kept { void* p; size_t counter_bytes; Kept* next; }* kept_scratch = nullptr;
 };
+
+using ScratchLock = std::lock_guard<std::recursive_mutex>;
 
 namespace scratch {
 
@@ -37,6 +43,7 @@ inline void outgrown(Scratch& s, void* p, size_t counter_bytes, bool in_graph) {
 // of outgrown blocks is no more than three times the last.  After an error the scratch is as it was: the new block is there before the old one goes, and where memory holds
 // them one at a time only, the old one comes back.
 inline cudaError_t grow(Scratch& s, cudaStream_t stream, size_t partial_bytes, size_t counters) {
+  const ScratchLock held(s.scratch_lock);
   if (partial_bytes <= s.partial_bytes && counters <= s.counters_n) return cudaSuccess;
   cudaError_t e = cudaStreamSynchronize(stream);  // fails in a capture, where nothing may be allocated
   if (e != cudaSuccess) return e;
@@ -94,6 +101,7 @@ inline cudaError_t grow(Scratch& s, cudaStream_t stream, size_t partial_bytes, s
 
 // A launch that gave up may have left some counted.
 inline void clear_counters(Scratch& s, cudaStream_t stream) {
+  const ScratchLock held(s.scratch_lock);
   if (s.counters) (void)cudaMemsetAsync(s.counters, 0, s.counters_n * sizeof(unsigned), stream);
   for (Scratch::Kept* k = s.kept_scratch; k; k = k->next)
     if (k->counter_bytes) (void)cudaMemsetAsync(k->p, 0, k->counter_bytes, stream);

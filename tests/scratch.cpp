@@ -1,11 +1,12 @@
 // Runs scratch.cuh against a stand-in for the CUDA runtime: addresses without memory behind them, a limit, and streams that can be
 // capturing.  One scenario per run; exit status 0: it held.
+#include <chrono>
 #include <cstdio>
 #include <cstdlib>
 #include <map>
 #include <mutex>
-#include <set>
 #include <string>
+#include <thread>
 
 #include "../ruai_b200/csrc/scratch.cuh"
 
@@ -128,6 +129,18 @@ int main(int argc, char** argv) {
     } else if (what == "half as much again does not fit") {
       fake::limit = fake::used + 12 * MB;
       CHECK(scratch::grow(s, kStream, 11 * MB, 0) == cudaSuccess && s.sound() && s.partial_bytes == 11 * MB);
+    } else if (what == "held by another thread") {
+      std::thread other;
+      {
+        const ScratchLock held(s.scratch_lock);
+        CHECK(scratch::grow(s, kStream, 12 * MB, 0) == cudaSuccess);  // by the one that holds it, at once
+        float* const p2 = s.partial;
+        other = std::thread([&] { CHECK(scratch::grow(s, kStream, 60 * MB, 9000) == cudaSuccess); });
+        std::this_thread::sleep_for(std::chrono::milliseconds(100));
+        CHECK(s.partial == p2 && s.counters == n && fake::has(p2, 12 * MB) && s.sound());
+      }
+      other.join();
+      CHECK(s.sound() && s.partial_bytes >= 60 * MB && s.counters_n >= 9000);
     } else {
       std::printf("no such scenario: %s\n", what.c_str());
       return 1;

@@ -149,3 +149,49 @@ def test_a_step_that_memory_does_not_hold_leaves_the_model_usable(dev):
     m.cache_clear()
     assert np.array_equal(m.generate(prompt, 6), want)
     m.close()
+
+
+def test_models_of_one_context_serve_in_threads(dev):
+    """Chunks and single tokens in f32, f16 and bf16, a model per thread, on a context whose scratch grows meanwhile: the bits of each by itself."""
+    import threading
+    kinds = [(llama, nn.F32), (llama, nn.BF16), (MODELS["llama int4 hd 128"], nn.F16), (MODELS["llama int4 hd 128"], nn.BF16), (gpt2, nn.F32), (gpt2, nn.F16)]
+
+    def steps(m, dtype, i):
+        rng, out = np.random.default_rng(i), []
+        for turn in range(6):
+            m.serve_start(60, 3, page=16, dtype=dtype)
+            n = 60 + 50 * turn
+            for new in ({0: n, 1: 7}, {0: 1, 1: 1}, {1: 90, 2: 3}, {0: 1, 1: 1, 2: 1}):
+                _, logits, nxt = m.serve_step({r: rng.integers(0, 500, t) for r, t in new.items()})
+                out += [logits, nxt]
+        return out
+
+    def made(d):
+        return [(make(d), dtype) for make, dtype in kinds]
+
+    alone_ones, want = made(dev), []
+    for i, (m, dtype) in enumerate(alone_ones):
+        want.append(steps(m, dtype, i))
+        m.close()
+    other = nn.Device(0)
+    models, got, errors = made(other), [None] * len(kinds), []
+    begin = threading.Barrier(len(kinds))
+
+    def work(i):
+        try:
+            begin.wait()
+            got[i] = steps(*models[i], i)
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(models))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    for i, (a, b) in enumerate(zip(got, want)):
+        assert all(np.array_equal(x, y) for x, y in zip(a, b)), i
+    for m, _ in models:
+        m.close()
+    nn._lib.check(other.L.ruai_ctx_destroy(other.ctx))
