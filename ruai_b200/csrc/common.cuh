@@ -18,12 +18,11 @@
 // Number of SMs of the target part; grids are sized in multiples of it.
 constexpr int kSmCountB200 = 148;
 
-struct ruai_ctx : Scratch {
+struct CtxState {
   int ordinal = 0;
   cudaStream_t stream = nullptr;
   bool own_stream = false;
   int sm_count = kSmCountB200;
-  std::string err;
   cudaEvent_t ev0 = nullptr, ev1 = nullptr;
   bool use_pdl = true;  // programmatic dependent launch between consecutive kernels
   bool use_bulk = true; // bulk-copy staged GEMV (gemv_bulk.cu) where the weight allows it
@@ -43,6 +42,9 @@ struct ruai_ctx : Scratch {
   // sampler scratch (sample.cu): sort keys, probabilities, the sort's temporary storage
   void* sample_buf = nullptr;
   size_t sample_bytes = 0;
+};
+struct ruai_ctx : Scratch, CtxState {
+  std::string err;
 };
 
 enum QLayout : uint32_t {

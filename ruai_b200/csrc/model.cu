@@ -1136,15 +1136,36 @@ static int run_decode_graph(ruai_model* m, uint32_t B) {
         if (w) need = std::max(need, ruai_gemv_xs_bytes(w, B));
     RUAI_TRY(ruai_ctx_reserve(c, need, tiles * ((B + 15) / 16) + 16));
     }
-    RUAI_CUDA(c, cudaStreamSynchronize(c->stream));
-    const unsigned long long before = c->launches;
+    // Captured on a stream of its own, through the context as it is but for that: what other threads put on the context's stream
+    // meanwhile stays out of the graph, and their waits for it do not end the capture.
+    ruai_ctx on;
+    static_cast<CtxState&>(on) = *c;
+    on.partial = c->partial; on.partial_bytes = c->partial_bytes; on.counters = c->counters; on.counters_n = c->counters_n;
+    on.launches = 0;
+    RUAI_CUDA(c, cudaStreamCreateWithFlags(&on.stream, cudaStreamNonBlocking));
+    if (!block_pool::attach(&on, on.ordinal, on.stream)) {  // nobody waits for the whole device meanwhile
+      cudaStreamDestroy(on.stream);
+      return model_fail(m, RUAI_ERR_CUDA, "no host memory to capture with");
+    }
     cudaGraph_t gr = nullptr;
-    RUAI_CUDA(c, cudaStreamBeginCapture(c->stream, cudaStreamCaptureModeThreadLocal));
-    int rc = issue_step(m, B, 1, HeadRows(), true);
-    cudaError_t e = cudaStreamEndCapture(c->stream, &gr);
-    if (rc != RUAI_OK) { if (gr) cudaGraphDestroy(gr); return rc; }
+    int rc = RUAI_OK;
+    cudaError_t e = cudaStreamBeginCapture(on.stream, cudaStreamCaptureModeThreadLocal);
+    if (e == cudaSuccess) {
+      m->ctx = &on;
+      rc = issue_step(m, B, 1, HeadRows(), true);
+      m->ctx = c;
+      e = cudaStreamEndCapture(on.stream, &gr);
+    }
+    block_pool::detach(&on, on.ordinal);
+    cudaStreamDestroy(on.stream);
+    c->launches += on.launches;
+    c->trace_seq = on.trace_seq;
+    if (rc != RUAI_OK) {
+      if (gr) cudaGraphDestroy(gr);
+      return ruai_fail(c, rc, "%s", on.err.c_str());
+    }
     if (e != cudaSuccess) return model_fail(m, RUAI_ERR_CUDA, "graph capture failed: %s", cudaGetErrorString(e));
-    m->graph_launches = (uint32_t)(c->launches - before);
+    m->graph_launches = (uint32_t)on.launches;
     e = cudaGraphInstantiate(&m->graph, gr, 0);
     cudaGraphDestroy(gr);
     if (e != cudaSuccess) { m->graph = nullptr; return model_fail(m, RUAI_ERR_CUDA, "graph instantiate failed: %s", cudaGetErrorString(e)); }

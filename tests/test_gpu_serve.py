@@ -153,7 +153,6 @@ def test_a_step_that_memory_does_not_hold_leaves_the_model_usable(dev):
 
 def test_models_of_one_context_serve_in_threads(dev):
     """Chunks and single tokens in f32, f16 and bf16, a model per thread, on a context whose scratch grows meanwhile: the bits of each by itself."""
-    import threading
     kinds = [(llama, nn.F32), (llama, nn.BF16), (MODELS["llama int4 hd 128"], nn.F16), (MODELS["llama int4 hd 128"], nn.BF16), (gpt2, nn.F32), (gpt2, nn.F16)]
 
     def steps(m, dtype, i):
@@ -169,13 +168,19 @@ def test_models_of_one_context_serve_in_threads(dev):
     def made(d):
         return [(make(d), dtype) for make, dtype in kinds]
 
-    alone_ones, want = made(dev), []
-    for i, (m, dtype) in enumerate(alone_ones):
-        want.append(steps(m, dtype, i))
-        m.close()
+    in_threads(dev, made, steps)
+
+
+def in_threads(dev, made, steps):
+    """The results of steps(*one, number) for each of made(device), by itself and in a thread each on a context of their own."""
+    import threading
+    want = []
+    for i, one in enumerate(made(dev)):
+        want.append(steps(*one, i))
+        one[0].close()
     other = nn.Device(0)
-    models, got, errors = made(other), [None] * len(kinds), []
-    begin = threading.Barrier(len(kinds))
+    models, errors = made(other), []
+    got, begin = [None] * len(models), threading.Barrier(len(models))
 
     def work(i):
         try:
@@ -192,6 +197,27 @@ def test_models_of_one_context_serve_in_threads(dev):
     assert not errors, errors
     for i, (a, b) in enumerate(zip(got, want)):
         assert all(np.array_equal(x, y) for x, y in zip(a, b)), i
-    for m, _ in models:
+    for m, *_ in models:
         m.close()
     nn._lib.check(other.L.ruai_ctx_destroy(other.ctx))
+
+
+def test_decoding_steps_are_captured_beside_models_that_serve(dev):
+    """Models that decode batches of changing sizes, each captured anew, while others serve and make the scratch grow: the bits of each by itself."""
+    def steps(m, dtype, i):
+        rng, out = np.random.default_rng(i), []
+        for turn in range(8):
+            if dtype is None:
+                B = 1 + (turn + i) % 5
+                m.cache_clear()
+                out.append(m.forward_cached(rng.integers(0, 500, (B, 9 + 20 * turn))))
+                out += [m.decode_step(B) for _ in range(12)]
+            else:
+                m.serve_start(60, 3, page=16, dtype=dtype)
+                for new in ({0: 40 + 50 * turn, 1: 7}, {0: 1, 1: 1}, {1: 90, 2: 3}):
+                    _, logits, nxt = m.serve_step({r: rng.integers(0, 500, t) for r, t in new.items()})
+                    out += [logits, nxt]
+        return out
+
+    kinds = [(llama, None), (llama, nn.F32), (gpt2, None), (MODELS["llama int4 hd 128"], nn.BF16), (MODELS["llama int4 hd 128"], None), (gpt2, nn.F16)]
+    in_threads(dev, lambda d: [(make(d), dtype) for make, dtype in kinds], steps)
