@@ -808,11 +808,11 @@ constexpr uint32_t kRowsAlone = 24;
 // f32: from 33 rows on whichever is the shorter by the times of both, which go by the pairs of a row and a key here, and there by the splitting
 // of all keys and the longest row of key tiles, which one CTA walks.  us, here | attn_prefill_tc.cu (the same heads): 64 rows of 8 requests of 4000 269 |
 // 245, of 64 of 200 185 | 138, of one of 8000 114 | 263; 48 rows of 32 requests of 1000 271 | 262; 32 rows of 32 requests of 1000 (heads of 64) 58 | 75.
-bool in_pieces(const PagedAttn& a, uint32_t rows) {
+bool in_pieces(const ruai_ctx* c, const PagedAttn& a, uint32_t rows) {
   if (rows <= 32) return false;
   const double len = a.most_len, rep = a.H / a.pool.KV, items = a.pool.KV * ceil(a.tokens * rep / 128.0);
   const double many = ceil((double)(a.tokens > a.R ? a.tokens - a.R : 0) / (a.most_fresh > 1 ? a.most_fresh - 1 : 1));  // requests with as many rows as the most
-  const double here = 10.0 + a.tokens * (double)a.H * len / 36e3, split = std::min(many, (double)a.R) * len * a.pool.KV * a.pool.hd * 16.0 / 3e6, there = split + 15.0 + 2.0 * ceil(len / 64.0) * ceil(items / 148.0);
+  const double here = 10.0 + a.tokens * (double)a.H * len / 36e3, split = std::min(many, (double)a.R) * len * a.pool.KV * a.pool.hd * 16.0 / 3e6, there = split + 15.0 + 2.0 * ceil(len / 64.0) * ceil(items / c->sm_count);
   return there < here;
 }
 
@@ -826,7 +826,7 @@ int ruai_paged_attention_launch(ruai_ctx* c, const PagedAttn& a) {
     if (capture != cudaStreamCaptureStatusNone) c->partial_in_graph = c->counters_in_graph = true;
   }
   uint32_t rows = a.most_fresh * (a.H / a.pool.KV), rows_most = 0xFFFFFFFFu;  // below 2^31: most_fresh is checked against the tokens
-  if (a.pool.dtype == RUAI_F32 ? in_pieces(a, rows) : rows > kRowsAlone) {
+  if (a.pool.dtype == RUAI_F32 ? in_pieces(c, a, rows) : rows > kRowsAlone) {
     const uint32_t rep = a.H / a.pool.KV, over = a.R > 1 && rep <= kRowsBeside ? kRowsBeside : 0u;
     const int took = a.pool.dtype == RUAI_F32 ? ruai_paged_attention_pieces(c, a, over) : ruai_paged_attention_tc(c, a, over);
     if (took < 0) return RUAI_ERR_CUDA;
