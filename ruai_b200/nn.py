@@ -278,7 +278,7 @@ def page_plan(cached, fresh, table, ring, words, page, tokens=None, out=None):
         raise ValueError("cached must be [requests], table [requests, pages] and ring [pages]")
     R, pages, width = cached.shape[0], ring.shape[0], table.shape[1]
     if out is None:
-        if tokens is None:
+        if tokens is None or tokens < 0:
             raise ValueError("page_plan: the step's number of rows is needed where no buffers are given")
         out = PagePlan(Tensor(dev, (R + 1,), np.int32), Tensor(dev, (tokens,), np.int32), Tensor(dev, (tokens,), np.int32), Tensor(dev, (3,), np.int32))
     starts, positions, slots, words_out = out
@@ -329,6 +329,8 @@ def paged_attention(q, k_pages, v_pages, table, cached, starts, most_fresh, most
         raise ValueError(f"q must be [tokens, heads, {dim}] of the pages' type, got {list(q.shape)}")
     if len(table.shape) != 2 or len(cached.shape) != 1:
         raise ValueError("cached must be [requests] and table [requests, pages]")
+    if window < 0 or most_fresh < 0 or most_len < 0:
+        raise ValueError(f"window {window}, most_fresh {most_fresh} and most_len {most_len} must not be negative")
     tokens, heads, _ = q.shape
     R, width = cached.shape[0], table.shape[1]
     _ints(dev, "table", table, (R, width))

@@ -88,3 +88,15 @@ def test_restated_attention_sees_the_window_only():
     out, _ = ref.attention(np.zeros((2, 1, 8)), np.zeros((2, 1, 16, 8)), v, np.array([[1, 0]]), [15], [0, 2], 1.0, 3, "f32")
     # positions 15 (last of page 1: values 16..31) and 16 (first of page 0)
     assert np.allclose(out[:, 0, 0], [(29 + 30 + 31) / 3, (30 + 31 + 0) / 3])
+
+
+@pytest.mark.parametrize("change", [dict(window=-1), dict(most_fresh=-1), dict(most_len=-5)])
+def test_attention_refuses_negative_bounds(change):
+    """As unsigned numbers they would be no window, or bounds that every request keeps."""
+    with pytest.raises(ValueError, match="negative"):
+        nn.paged_attention(**{**attention_args(), **change})
+
+
+def test_plan_refuses_a_negative_number_of_rows():
+    with pytest.raises(ValueError, match="number of rows"):
+        nn.page_plan(**{**plan_args(), "out": None, "tokens": -1})
