@@ -719,3 +719,14 @@ def test_graphs_captured_between_growths_of_the_scratch(capturing, dtype):
         capturing.cu.cuGraphDestroy(graph)
     for t in keep:
         t.free()
+
+
+@pytest.mark.parametrize("most_len", [4000, 33000])
+def test_attention_f32_chunks_whose_bound_fills_the_scratch(dev, most_len):
+    """Chunks in f32 with room for so many positions that the pieces of seven requests of the twelve are made at a time, or those of none."""
+    rng = np.random.default_rng(37)
+    cached, fresh = np.full(12, 30), np.ones(12, int)
+    cached[[1, 10]], fresh[[1, 10]] = (500, 61), (130, 129)
+    got, want, tol, before = attend(dev, rng, cached, fresh, 8, 8, 128, "f32", 16, most=(130, most_len))
+    dev.synchronize()
+    hold(got, want, tol, before, int(fresh.sum()))
