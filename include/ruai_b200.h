@@ -16,6 +16,8 @@
  *    asks the driver which it is).
  *  - all work is issued on the context's stream and is asynchronous unless a
  *    host buffer has to be filled.
+ *  - models of one context may be stepped by several threads, each model by
+ *    one at a time; the context's error text is the last failure's.
  *  - matrices are row-major.  Weights are `[in, out]` = `[k, n]` as in the
  *    reference (`Linear::weight`, layers.rs:29).
  *  - there is no CPU fallback: without a CUDA device every call that touches

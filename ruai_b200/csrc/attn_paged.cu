@@ -5,8 +5,9 @@
 // query head) pairs of one request and key head, 16 WR of them, so that a cached row is read once for all query heads of its key
 // head.  HBM bounds it; an item's keys pass through once, in tiles of TK, with a running maximum m, sum l and weighted values o per row:
 // o <- o 2^(m - m') + 2^(s - m') v, in f32 registers.
-// 64 requests of 64 to 4096 positions (32 heads of 128, 8 of keys, bf16; 610 MB): 105 us, 5.8 TB/s; one of 32000: 37 us, 3.5 TB/s (the parts' way through
-// scratch and its join are latency); 24 drafts of five tokens in f32 (124 MB): 36 us, the splitting of operands.
+// 64 requests of 64 to 4096 positions (32 heads of 128, 8 of keys, bf16; 610 MB): 104 us, 5.8 TB/s; one of 32000: 37 us, 3.5 TB/s (the parts' way through
+// scratch and its join are latency); 24 drafts of five tokens in f32 (124 MB): 40 us, the splitting of operands.  (Here and below: inputs
+// that change from call to call.)
 //   Split: the tiles of all items, in a row, are cut into equal runs, one per CTA, whatever the requests' lengths are (they are known to the
 // device only).  An item cut by a run's end leaves (m, l, o) of its part in scratch, and the CTA that arrives last joins the parts, in
 // their order: the same bits every time.
@@ -15,6 +16,8 @@
 // by 8 keys fit few query heads where a tcgen05 tile would be a sixteenth full.  f32 operands are split in two tf32 numbers, x = hi + lo
 // (22 bits), three of the four products; the
 // tensor core's sums truncate, so it adds up 32 elements of a score and a tile's keys only, f32 registers the rest.  In 16 bits the weights are rounded once, to the values' type; l sums them unrounded.
+// (bf16: 1.7e-3 of the outputs' norm off from 64 bits for single tokens, as with unrounded weights, whose outputs round to 1.7e-3; f16 2.2e-4 for 2.1e-4.
+// Two pieces of each weight would double the products of weights and values.)  f16: under a power of two (weights_up).
 //   A row that is not finite at the end is worked out again key by key (row_again): a key that it does not see, or that weighs
 // nothing, must not reach it through 0 x inf.
 #include <cuda.h>
@@ -802,12 +805,13 @@ int launch_type(ruai_ctx* c, const PagedAttn& a, uint32_t rows, uint32_t rows_mo
 
 // A step whose requests all have few rows stays on the kernel here; else it keeps those of up to kRowsBeside rows.
 constexpr uint32_t kRowsBeside = 16;
-// f16 and bf16: up to 24 rows.  us, here | attn_paged_tc.cu, heads of 128, 8 of keys: 20 rows of 4 requests of 1000 28 | 24, of 32 47 | 47, 24 rows (heads of
-// 64) of 64 requests of 200 12 | 23; 32 rows of 8 requests of 4000 60 | 44, of 64 of 200 44 | 35, of one of 8000 55 | 26; 64 rows of 8 of 4000 110 | 43.
+// f16 and bf16: up to 24 rows.  us, here | attn_paged_tc.cu, heads of 128, 8 of keys: 20 rows of 4 requests of 1000 28 | 24 (a rule by rows alone leaves
+// these 4 us), of 32 47 | 47, 24 rows (heads of 64) of 64 requests of 200 11 | 19; 32 rows of 8 requests of 4000 60 | 44, of 64 of 200 46 | 33, of one of 8000
+// 49 | 27; 64 rows of 8 of 4000 110 | 44.
 constexpr uint32_t kRowsAlone = 24;
 // f32: from 33 rows on whichever is the shorter by the times of both, which go by the pairs of a row and a key here, and there by the splitting
-// of all keys and the longest row of key tiles, which one CTA walks.  us, here | attn_prefill_tc.cu (the same heads): 64 rows of 8 requests of 4000 269 |
-// 245, of 64 of 200 185 | 138, of one of 8000 114 | 263; 48 rows of 32 requests of 1000 271 | 262; 32 rows of 32 requests of 1000 (heads of 64) 58 | 75.
+// of all keys and the longest row of key tiles, which one CTA walks.  us, here | attn_prefill_tc.cu (the same heads): 64 rows of 8 requests of 4000 270 |
+// 246, of 64 of 200 187 | 138, of one of 8000 118 | 265; 48 rows of 32 requests of 1000 272 | 263; 32 rows of 32 requests of 1000 (heads of 64) 60 | 75.
 bool in_pieces(const ruai_ctx* c, const PagedAttn& a, uint32_t rows) {
   if (rows <= 32) return false;
   const double len = a.most_len, rep = a.H / a.pool.KV, items = a.pool.KV * ceil(a.tokens * rep / 128.0);

@@ -8,11 +8,14 @@
 // probabilities (written over the scores, rounded once to the values' type) and outputs stay in tensor memory: 2 x (128 + 128)
 // columns.  Outputs are rescaled only where a row's maximum has grown by more than 2^8 since the last time: weights of up to 256 are as exact
 // as those of up to 1, and nearly every tile leaves the outputs where they are (f16: of up to 2^15, the largest of 2^7 at least: attn_paged.cuh).
-//   Split: the key tiles of all items, in a row, in equal runs, one per CTA, their ends moved to an item's edge where one is near (four
-// prompts of 2000: 175 -> 158 us; one of 2000: 74 -> 64; one of 500 after 8192: 85 -> 78).  An item cut by a run's end leaves (m, l, o) of its parts in
+//   Split: the key tiles of all items, in a row, in equal runs, one per CTA, their ends moved to an item's edge where one is near (us: four
+// prompts of 2000 177 -> 172, one of 2000 64.3 -> 63.6; 500 tokens after 8192 83.5 -> 84.3, 64 after 8192 32.1 -> 33.3).  An item cut by a run's end leaves (m, l, o) of its parts in
 // scratch, and join_kernel adds them up, many CTAs to an item (the last CTA to arrive alone took 90 us for 17 parts).
 //   Bound by the softmax warps (an exponential per pair, scores and weights through tensor memory) beside the MMAs.  32 heads of 128, 8 of keys, bf16:
-// one prompt of 8000 465 us, 1128 TFLOP/s; 2048 tokens after 8192 269 us, 1149 TFLOP/s; four prompts of 2000 157 us, 836 TFLOP/s (short items).
+// one prompt of 8000 530 us, 990 TFLOP/s; 2048 tokens after 8192 311 us, 994 TFLOP/s; four prompts of 2000 172 us, 761 TFLOP/s (short items).  All times:
+// inputs that change from call to call (the same ones again and again: 465, 269 and 157).
+//   Weights in bf16 leave outputs 2.1e-3 to 2.3e-3 of their norm off from 64 bits, unrounded ones 1.7e-3 (f16 2.8e-4 and 2.1e-4): two pieces of each
+// would take half as many products again, and as much packing once more on the softmax warps, which are the bound.
 //   Values of the positions behind a request's end are cleared in shared memory (0 x NaN), and a row that is not finite at the end is worked
 // out again key by key.  Every mbarrier wait is bounded.
 #include <algorithm>
@@ -32,7 +35,7 @@ constexpr uint32_t kOutCol = 256;  // tensor memory: scores of both tiles, then 
 constexpr float kGrowth = 8.0f;
 constexpr int kItemCost = 2;    // units of a run that an item takes beside its tiles: its queries' and outputs' way, 5500 clocks where a tile takes 3100
 constexpr int kTilesLeast = 6;  // units of a run
-constexpr int kSnap = 1, kSnapShare = 32;  // units, or a share of a run, that a run's end may move to an item's edge (up to 4 units: 500 after 8192 78 -> 84 us)
+constexpr int kSnap = 1, kSnapShare = 32;  // units, or a share of a run, that a run's end may move to an item's edge (up to 4 units: 500 after 8192 85 -> 88 us)
 
 struct alignas(64) Maps { CUtensorMap q, k, v, o; };
 
