@@ -39,6 +39,9 @@ struct Pool {  // of a device
   size_t bytes = 0;                        // in clean, in aside and on the way from one to the other
   std::mutex settling;                     // held while blocks are on that way: whoever wants all that is kept waits for them; taken before the lock
   std::map<const void*, cudaStream_t> contexts;
+  // Held for a wait for the device, and by whoever captures work of the library's own: such a wait ends every capture that is under way.
+  // Taken after the two above and a context's scratch_lock.  (Recursive: an allocation inside a capture is an error, not a wait without end.)
+  std::recursive_mutex device_wide;
 };
 struct State {
   std::mutex lock;  // held for bookkeeping, not for a wait or a call that maps or unmaps memory
@@ -85,7 +88,11 @@ inline bool settle(Pool& p) {
     moved.swap(p.aside);
   }
   if (moved.empty()) return true;  // another thread has just waited
-  const bool ok = cudaDeviceSynchronize() == cudaSuccess;
+  bool ok;
+  {
+    std::lock_guard<std::recursive_mutex> wide(p.device_wide);
+    ok = cudaDeviceSynchronize() == cudaSuccess;
+  }
   if (!ok) (void)cudaGetLastError();
   Lock l(state().lock);
   merge(ok ? p.clean : p.aside, moved);
@@ -103,7 +110,10 @@ inline void trim(Pool& p) {
     forget(out);
   }
   if (out.empty()) return;
-  if (cudaDeviceSynchronize() != cudaSuccess) (void)cudaGetLastError();
+  {
+    std::lock_guard<std::recursive_mutex> wide(p.device_wide);
+    if (cudaDeviceSynchronize() != cudaSuccess) (void)cudaGetLastError();
+  }
   for (auto& kv : out)
     for (void* q : kv.second) cudaFree(q);
 }

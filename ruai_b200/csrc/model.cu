@@ -1143,23 +1143,24 @@ static int run_decode_graph(ruai_model* m, uint32_t B) {
     on.partial = c->partial; on.partial_bytes = c->partial_bytes; on.counters = c->counters; on.counters_n = c->counters_n;
     on.launches = 0;
     RUAI_CUDA(c, cudaStreamCreateWithFlags(&on.stream, cudaStreamNonBlocking));
-    if (!block_pool::attach(&on, on.ordinal, on.stream)) {  // nobody waits for the whole device meanwhile
-      cudaStreamDestroy(on.stream);
-      return model_fail(m, RUAI_ERR_CUDA, "no host memory to capture with");
-    }
     cudaGraph_t gr = nullptr;
     int rc = RUAI_OK;
-    cudaError_t e = cudaStreamBeginCapture(on.stream, cudaStreamCaptureModeThreadLocal);
-    if (e == cudaSuccess) {
-      m->ctx = &on;
-      rc = issue_step(m, B, 1, HeadRows(), true);
-      m->ctx = c;
-      e = cudaStreamEndCapture(on.stream, &gr);
+    cudaError_t e;
+    {
+      std::unique_lock<std::recursive_mutex> wide;  // nobody of the library waits for the whole device meanwhile
+      if (block_pool::pooled(c->ordinal)) wide = std::unique_lock<std::recursive_mutex>(block_pool::of(c->ordinal).device_wide);
+      e = cudaStreamBeginCapture(on.stream, cudaStreamCaptureModeThreadLocal);
+      if (e == cudaSuccess) {
+        m->ctx = &on;
+        rc = issue_step(m, B, 1, HeadRows(), true);
+        m->ctx = c;
+        e = cudaStreamEndCapture(on.stream, &gr);
+      }
     }
-    block_pool::detach(&on, on.ordinal);
     cudaStreamDestroy(on.stream);
     c->launches += on.launches;
     c->trace_seq = on.trace_seq;
+    if (rc != RUAI_OK || e != cudaSuccess) (void)cudaGetLastError();  // not sticky: later launch checks must not see it
     if (rc != RUAI_OK) {
       if (gr) cudaGraphDestroy(gr);
       return ruai_fail(c, rc, "%s", on.err.c_str());

@@ -1,5 +1,6 @@
 // Runs scratch.cuh against a stand-in for the CUDA runtime: addresses without memory behind them, a limit, and streams that can be
 // capturing.  One scenario per run; exit status 0: it held.
+#include <atomic>
 #include <chrono>
 #include <cstdio>
 #include <cstdlib>
@@ -21,6 +22,7 @@ std::map<char*, size_t> memory;  // what the driver has handed out
 std::map<char*, size_t> zeroed;
 size_t limit = ~(size_t)0, used = 0;
 bool capturing = false;
+std::atomic<int> device_waits{0};
 char* next = (char*)0x1000000;
 bool has(const void* p, size_t bytes) {
   auto it = memory.find((char*)p);
@@ -53,7 +55,7 @@ cudaError_t cudaMemsetAsync(void* p, int, size_t bytes, cudaStream_t) {
   return cudaSuccess;
 }
 cudaError_t cudaStreamSynchronize(cudaStream_t) { return fake::capturing ? cudaErrorStreamCaptureUnsupported : cudaSuccess; }
-cudaError_t cudaDeviceSynchronize(void) { return cudaSuccess; }
+cudaError_t cudaDeviceSynchronize(void) { ++fake::device_waits; return cudaSuccess; }
 cudaError_t cudaStreamIsCapturing(cudaStream_t, cudaStreamCaptureStatus* st) {
   *st = fake::capturing ? cudaStreamCaptureStatusActive : cudaStreamCaptureStatusNone;
   return cudaSuccess;
@@ -141,6 +143,20 @@ int main(int argc, char** argv) {
       }
       other.join();
       CHECK(s.sound() && s.partial_bytes >= 60 * MB && s.counters_n >= 9000);
+    } else if (what == "no wait for the device during a capture") {
+      CHECK(block_pool::attach(&s, 0, kStream));
+      void* q = nullptr;
+      CHECK(block_pool::allocate(0, 5000, &q) == cudaSuccess && block_pool::give_back(0, kStream, q) == cudaSuccess && fake::device_waits == 0);
+      std::thread other;
+      {
+        const std::lock_guard<std::recursive_mutex> captures(block_pool::of(0).device_wide);
+        other = std::thread([] { CHECK(block_pool::settle(block_pool::of(0))); });
+        std::this_thread::sleep_for(std::chrono::milliseconds(100));
+        CHECK(fake::device_waits == 0);
+      }
+      other.join();
+      CHECK(fake::device_waits == 1);
+      block_pool::detach(&s, 0);
     } else {
       std::printf("no such scenario: %s\n", what.c_str());
       return 1;

@@ -221,3 +221,44 @@ def test_decoding_steps_are_captured_beside_models_that_serve(dev):
 
     kinds = [(llama, None), (llama, nn.F32), (gpt2, None), (MODELS["llama int4 hd 128"], nn.BF16), (MODELS["llama int4 hd 128"], None), (gpt2, nn.F16)]
     in_threads(dev, lambda d: [(make(d), dtype) for make, dtype in kinds], steps)
+
+
+def test_decoding_steps_are_captured_beside_tensors_that_come_and_go(dev):
+    """A thread's tensors, whose blocks are set aside and waited for with the whole device, spoil no capture of another thread."""
+    import threading
+    m, stop, errors = llama(dev), threading.Event(), []
+    x = nn.Tensor.from_numpy(dev, np.ones((4, 2048), np.float32))
+
+    def tensors():
+        try:
+            while not stop.is_set():
+                for n in (100, 5000, 70000):
+                    kept = [nn.Tensor(dev, (n,), np.float32, nn.F32) for _ in range(40)]
+                    for t in kept:
+                        t.free()
+                nn.Tensor.from_numpy(dev, x.numpy()).free()
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    def steps():
+        out = []
+        for turn in range(150):
+            B = 1 + turn % 5
+            m.cache_clear()
+            m.forward_cached(np.full((B, 3), turn % 400))
+            out += [m.decode_step(B).tolist() for _ in range(2)]
+        return out
+
+    want = steps()
+    others = [threading.Thread(target=tensors) for _ in range(3)]
+    for t in others:
+        t.start()
+    try:
+        got = steps()
+    finally:
+        stop.set()
+        for t in others:
+            t.join()
+    assert not errors, errors
+    assert got == want
+    m.close()

@@ -16,7 +16,8 @@ def program(tmp_path_factory):
 
 
 @pytest.mark.parametrize("scenario", ["grows", "out of memory", "out of memory for both", "out of memory and kept for a graph", "out of memory for counters", "in a capture", "kept for a graph", "kept only if captured", "rising little by little",
-                                      "half as much again does not fit", "held by another thread"])
+                                      "half as much again does not fit", "held by another thread",
+                                      "no wait for the device during a capture"])
 def test_scenario(program, scenario):
     r = subprocess.run([program, scenario], capture_output=True, text=True, timeout=60)
     assert r.returncode == 0, r.stdout + r.stderr
