@@ -45,6 +45,7 @@ struct CtxState {
 };
 struct ruai_ctx : Scratch, CtxState {
   std::string err;
+  std::mutex err_lock;  // calls of several threads may fail at once
 };
 
 enum QLayout : uint32_t {

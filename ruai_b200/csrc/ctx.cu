@@ -13,7 +13,10 @@ int ruai_fail(ruai_ctx* ctx, int code, const char* fmt, ...) {
   va_start(ap, fmt);
   vsnprintf(buf, sizeof buf, fmt, ap);
   va_end(ap);
-  if (ctx) ctx->err = buf;
+  if (ctx) {
+    const std::lock_guard<std::mutex> held(ctx->err_lock);
+    ctx->err = buf;
+  }
   g_ruai_global_err = buf;
   return code;
 }
@@ -29,7 +32,13 @@ RUAI_API int ruai_device_count(void) {
   return n;
 }
 
-RUAI_API const char* ruai_last_error(const ruai_ctx* ctx) { return ctx ? ctx->err.c_str() : g_ruai_global_err.c_str(); }
+RUAI_API const char* ruai_last_error(const ruai_ctx* ctx) {
+  if (!ctx) return g_ruai_global_err.c_str();
+  static thread_local std::string text;  // the caller's own: another thread's failure may replace the context's meanwhile
+  const std::lock_guard<std::mutex> held(const_cast<ruai_ctx*>(ctx)->err_lock);
+  text = ctx->err;
+  return text.c_str();
+}
 
 RUAI_API int ruai_ctx_create(int ordinal, void* stream_or_null, ruai_ctx** out) {
   if (!out) return ruai_fail(nullptr, RUAI_ERR_ARG, "ruai_ctx_create: out is NULL");

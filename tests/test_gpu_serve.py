@@ -262,3 +262,26 @@ def test_decoding_steps_are_captured_beside_tensors_that_come_and_go(dev):
     assert not errors, errors
     assert got == want
     m.close()
+
+
+def test_failures_of_several_threads_keep_their_texts(dev):
+    """Refused calls from threads on one context: each thread reads the text of a failure, whole."""
+    import threading
+    import ctypes as C
+    p, texts, errors = C.c_void_p(64), [], []
+
+    def refused(page):
+        try:
+            for _ in range(3000):
+                assert dev.L.ruai_page_plan(dev.ctx, p, p, 1, 1, page, p, 1, p, 1, p, p, p, p, p) != 0
+                texts.append(dev.L.ruai_last_error(dev.ctx))
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=refused, args=(8 + i * 10 ** i,)) for i in range(6)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    assert set(texts) <= {f"ruai_page_plan: pages of {8 + i * 10 ** i}: a power of two from 16 to 256".encode() for i in range(6)}
