@@ -17,7 +17,9 @@
  *  - all work is issued on the context's stream and is asynchronous unless a
  *    host buffer has to be filled.
  *  - models of one context may be stepped by several threads, each model by
- *    one at a time; the context's error text is the last failure's.
+ *    one at a time; the context's error text is the last failure's.  Decoding
+ *    steps are captured into graphs, beside which CUDA allows no thread to wait
+ *    for the whole device: wait for the context instead.
  *  - matrices are row-major.  Weights are `[in, out]` = `[k, n]` as in the
  *    reference (`Linear::weight`, layers.rs:29).
  *  - there is no CPU fallback: without a CUDA device every call that touches

@@ -21,6 +21,7 @@ constexpr int kSmCountB200 = 148;
 struct CtxState {
   int ordinal = 0;
   cudaStream_t stream = nullptr;
+  cudaStream_t capture_stream = nullptr;  // where decoding steps are captured (model.cu); nothing runs on it
   bool own_stream = false;
   int sm_count = kSmCountB200;
   cudaEvent_t ev0 = nullptr, ev1 = nullptr;

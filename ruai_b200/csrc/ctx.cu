@@ -93,6 +93,7 @@ RUAI_API int ruai_ctx_destroy(ruai_ctx* c) {
   cudaFree(c->sample_buf);
   cudaEventDestroy(c->ev0);
   cudaEventDestroy(c->ev1);
+  if (c->capture_stream) cudaStreamDestroy(c->capture_stream);
   if (c->own_stream) cudaStreamDestroy(c->stream);
   delete c;
   return RUAI_OK;

@@ -1138,11 +1138,12 @@ static int run_decode_graph(ruai_model* m, uint32_t B) {
     }
     // Captured on a stream of its own, through the context as it is but for that: what other threads put on the context's stream
     // meanwhile stays out of the graph, and their waits for it do not end the capture.
+    if (!c->capture_stream) RUAI_CUDA(c, cudaStreamCreateWithFlags(&c->capture_stream, cudaStreamNonBlocking));
     ruai_ctx on;
     static_cast<CtxState&>(on) = *c;
     on.partial = c->partial; on.partial_bytes = c->partial_bytes; on.counters = c->counters; on.counters_n = c->counters_n;
     on.launches = 0;
-    RUAI_CUDA(c, cudaStreamCreateWithFlags(&on.stream, cudaStreamNonBlocking));
+    on.stream = c->capture_stream;
     cudaGraph_t gr = nullptr;
     int rc = RUAI_OK;
     cudaError_t e;
@@ -1157,7 +1158,6 @@ static int run_decode_graph(ruai_model* m, uint32_t B) {
         e = cudaStreamEndCapture(on.stream, &gr);
       }
     }
-    cudaStreamDestroy(on.stream);
     c->launches += on.launches;
     c->trace_seq = on.trace_seq;
     if (rc != RUAI_OK || e != cudaSuccess) (void)cudaGetLastError();  // not sticky: later launch checks must not see it
