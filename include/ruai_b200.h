@@ -19,7 +19,9 @@
  *  - models of one context may be stepped by several threads, each model by
  *    one at a time; the context's error text is the last failure's.  Decoding
  *    steps are captured into graphs, beside which CUDA allows no thread to wait
- *    for the whole device: wait for the context instead.
+ *    for the whole device: wait for the context instead.  A graph of the
+ *    caller's own that holds calls of a context is replayed while no other
+ *    thread is in one.
  *  - matrices are row-major.  Weights are `[in, out]` = `[k, n]` as in the
  *    reference (`Linear::weight`, layers.rs:29).
  *  - there is no CPU fallback: without a CUDA device every call that touches
